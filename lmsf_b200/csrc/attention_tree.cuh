@@ -1,0 +1,167 @@
+// Attention of drafted trees: what its kernels share.
+//
+// A request has `prefix_len` cached keys in pages and n drafted nodes whose keys and values are rows of the step's own k and v.
+// A node sees the cached keys (inside its window, if there is one) and the nodes whose bits are set in its mask row.  The rows of
+// one kv head of one request are its nodes x the heads of the group, node-major: row = node * group + head of the group.
+//
+// The work is cut as follows.  A unit is (request, kv head, item of up to kRows rows); it has the request's tiles of kKeys keys: its
+// cached keys first, then the nodes.  All units' tiles in a row, requests in order, are shared out evenly: of G blocks block b
+// takes the tiles [b W / G, (b + 1) W / G) of all W (G no more than W), whatever the lengths are; no plan is made on the host, so a captured launch
+// serves any lengths.  A unit that lies in one block's range is finished there.  Of a unit that is cut every block leaves a
+// partial (unnormalised output, running maximum, sum; float32) in the workspace: at most two for a block, one for the unit that it
+// begins with and one for the unit that it ends with.  A second kernel adds them up in the order of the blocks; both
+// depend only on lengths and G, so the result is the same in every run.
+#pragma once
+#include "common.cuh"
+
+namespace lmsf {
+namespace tree {
+
+constexpr int kMaxSeqs = 4096;             // requests of a step (their work is added up in shared memory)
+
+struct Args {
+  const void* q; long long q_stride;
+  const void* k; long long k_stride;       // drafted tokens' keys [rows][kv heads x head size], values alike
+  const void* v; long long v_stride;
+  void* out; long long out_stride;
+  const void* cache; long long page_stride, v_off; int pages;   // [page][2][kv head][slot][head size], in elements
+  const int* block_table; int max_blocks, block_size;
+  const int* cu_q; const int* prefix_len;
+  const unsigned* mask; int words;
+  const int* positions; int window;        // window > 0: a node at position p sees cached keys > p - window
+  float scale;
+  int n_seqs, n_rows, n_q_heads, n_kv, group, hd;
+  float* partials; int4* notes;            // workspace: two partials and two notes for every block
+};
+
+struct Request { int start, n, nk, prefix, lo, first, n_pre, tiles, items; };
+
+// kKeys keys a tile; an item has `rows` rows.
+template <int kKeys>
+__device__ __forceinline__ Request request(const Args& a, int s, int rows) {
+  Request r;
+  r.start = min(max(a.cu_q[s], 0), a.n_rows);
+  r.n = min(max(a.cu_q[s + 1] - r.start, 0), a.n_rows - r.start);
+  r.nk = min(r.n, 32 * a.words);                                 // a node behind the mask's last bit is seen by nobody
+  r.prefix = (int)min((long long)max(a.prefix_len[s], 0), (long long)a.max_blocks * a.block_size);
+  r.lo = a.window > 0 ? min(max(r.prefix - a.window + 1, 0), r.prefix) : 0;    // a node's position is the prefix or behind it
+  r.first = r.lo / kKeys;
+  r.n_pre = (r.prefix + kKeys - 1) / kKeys - r.first;
+  if (r.lo >= r.prefix) r.n_pre = 0;
+  r.tiles = max(1, r.n_pre + (r.nk + kKeys - 1) / kKeys);        // (rows that see nothing are still written)
+  r.items = (r.n * a.group + rows - 1) / rows;
+  return r;
+}
+
+// offs[s] = tiles before request s, for 0 <= s <= n_seqs; by all threads of the block (a multiple of 32, at most 1024).
+template <int kKeys>
+__device__ __forceinline__ void add_up_work(const Args& a, int rows, int items_per_unit, int* offs, int* scratch) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = blockDim.x >> 5;
+  const int per = (a.n_seqs + blockDim.x - 1) / blockDim.x;
+  const int s0 = min(tid * per, a.n_seqs), s1 = min(s0 + per, a.n_seqs);
+  int sum = 0;
+  for (int s = s0; s < s1; ++s) {
+    const Request r = request<kKeys>(a, s, rows);
+    const int w = r.tiles * ((r.items + items_per_unit - 1) / items_per_unit) * a.n_kv;
+    offs[s] = sum;
+    sum += w;
+  }
+  int x = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  if (lane == 31) scratch[warp] = x;
+  __syncthreads();
+  int base = x - sum;
+  for (int w = 0; w < warp; ++w) base += scratch[w];
+  for (int s = s0; s < s1; ++s) offs[s] += base;
+  if (tid == 0) {
+    int all = 0;
+    for (int w = 0; w < nw; ++w) all += scratch[w];
+    offs[a.n_seqs] = all;
+  }
+  __syncthreads();
+}
+
+// The tiles that this block takes of `work`.  Of fewer tiles than blocks, the first blocks take one each: no block with an empty
+// share stands between the pieces of a unit.
+__device__ __forceinline__ void share_of_block(int work, int& begin, int& end) {
+  const int b = blockIdx.x, blocks = min((int)gridDim.x, work);
+  begin = end = 0;
+  if (b >= blocks) return;
+  begin = (int)((long long)work * b / blocks);
+  end = (int)((long long)work * (b + 1) / blocks);
+}
+
+// The request whose tiles hold place p (0 <= p < offs[n_seqs]).
+__device__ __forceinline__ int request_at(const int* offs, int n_seqs, int p) {
+  int lo = 0, hi = n_seqs;                                       // offs[lo] <= p < offs[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (offs[mid] <= p) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// A block's share of one unit: tiles [t0, t1) of the unit's.
+struct Piece { int s, kvh, item, t0, t1; Request r; };
+template <int kKeys>
+__device__ __forceinline__ Piece piece_at(const Args& a, const int* offs, int rows, int items_per_unit, int p, int end) {
+  Piece x;
+  x.s = request_at(offs, a.n_seqs, p);
+  x.r = request<kKeys>(a, x.s, rows);
+  const int units = (x.r.items + items_per_unit - 1) / items_per_unit, rem = p - offs[x.s], u = rem / x.r.tiles;
+  x.t0 = rem % x.r.tiles;
+  x.t1 = min(x.r.tiles, x.t0 + (end - p));
+  x.kvh = u / units;
+  x.item = (u % units) * items_per_unit;                         // the unit's first item: its neighbours read the same keys
+  return x;
+}
+
+// Note of a partial: x = request, or -1: none; y = kv head; z = first row among the request's rows of that kv head;
+// w = rows | 0x10000 if the unit goes on in the next block.
+constexpr int kGoesOn = 0x10000;
+
+// Adds the partials of the units that were cut: one block row of the grid per block b of the first kernel; it acts if a unit begins
+// in b's last piece and goes on.  Partial p: out [rows][hd], then [rows] maxima (in log2 units), then [rows] sums.
+template <typename T, int kRows>
+__global__ void __launch_bounds__(256) join_kernel(Args a) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int b = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int4 note = a.notes[2 * b + 1];
+  if (note.x < 0 || !(note.w & kGoesOn)) return;
+  const int rows = note.w & 0xffff;
+  const size_t slot_floats = (size_t)kRows * (a.hd + 2);
+  // the unit goes on in the first partials of the blocks behind, up to the one that ends it
+  int last = b + 1;
+  while (last < (int)gridDim.x - 1 && (a.notes[2 * last].w & kGoesOn)) ++last;
+  const int start = min(max(a.cu_q[note.x], 0), a.n_rows);
+  auto slot = [&](int i) { return a.partials + slot_floats * (i == b ? 2 * b + 1 : 2 * i); };
+  for (int row = blockIdx.y * 8 + warp; row < rows; row += gridDim.y * 8) {
+    float m = -INFINITY;
+    for (int i = b + lane; i <= last; i += 32) m = fmaxf(m, slot(i)[(size_t)kRows * a.hd + row]);
+    m = warp_max(m);
+    const float base = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+    for (int i = b + lane; i <= last; i += 32) l += slot(i)[(size_t)kRows * (a.hd + 1) + row] * exp2f(slot(i)[(size_t)kRows * a.hd + row] - base);
+    l = warp_sum(l);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int r = note.z + row, node = r / a.group, head = note.y * a.group + r % a.group;
+    T* out = (T*)a.out + (start + node) * a.out_stride + (size_t)head * a.hd;
+    for (int c = lane; c < a.hd; c += 32) {
+      float sum = 0.f;
+      for (int i = b; i <= last; ++i) {
+        const float* p = slot(i);
+        sum += p[(size_t)row * a.hd + c] * exp2f(p[(size_t)kRows * a.hd + row] - base);
+      }
+      out[c] = from_f32<T>(sum * inv);
+    }
+  }
+}
+
+}  // namespace tree
+}  // namespace lmsf

@@ -417,5 +417,6 @@ class ModelRunner:
             what = {1: "a token id outside the vocabulary reached the embedding",
                     2: "a token was to be cached at a position that has no page",
                     3: "a tensor-core attention block gave up waiting for its own products",
-                    4: "a block of the streaming matrix product gave up waiting for its own copies or products"}.get(code, f"code {code}")
+                    4: "a block of the streaming matrix product gave up waiting for its own copies or products",
+                    5: "a drafted tree is no tree or larger than its buffers, or a row of logits names options that are not there"}.get(code, f"code {code}")
             raise StepError(f"the device reported an error during the step: {what}")

@@ -1,0 +1,100 @@
+"""The refusals of the operators on drafted trees that need no device, and their plain implementations by themselves."""
+import math
+import random
+
+import pytest
+import torch
+
+import plain_tree as P
+from lmsf_b200 import kernels
+from lmsf_b200.kernels import KernelError
+
+I = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
+L = lambda *s: torch.zeros(s, dtype=torch.int64)  # noqa: E731
+F = lambda *s: torch.zeros(s, dtype=torch.float32)  # noqa: E731
+
+
+def layout_args(**kw):
+    a = dict(cu_q=I(3), token_seq=I(9), positions=I(9), slots=L(9), mask=I(9, 2), parents=I(9), tree_len=I(2), prefix_len=I(2),
+             block_table=I(2, 4), block_size=16)
+    a.update(kw)
+    return a
+
+
+@pytest.mark.parametrize("kw", [dict(cu_q=I(2)), dict(token_seq=L(9)), dict(positions=I(8)), dict(slots=I(9)), dict(slots=L(18)[::2]), dict(mask=I(8, 2)),
+                                dict(mask=I(9, 9)), dict(mask=I(9, 0)), dict(mask=I(9)), dict(parents=I(4)), dict(tree_len=I(3)), dict(prefix_len=I(1)),
+                                dict(block_table=I(3, 4)), dict(block_table=I(4)), dict(block_size=0), dict(window=-1), dict(mask=None, window=4),
+                                dict()])
+def test_layout_refuses(kw):
+    """Shapes, types and options; with nothing else wrong, tensors that are on no device."""
+    with pytest.raises(KernelError):
+        kernels.tree_layout(**layout_args(**kw))
+
+
+def attention_args(**kw):
+    a = dict(out=F(9, 64), q=F(9, 64), k=F(9, 32), v=F(9, 32), cache=F(5, 2, 2, 16, 16), block_table=I(2, 4), block_size=16, cu_q=I(3), prefix_len=I(2),
+             mask=I(9, 1), scale=0.25, n_q_heads=4, n_kv_heads=2, head_dim=16)
+    a.update(kw)
+    return a
+
+
+@pytest.mark.parametrize("kw", [dict(out=F(9, 48)), dict(out=F(64, 9).t()), dict(k=F(9, 64)), dict(v=F(8, 32)), dict(cache=F(5, 2, 2, 16, 32)),
+                                dict(cache=F(5, 1, 2, 16, 16)), dict(cache=F(5, 2, 2, 16, 16).transpose(2, 3)), dict(block_size=8), dict(block_table=I(3, 4)),
+                                dict(cu_q=I(2)), dict(cu_q=L(3)), dict(mask=I(9)), dict(mask=I(9, 0)), dict(mask=I(8, 1)), dict(n_q_heads=3),
+                                dict(n_kv_heads=3), dict(window=5), dict(window=-1), dict(window=5, positions=I(8)), dict(scale=math.nan),
+                                dict(q=F(9, 64).half()), dict(v=F(9, 32).bfloat16()), dict(q=F(9, 128)[:, ::2]), dict()])
+def test_attention_refuses(kw):
+    with pytest.raises(KernelError):
+        kernels.attention_tree(**attention_args(**kw))
+
+
+def adjust_args(**kw):
+    a = dict(out=F(6, 40), logits=F(6, 40), row_req=I(6), history=(I(2, 7), I(2), I(2)), penalties=(F(2), F(2), F(2)), tree=(I(6), I(6, 1), I(3)),
+             bias=(I(3), I(5), F(5)), allowed=(I(3, 2), I(6)))
+    a.update(kw)
+    return a
+
+
+@pytest.mark.parametrize("kw", [dict(out=F(6, 41)), dict(logits=F(6, 40).bfloat16()), dict(logits=F(40, 6).t()), dict(logits=F(1, 40).expand(6, 40)), dict(row_req=I(5)),
+                                dict(row_req=None), dict(history=(I(3, 7), I(2), I(2))), dict(history=(L(2, 7), I(2), I(2))), dict(history=(I(2, 7), I(3), I(2))),
+                                dict(penalties=None), dict(penalties=(F(2), F(3), F(2))), dict(tree=(I(5), I(6, 1), I(3))), dict(tree=(I(6), I(6), I(3))),
+                                dict(tree=(I(6), I(6, 1), I(4))), dict(bias=(I(4), I(5), F(5))), dict(bias=(I(3), I(5), F(4))), dict(allowed=(I(3, 1), I(6))),
+                                dict(allowed=(I(2), I(6))), dict(allowed=(I(3, 2), I(3))), dict()])
+def test_adjust_refuses(kw):
+    with pytest.raises(KernelError):
+        kernels.adjust_logits(**adjust_args(**kw))
+
+
+def test_adjust_refuses_a_shifted_self():
+    x = F(13, 40)
+    with pytest.raises(KernelError, match="apart"):
+        kernels.adjust_logits(x[::2][:6], x[:6])
+
+
+def accept_args(**kw):
+    a = dict(n_kept=I(2), path=I(2, 4), next_token=I(2), new_len=I(2), target=I(9), tokens=I(9), parents=I(9), cu_q=I(3), prefix_len=I(2), slots=L(9),
+             k=F(3, 9, 32), v=F(3, 9, 32), cache=F(3, 5, 2, 2, 16, 16))
+    a.update(kw)
+    return a
+
+
+@pytest.mark.parametrize("kw", [dict(n_kept=I(3)), dict(path=I(2)), dict(path=I(2, 0)), dict(path=I(2, 257)), dict(path=I(3, 4)), dict(next_token=L(2)), dict(tokens=I(8)),
+                                dict(parents=I(10)), dict(cu_q=I(2)), dict(slots=None), dict(k=None), dict(cache=None), dict(slots=I(9)),
+                                dict(cache=F(3, 5, 1, 2, 16, 16)), dict(cache=F(5, 2, 2, 16, 16)), dict(k=F(3, 9, 16)), dict(k=F(3, 9, 32).bfloat16()),
+                                dict(v=F(3, 32, 9).transpose(1, 2)), dict(cache=F(3, 5, 2, 2, 16, 16).half(), k=F(3, 9, 32).half(), v=F(3, 9, 32).half()), dict()])
+def test_accept_refuses(kw):
+    with pytest.raises(KernelError):
+        kernels.tree_accept(**accept_args(**kw))
+
+
+def test_plain_tree_and_a_chain():
+    """A chain's ancestors are the nodes before it; a walk down a tree that was built to be right takes all of it."""
+    rng = random.Random(3)
+    assert P.ancestors([-1, 0, 1]) == [{0}, {0, 1}, {0, 1, 2}]
+    cu, seq, pos, slots, mask = P.layout([[-1, 0, 0, 2]], [15], [[7, 3]], 16, 1)
+    assert (cu, seq, pos, slots) == ([0, 4], [0] * 4, [15, 16, 16, 17], [7 * 16 + 15, 48, 49, 50])
+    assert mask.flatten().tolist() == [1, 3, 5, 13]
+    assert P.layout([[-1, 0, 0, 2]], [15], [[7, 3]], 16, 1, window=2)[4].flatten().tolist() == [1, 3, 5, 12]
+    tokens = [rng.randrange(50) for _ in range(20)]
+    assert P.accept(tokens[1:] + [99], tokens, list(range(-1, 19)), [0, 20], 32) == ([list(range(20))], [99])
+    assert P.accept(tokens[1:] + [99], tokens, list(range(-1, 19)), [0, 20], 6) == ([list(range(6))], [tokens[6]])
