@@ -196,21 +196,20 @@ __global__ void __launch_bounds__(kThreads) attention_tree_kernel(Args a, bool w
       }
     } else {
       const int slot = 2 * b + (begins ? 1 : 0);
-      float* o = a.partials + (size_t)slot * kRows * (a.hd + 2);
+      float* o = a.partials + slot * partial_floats(kRows, a.hd);
+      const int quads = (a.hd + 3) / 4;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int row = 2 * ty + i;
         if (row >= rows) continue;
 #pragma unroll
-        for (int c = 0; c < HDP / 64; ++c)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int col = 64 * c + 4 * tx + e;
-            if (col < a.hd) o[(size_t)row * a.hd + col] = acc[i][c][e];
-          }
+        for (int c = 0; c < HDP / 64; ++c) {
+          const int quad = 16 * c + tx;
+          if (quad < quads) st4(o + ((size_t)quad * kRows + row) * 4, acc[i][c]);
+        }
         if (tx == 0) {
-          o[(size_t)kRows * a.hd + row] = m[i];
-          o[(size_t)kRows * (a.hd + 1) + row] = l[i];
+          o[(size_t)quads * 4 * kRows + row] = m[i];
+          o[(size_t)quads * 4 * kRows + kRows + row] = l[i];
         }
       }
       if (tid == 0) a.notes[slot] = make_int4(u.s, u.kvh, row0, rows | (ends ? 0 : kGoesOn));
@@ -233,7 +232,7 @@ static int launch(const Args& a, int blocks, bool wide, cudaStream_t st) {
   }
   int rc = launch_pdl(attention_tree_kernel<T, HDP>, dim3(blocks), dim3(kThreads), smem, st, a, wide);
   if (rc) return rc;
-  return launch_pdl(join_kernel<T, kRows>, dim3(blocks, 4), dim3(256), 0, st, a);
+  return launch_pdl(join_kernel<T, kRows, 1>, dim3(blocks, 1), dim3(256), 0, st, a);
 }
 
 }  // namespace tree
@@ -243,7 +242,7 @@ static int launch(const Args& a, int blocks, bool wide, cudaStream_t st) {
 LMSF_API int lmsf_attention_tree_blocks(int sms) { return 2 * sms; }
 LMSF_API long long lmsf_attention_tree_workspace(int sms, int hd) {
   const long long blocks = lmsf_attention_tree_blocks(sms);
-  return 2 * blocks * (lmsf::tree::kRows * (hd + 2ll) * 4 + 16);
+  return 2 * blocks * ((long long)lmsf::tree::partial_floats(lmsf::tree::kRows, hd) * 4 + 16);
 }
 
 // q, out [n_rows, heads x hd]; k, v [n_rows, kv heads x hd]; strides in elements.  workspace: lmsf_attention_tree_workspace

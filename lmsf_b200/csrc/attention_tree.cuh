@@ -8,8 +8,8 @@
 // cached keys first, then the nodes.  All units' tiles in a row, requests in order, are shared out evenly: of G blocks block b
 // takes the tiles [b W / G, (b + 1) W / G) of all W (G no more than W), whatever the lengths are; no plan is made on the host, so a captured launch
 // serves any lengths.  A unit that lies in one block's range is finished there.  Of a unit that is cut every block leaves a
-// partial (unnormalised output, running maximum, sum; float32) in the workspace: at most two for a block, one for the unit that it
-// begins with and one for the unit that it ends with.  A second kernel adds them up in the order of the blocks; both
+// partial (unnormalised output, running maximum, sum; float32) in the workspace: at most two for a block (and item), one for the unit
+// that it begins with and one for the unit that it ends with.  A second kernel adds them up in the order of the blocks; both
 // depend only on lengths and G, so the result is the same in every run.
 #pragma once
 #include "common.cuh"
@@ -121,44 +121,61 @@ __device__ __forceinline__ Piece piece_at(const Args& a, const int* offs, int ro
   return x;
 }
 
-// Note of a partial: x = request, or -1: none; y = kv head; z = first row among the request's rows of that kv head;
-// w = rows | 0x10000 if the unit goes on in the next block.
+// Partial number (2 block + which) * kItems + item: which = 0 for the unit that the block's share begins inside, 1 for the one that it ends
+// inside.  Columns in fours: [hd / 4, rounded up][kRows][4], so that threads that own a row each write and read whole lines;
+// then [kRows] maxima (in log2 units) and [kRows] sums.
+// Its note: x = request, or -1: none; y = kv head; z = first row among the request's rows of that kv head;
+// w = rows | kGoesOn if the unit goes on in the next block.
 constexpr int kGoesOn = 0x10000;
+__host__ __device__ __forceinline__ size_t partial_floats(int rows, int hd) { return (size_t)rows * ((hd + 3) / 4 * 4 + 2); }
 
-// Adds the partials of the units that were cut: one block row of the grid per block b of the first kernel; it acts if a unit begins
-// in b's last piece and goes on.  Partial p: out [rows][hd], then [rows] maxima (in log2 units), then [rows] sums.
-template <typename T, int kRows>
+// Adds the partials of the units that were cut: block (b, y) of the grid acts if a unit begins in b's last piece and goes on; y is
+// an item and 32 of its rows.  A thread has one row and every eighth group of four columns, and keeps the sums of up to four
+// groups in registers while it goes over the partials.
+template <typename T, int kRows, int kItems>
 __global__ void __launch_bounds__(256) join_kernel(Args a) {
+  constexpr int kGroups = 4;
   pdl_launch_dependents();
   pdl_wait();
-  const int b = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int4 note = a.notes[2 * b + 1];
-  if (note.x < 0 || !(note.w & kGoesOn)) return;
-  const int rows = note.w & 0xffff;
-  const size_t slot_floats = (size_t)kRows * (a.hd + 2);
+  const int b = blockIdx.x, item = blockIdx.y / (kRows / 32), row = (blockIdx.y % (kRows / 32)) * 32 + (threadIdx.x & 31), warp = threadIdx.x >> 5;
+  const int4 note = a.notes[(2 * b + 1) * kItems + item];
+  if (note.x < 0 || !(note.w & kGoesOn) || row >= (note.w & 0xffff)) return;
   // the unit goes on in the first partials of the blocks behind, up to the one that ends it
   int last = b + 1;
-  while (last < (int)gridDim.x - 1 && (a.notes[2 * last].w & kGoesOn)) ++last;
-  const int start = min(max(a.cu_q[note.x], 0), a.n_rows);
-  auto slot = [&](int i) { return a.partials + slot_floats * (i == b ? 2 * b + 1 : 2 * i); };
-  for (int row = blockIdx.y * 8 + warp; row < rows; row += gridDim.y * 8) {
-    float m = -INFINITY;
-    for (int i = b + lane; i <= last; i += 32) m = fmaxf(m, slot(i)[(size_t)kRows * a.hd + row]);
-    m = warp_max(m);
-    const float base = m == -INFINITY ? 0.f : m;
+  while (last < (int)gridDim.x - 1 && (a.notes[2 * last * kItems + item].w & kGoesOn)) ++last;
+  const int quads = (a.hd + 3) / 4;
+  const size_t stride = partial_floats(kRows, a.hd);
+  auto part = [&](int i) { return a.partials + stride * ((size_t)(i == b ? 2 * b + 1 : 2 * i) * kItems + item); };
+  const size_t at_m = (size_t)quads * 4 * kRows + row, at_l = at_m + kRows;
+  float m = -INFINITY;
+  for (int i = b; i <= last; ++i) m = fmaxf(m, part(i)[at_m]);
+  const float base = m == -INFINITY ? 0.f : m;
+  const int r = note.z + row, node = r / a.group, head = note.y * a.group + r % a.group;
+  T* out = (T*)a.out + (min(max(a.cu_q[note.x], 0), a.n_rows) + node) * a.out_stride + (size_t)head * a.hd;
+  for (int q0 = warp; q0 < quads; q0 += 8 * kGroups) {
+    float4 sum[kGroups] = {};
     float l = 0.f;
-    for (int i = b + lane; i <= last; i += 32) l += slot(i)[(size_t)kRows * (a.hd + 1) + row] * exp2f(slot(i)[(size_t)kRows * a.hd + row] - base);
-    l = warp_sum(l);
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    const int r = note.z + row, node = r / a.group, head = note.y * a.group + r % a.group;
-    T* out = (T*)a.out + (start + node) * a.out_stride + (size_t)head * a.hd;
-    for (int c = lane; c < a.hd; c += 32) {
-      float sum = 0.f;
-      for (int i = b; i <= last; ++i) {
-        const float* p = slot(i);
-        sum += p[(size_t)row * a.hd + c] * exp2f(p[(size_t)kRows * a.hd + row] - base);
+    for (int i = b; i <= last; ++i) {
+      const float* p = part(i);
+      const float w = exp2f(p[at_m] - base);
+      l += p[at_l] * w;
+#pragma unroll
+      for (int k = 0; k < kGroups; ++k) {
+        const int q = q0 + 8 * k;
+        if (q < quads) {
+          const float4 x = *reinterpret_cast<const float4*>(p + ((size_t)q * kRows + row) * 4);
+          sum[k].x += x.x * w; sum[k].y += x.y * w; sum[k].z += x.z * w; sum[k].w += x.w * w;
+        }
       }
-      out[c] = from_f32<T>(sum * inv);
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int k = 0; k < kGroups; ++k) {
+      const int c = 4 * (q0 + 8 * k);
+      const float v[4] = {sum[k].x * inv, sum[k].y * inv, sum[k].z * inv, sum[k].w * inv};
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (c + e < a.hd) out[c + e] = from_f32<T>(v[e]);
     }
   }
 }

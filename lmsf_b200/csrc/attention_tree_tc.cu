@@ -1,0 +1,704 @@
+// Attention of drafted trees on tcgen05 tensor cores: bfloat16, head sizes 64 to 128 (multiples of 16, -DLMSF_HEAD_DIM), pages of a
+// power of two of at least 8 keys.  The mathematics is attention_tree.cuh's: one pass over the keys with the running maximum and sum of the softmax.
+//
+// What bounds it: a request's keys and values are read once for all its nodes and all heads of a group, so up to some 150 rows a
+// kv head (nodes x heads of the group) the kernel is bound by their bytes, above by the tensor cores and the exponentials.
+//
+// An item is up to 128 rows: 128 / group nodes x the heads of the group, which one copy brings into shared memory node-major.  A
+// block works on pieces of units (a request, a kv head, two items; see attention_tree.cuh) with 128 keys a tile:
+//   * a unit of two items: both take every tile, each its own queries;
+//   * a unit of one item: the two halves of the block take the tiles in turn with the same queries, each with an output and a maximum of
+//     its own, and add up at the end, so that one half's products run beside the other's softmax here too.
+// Warps: 0-3 and 4-7 softmax of half 0 and 1, a row per thread; 8 and 9 bring tiles of k and v by tensor-map copies (a box per page, or
+// 32 rows of the step's own k and v for drafted tokens); 10 issues the products; 11 brings the queries and goes over those
+// tiles of v that some row must not see all of: rows that nobody sees are cleared, and in a tile whose rows not every row sees
+// (drafted tokens, the edge of a window) values that are no numbers are set to zero and remembered, since their zero weights would
+// make NaN of them; the rows that do see them get them added at the end.
+// Tensor memory: S of half x (128 columns, P over the first 64 of them as bfloat16 pairs) at 128 x, its output at 256 + 128 x.
+// Weights are rounded to bfloat16 for P V (2^-8 relative, the operand type of the product); sums, maxima, outputs are float32.
+// Every wait is bounded; when one runs out the block raises the error word (code 3), leaves its waits and ends in good order.
+#include <cstring>
+
+#include "attention_tree.cuh"
+#include "tc_common.cuh"
+
+#ifndef LMSF_HEAD_DIM
+#error "compile with -DLMSF_HEAD_DIM=64, 80, 96, 112 or 128"
+#endif
+
+LMSF_DEFINE_LAST_ERROR(lmsf_attention_tree_tc)
+
+namespace lmsf {
+namespace tree {
+
+using namespace lmsf::tc;
+
+constexpr int HD = LMSF_HEAD_DIM;
+static_assert(HD % 16 == 0 && HD >= 64 && HD <= 128, "head sizes 64 to 128 in steps of 16");
+constexpr int BM = 128, BN = 128;
+constexpr int kHB = (HD + 63) / 64;            // 64-wide blocks of the head dimension
+constexpr int kTileBytes = kHB * BN * 128;     // one tile of q, k or v
+constexpr int kStages = HD > 64 ? 2 : 4;       // tiles of k in flight, and of v
+constexpr int kOffK = 2 * kTileBytes, kOffV = kOffK + kStages * kTileBytes, kOffWork = kOffV + kStages * kTileBytes;
+constexpr uint32_t kTmemCols = 512, kOCol = 256;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kRescale = 8.0f;               // the output is rescaled when the maximum grew by more than this (log2 units)
+constexpr int kThreadsTotal = 384, kHalf = 128;
+constexpr int kRegsSoftmax = 224, kRegsOther = 56;
+constexpr int kRing = 8;                       // notes of tiles and of pieces that warps leave one another
+static_assert(kStages + 3 <= kRing, "notes are read before they are written again");
+
+struct TcArgs {
+  Args a;
+  int nodes_per_item, block_shift, rows_box;
+  int wide_out;                                // rows of the output take 16-byte stores
+  int* error_flag;
+};
+
+__device__ __forceinline__ float ex2_approx(float x) {      // 2^x, 0 for -inf
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float fmax3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t pk2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void upk2(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ void tmem_ld8_issue(uint32_t taddr, float* r) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n"
+               : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]) : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st8_issue(uint32_t taddr, const float* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n"
+               ::"r"(taddr), "f"(r[0]), "f"(r[1]), "f"(r[2]), "f"(r[3]), "f"(r[4]), "f"(r[5]), "f"(r[6]), "f"(r[7]) : "memory");
+}
+__device__ __forceinline__ void tma_load_box_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t mbar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+      ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(mbar) : "memory");
+}
+__device__ __forceinline__ void both_halves() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+// bits [lo, hi) of a word
+__device__ __forceinline__ uint32_t bits(int lo, int hi) {
+  lo = min(max(lo, 0), 32);
+  hi = min(max(hi, 0), 32);
+  const uint32_t upto = hi >= 32 ? 0xffffffffu : (1u << hi) - 1u, below = lo >= 32 ? 0xffffffffu : (1u << lo) - 1u;
+  return upto & ~below;
+}
+
+__global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(const TcArgs ta, const __grid_constant__ CUtensorMap q_map,
+                                                                             const __grid_constant__ CUtensorMap k_map,
+                                                                             const __grid_constant__ CUtensorMap v_map,
+                                                                             const __grid_constant__ CUtensorMap cache_map) {
+  const Args& a = ta.a;
+  extern __shared__ unsigned char smem_raw[];
+  // k_full[kStages], k_empty, v_full, v_fixed, v_empty [kStages each], s_full[2], p_full[2][half of P], o_done[2], q_full[2], q_free[2]
+  __shared__ __align__(8) uint64_t bars[5 * kStages + 12];
+  __shared__ uint32_t tmem_base_mem;
+  __shared__ int failed_mem, scratch[32];
+  __shared__ uint32_t k_holes[kRing], v_holes[kRing];    // boxes of the tile whose page is not there
+  __shared__ int odd_values[kRing];                      // of a piece: values that are no numbers were set to zero
+  __shared__ float2 stats[2][kHalf];                     // maximum and sum of a half's rows (a unit of one item)
+  volatile int* failed = &failed_mem;
+  const uint32_t smem = (smem_addr(smem_raw) + 1023u) & ~1023u;
+  int* offs = (int*)(smem_raw + (smem - smem_addr(smem_raw)) + kOffWork);
+  const uint32_t sQ = smem, sK = smem + kOffK, sV = smem + kOffV, bar0 = smem_addr(&bars[0]);
+  auto k_full = [&](int s) { return bar0 + 8u * s; };
+  auto k_empty = [&](int s) { return bar0 + 8u * (kStages + s); };
+  auto v_full = [&](int s) { return bar0 + 8u * (2 * kStages + s); };
+  auto v_fixed = [&](int s) { return bar0 + 8u * (3 * kStages + s); };
+  auto v_empty = [&](int s) { return bar0 + 8u * (4 * kStages + s); };
+  auto s_full = [&](int x) { return bar0 + 8u * (5 * kStages + x); };
+  auto p_full = [&](int x, int h) { return bar0 + 8u * (5 * kStages + 2 + 2 * x + h); };
+  auto o_done = [&](int x) { return bar0 + 8u * (5 * kStages + 6 + x); };
+  auto q_full = [&](int x) { return bar0 + 8u * (5 * kStages + 8 + x); };
+  auto q_free = [&](int x) { return bar0 + 8u * (5 * kStages + 10 + x); };
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  pdl_launch_dependents();
+  if (tid == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(k_full(s), 1);
+      mbar_init(k_empty(s), 1);
+      mbar_init(v_full(s), 1);
+      mbar_init(v_fixed(s), 1);
+      mbar_init(v_empty(s), 1);
+    }
+    for (int x = 0; x < 2; ++x) {
+      // the products' completion and an arrival of the thread that issued them: what that thread had seen before (notes of the
+      // tile) is then seen by those who wait here
+      mbar_init(s_full(x), 2);
+      mbar_init(o_done(x), 2);
+      mbar_init(p_full(x, 0), kHalf);
+      mbar_init(p_full(x, 1), kHalf);
+      mbar_init(q_full(x), 1);
+      mbar_init(q_free(x), 1);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    failed_mem = 0;
+  }
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_base_mem)), "r"(kTmemCols));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  pdl_wait();
+  const int rows_item = ta.nodes_per_item * a.group;
+  add_up_work<BN>(a, rows_item, 2, offs, scratch);
+  if (tid < 4) a.notes[4 * blockIdx.x + tid] = make_int4(-1, 0, 0, 0);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_base_mem;
+  int begin, end;
+  share_of_block(offs[a.n_seqs], begin, end);
+  auto piece = [&](int p) { return piece_at<BN>(a, offs, rows_item, 2, p, end); };
+
+  if (warp >= 8) {
+    regs_dec<kRegsOther>();
+    if (warp == 8 || warp == 9) {
+      // ------------------------------------------------------------------ producers: warp 8 of k, warp 9 of v
+      const bool is_v = warp == 9;
+      const uint32_t ring = is_v ? sV : sK;
+      const CUtensorMap* own_map = is_v ? &v_map : &k_map;
+      uint32_t* holes = is_v ? v_holes : k_holes;
+      auto full = [&](int s) { return is_v ? v_full(s) : k_full(s); };
+      auto empty = [&](int s) { return is_v ? v_empty(s) : k_empty(s); };
+      const int n_box = BN / ta.rows_box;
+      int g = 0;                                                 // tiles of the block so far
+      bool ok = true;
+      for (int p = begin; p < end && ok;) {
+        const Piece u = piece(p);
+        const int* table = a.block_table + (size_t)u.s * a.max_blocks;
+        const int head_row = (is_v ? a.n_kv : 0) + u.kvh;
+        // the first key of this lane's box, and its page: -2 where nobody sees the box, -1 where it is not there
+        auto box_key = [&](int t) { return (u.r.first + t) * BN + lane * ta.rows_box; };
+        auto fetch = [&](int t) {
+          const int key = box_key(t);
+          if (t >= u.t1 || t >= u.r.n_pre || lane >= n_box || key >= u.r.prefix || key + ta.rows_box <= u.r.lo) return -2;
+          const int page = table[key >> ta.block_shift];         // (the prefix ends inside the table)
+          return page >= 0 && page < a.pages ? page : -1;
+        };
+        int page = fetch(u.t0);
+        for (int t = u.t0; t < u.t1; ++t, ++g) {
+          const int s = g % kStages;
+          if (g >= kStages && !mbar_wait_f(empty(s), (uint32_t)((g / kStages - 1) & 1), failed)) { ok = false; break; }
+          const int next = fetch(t + 1);
+          const uint32_t dst = ring + s * kTileBytes;
+          if (t >= u.r.n_pre) {                                  // drafted tokens: boxes of 32 rows
+            const int j0 = (t - u.r.n_pre) * BN, boxes = (min(BN, u.r.nk - j0) + 31) / 32;
+            if (lane == 0) {
+              holes[g % kRing] = 0u;
+              mbar_arrive_expect_tx(full(s), (uint32_t)(boxes * 32 * 128 * kHB));
+            }
+            __syncwarp();
+            if (lane < boxes) {
+#pragma unroll
+              for (int hb = 0; hb < kHB; ++hb)
+                tma_load_box_3d(dst + hb * (BN * 128) + lane * (32 * 128), own_map, hb * 64, u.kvh, u.r.start + j0 + lane * 32, full(s));
+            }
+          } else {
+            const uint32_t here = __ballot_sync(0xffffffffu, page >= 0), missing = __ballot_sync(0xffffffffu, page == -1);
+            if (lane == 0) {
+              holes[g % kRing] = missing;
+              mbar_arrive_expect_tx(full(s), (uint32_t)(__popc(here) * ta.rows_box * 128 * kHB));
+            }
+            __syncwarp();
+            if (page >= 0) {
+              const int slot = box_key(t) & (a.block_size - 1);
+#pragma unroll
+              for (int hb = 0; hb < kHB; ++hb)
+                tma_load_box(dst + hb * (BN * 128) + lane * ta.rows_box * 128, &cache_map, hb * 64, slot, head_row, page, full(s));
+            }
+          }
+          page = next;
+        }
+        p += u.t1 - u.t0;
+      }
+      // no copy of this block may be in flight when it ends
+      for (int i = max(0, g - kStages); i < g; ++i) mbar_wait_drain(full(i % kStages), (uint32_t)((i / kStages) & 1));
+      // nor an arrival on its barriers
+      for (int i = max(0, g - kStages); i < g && ok; ++i) ok = mbar_wait_f(empty(i % kStages), (uint32_t)((i / kStages) & 1), failed);
+    } else if (warp == 10) {
+      // ------------------------------------------------------------------ tensor-core issue
+      constexpr uint32_t idesc_s = instr_desc(BM, BN, 0), idesc_o = instr_desc(BM, HD, 1);
+      const bool leader = elect_one();
+      const uint64_t dq0 = smem_desc(sQ, 16, 1024), dk0 = smem_desc(sK, 16, 1024), dv0 = smem_desc(sV, BN * 128, 1024);
+      int g0 = 0, n_p[2] = {0, 0}, n_q[2] = {0, 0};              // tiles of the block before the piece; P's and queries of a half so far
+      bool ok = true;
+      for (int p = begin; p < end && ok;) {
+        const Piece u = piece(p);
+        const bool two = u.item + 1 < u.r.items;
+        const int nt = u.t1 - u.t0;
+        auto issue_s = [&](int x, int j) {
+          const uint64_t dq = dq0 + (uint64_t)(((two ? x : 0) * kTileBytes) >> 4), dk = dk0 + (uint64_t)((((g0 + j) % kStages) * kTileBytes) >> 4);
+#pragma unroll
+          for (int ks = 0; ks < HD / 16; ++ks) {
+            const uint32_t off = (ks / 4) * (BN * 128) + (ks % 4) * 32;
+            umma(leader, tmem + x * BN, dq + (off >> 4), dk + (off >> 4), idesc_s, ks > 0);
+          }
+          umma_commit(leader, s_full(x));
+          if (leader) mbar_arrive(s_full(x));
+          if (two || x == (j & 1)) {
+            if (j == nt - 1) umma_commit(leader, q_free(two ? x : 0));             // the piece's last scores from these queries
+            if (!two || x == 1) umma_commit(leader, k_empty((g0 + j) % kStages));
+          }
+        };
+        auto issue_pv = [&](int x, int j, bool first, int h) {
+          const uint64_t dv = dv0 + (uint64_t)((((g0 + j) % kStages) * kTileBytes) >> 4);
+#pragma unroll
+          for (int k4 = 0; k4 < BN / 32; ++k4) {
+            const int ks = h * (BN / 32) + k4;
+            umma_ts(leader, tmem + kOCol + x * 128, tmem + x * BN + ks * 8, dv + ((ks * 16 * 128) >> 4), idesc_o, (!first || ks > 0) ? 1u : 0u);
+          }
+        };
+        int k_ready = -1;
+        auto k_wait = [&](int j) {
+          if (k_ready >= j) return true;
+          const int g = g0 + j;
+          if (!mbar_wait_f(k_full(g % kStages), (uint32_t)((g / kStages) & 1), failed)) return false;
+          tc_fence_after();
+          k_ready = j;
+          return true;
+        };
+        const int step = two ? 1 : 2;                            // tiles between two of a half
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          if ((x == 0 || two) && ok) {
+            ok = mbar_wait_f(q_full(x), (uint32_t)(n_q[x] & 1), failed);
+            ++n_q[x];
+          }
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const int j = two ? 0 : x;
+          if (ok && j < nt) {
+            ok = k_wait(j);
+            if (ok) issue_s(x, j);
+          }
+        }
+        for (int j = 0; j < nt && ok; ++j) {
+          const int g = g0 + j, s = g % kStages;
+          ok = mbar_wait_f(v_full(s), (uint32_t)((g / kStages) & 1), failed) && mbar_wait_f(v_fixed(s), (uint32_t)((g / kStages) & 1), failed);
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            if (!ok || (!two && x != (j & 1))) continue;
+            const bool first = j < step;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              if (ok) ok = mbar_wait_f(p_full(x, h), (uint32_t)(n_p[x] & 1), failed);
+              if (!ok) continue;
+              tc_fence_after();
+              issue_pv(x, j, first, h);
+            }
+            if (!ok) continue;
+            ++n_p[x];
+            if (!two || x == 1) umma_commit(leader, v_empty(s));
+            if (j + step < nt) {
+              ok = k_wait(j + step);
+              if (ok) issue_s(x, j + step);
+            } else {
+              umma_commit(leader, o_done(x));
+              if (leader) mbar_arrive(o_done(x));
+            }
+          }
+        }
+        g0 += nt;
+        p += nt;
+      }
+    } else {
+      // ------------------------------------------------------------------ queries, and the tiles of v that are not for everybody
+      int g = 0, n_q[2] = {0, 0}, n_piece = 0;
+      bool ok = true;
+      for (int p = begin; p < end && ok; ++n_piece) {
+        const Piece u = piece(p);
+        const int items = min(2, u.r.items - u.item);
+        for (int x = 0; x < items && ok; ++x) {
+          if (n_q[x] > 0) ok = mbar_wait_f(q_free(x), (uint32_t)((n_q[x] - 1) & 1), failed);
+          if (!ok) break;
+          if (lane == 0) {
+            mbar_arrive_expect_tx(q_full(x), (uint32_t)(rows_item * 128 * kHB));
+#pragma unroll
+            for (int hb = 0; hb < kHB; ++hb)
+              tma_load_box_3d(sQ + x * kTileBytes + hb * (BM * 128), &q_map, hb * 64, u.kvh * a.group, u.r.start + (u.item + x) * ta.nodes_per_item, q_full(x));
+          }
+          ++n_q[x];
+        }
+        if (lane == 0) odd_values[n_piece % kRing] = 0;
+        for (int t = u.t0; t < u.t1 && ok; ++t, ++g) {
+          const int s = g % kStages;
+          ok = mbar_wait_f(v_full(s), (uint32_t)((g / kStages) & 1), failed);
+          if (!ok) break;
+          const bool nodes = t >= u.r.n_pre;
+          const int key0 = nodes ? (t - u.r.n_pre) * BN : (u.r.first + t) * BN;
+          const int lo = nodes ? 0 : u.r.lo - key0, hi = (nodes ? u.r.nk : u.r.prefix) - key0;       // rows [lo, hi) are seen
+          const bool some = nodes || (a.window > 0 && key0 <= u.r.prefix + u.r.n - 1 - a.window);    // but perhaps not by every row
+          const uint32_t missing = v_holes[g % kRing];
+          if (some || lo > 0 || hi < BN || missing) {
+            const uint32_t v = sV + s * kTileBytes;
+            bool odd = false;
+#pragma unroll 4
+            for (int i = lane; i < kHB * BN * 8; i += 32) {
+              const int row = (i >> 3) % BN;
+              const uint32_t at = v + i * 16;
+              if (row < lo || row >= hi || ((missing >> (row / ta.rows_box)) & 1u)) {
+                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
+              } else if (some) {
+                uint32_t w[4];
+                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
+                bool bad = false;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const bool high = (w[e] & 0x7f800000u) == 0x7f800000u, low = (w[e] & 0x7f80u) == 0x7f80u;
+                  if (high) w[e] &= 0xffffu;
+                  if (low) w[e] &= 0xffff0000u;
+                  bad |= high | low;
+                }
+                if (bad) {
+                  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+                  odd = true;
+                }
+              }
+            }
+            if (__any_sync(0xffffffffu, odd) && lane == 0) odd_values[n_piece % kRing] = 1;
+            fence_async_smem();
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(v_fixed(s));
+        }
+        p += u.t1 - u.t0;
+      }
+      for (int x = 0; x < 2; ++x)
+        if (n_q[x] > 0) {
+          mbar_wait_drain(q_full(x), (uint32_t)((n_q[x] - 1) & 1));
+          if (ok) ok = mbar_wait_f(q_free(x), (uint32_t)((n_q[x] - 1) & 1), failed);
+        }
+    }
+  } else {
+    // ------------------------------------------------------------------ softmax of half x
+    regs_inc<kRegsSoftmax>();
+    const int x = warp >> 2, row = tid & 127;
+    const uint32_t t_row = tmem + ((uint32_t)((warp & 3) * 32) << 16), t_s = t_row + x * BN, t_o = t_row + kOCol + x * 128;
+    const float sl2 = a.scale * kLog2e;
+    int n_s = 0, n_o = 0, g0 = 0, n_piece = 0;                   // scores and outputs of this half so far; tiles and pieces of the block
+    bool ok = true;                                              // false: no more waits, but every barrier of the two halves is kept
+    for (int p = begin; p < end; ++n_piece) {
+      const Piece u = piece(p);
+      const bool two = u.item + 1 < u.r.items;
+      const int item = u.item + (two ? x : 0), node = row < rows_item ? item * ta.nodes_per_item + row / a.group : u.r.n;
+      const bool mine = node < u.r.n, any_mine = __any_sync(0xffffffffu, mine);
+      const int after = mine && a.window > 0 ? a.positions[u.r.start + node] - a.window : -1;
+      const unsigned* mask = a.mask + (size_t)(u.r.start + (mine ? node : 0)) * a.words;
+      const int nt = u.t1 - u.t0, step = two ? 1 : 2, j0 = two ? 0 : x;
+      float m = -INFINITY, l = 0.f;
+      for (int j = j0; j < nt; j += step, ++n_s) {
+        // S of the tile is complete, and with it every product issued before it: P V of this half's tile before too
+        if (ok) ok = mbar_wait_f(s_full(x), (uint32_t)(n_s & 1), failed);
+        if (!ok || !any_mine) {                                  // a warp without rows: its P is never looked at
+          mbar_arrive(p_full(x, 0));
+          mbar_arrive(p_full(x, 1));
+          continue;
+        }
+        tc_fence_after();
+        float sc[BN];
+#pragma unroll
+        for (int c = 0; c < BN; c += 32) tmem_ld32_issue(t_s + c, sc + c);
+        const int t = u.t0 + j;
+        const bool nodes = t >= u.r.n_pre;
+        const int key0 = nodes ? (t - u.r.n_pre) * BN : (u.r.first + t) * BN;
+        const uint32_t missing = k_holes[(g0 + j) % kRing];
+        uint32_t sees[4];
+        if (nodes) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int k = key0 + 32 * i;
+            sees[i] = mine && k < u.r.nk ? mask[k >> 5] & bits(0, u.r.nk - k) : 0u;
+          }
+        } else {
+          const int from = max(u.r.lo, after + 1) - key0, to = u.r.prefix - key0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sees[i] = bits(from - 32 * i, to - 32 * i);
+          if (missing) {
+            for (int b = 0; b < BN / ta.rows_box; ++b)
+              if ((missing >> b) & 1u) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sees[i] &= ~bits(b * ta.rows_box - 32 * i, (b + 1) * ta.rows_box - 32 * i);
+              }
+          }
+        }
+        tmem_wait_ld();
+        if (__any_sync(0xffffffffu, (sees[0] & sees[1] & sees[2] & sees[3]) != 0xffffffffu)) {
+#pragma unroll
+          for (int i = 0; i < BN; ++i)
+            if (!((sees[i >> 5] >> (i & 31)) & 1u)) sc[i] = -INFINITY;
+        }
+        float m0 = fmax3(sc[0], sc[1], sc[2]), m1 = fmax3(sc[3], sc[4], sc[5]), m2 = fmax3(sc[6], sc[7], sc[8]), m3 = fmax3(sc[9], sc[10], sc[11]);
+#pragma unroll
+        for (int i = 12; i + 7 < BN; i += 8) {
+          m0 = fmax3(m0, sc[i], sc[i + 1]);
+          m1 = fmax3(m1, sc[i + 2], sc[i + 3]);
+          m2 = fmax3(m2, sc[i + 4], sc[i + 5]);
+          m3 = fmax3(m3, sc[i + 6], sc[i + 7]);
+        }
+        float top = fmaxf(fmax3(m0, m1, m2), fmax3(m3, sc[BN - 4], sc[BN - 3]));
+        top = fmax3(top, sc[BN - 2], sc[BN - 1]) * sl2;
+        const bool grow = top > m + kRescale;                    // (and at the first key that a row sees)
+        float alpha = 1.f;
+        if (grow) {
+          alpha = ex2_approx(m - top);
+          m = top;
+          l *= alpha;
+        }
+        if (j > j0 && __any_sync(0xffffffffu, grow)) {
+#pragma unroll
+          for (int c = 0; c < HD; c += 16) {
+            float r[16];
+            tmem_ld8_issue(t_o + c, r);
+            tmem_ld8_issue(t_o + c + 8, r + 8);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) r[i] *= alpha;
+            tmem_st8_issue(t_o + c, r);
+            tmem_st8_issue(t_o + c + 8, r + 8);
+          }
+          tmem_wait_st();
+        }
+        const float neg_m = m == -INFINITY ? 0.f : -m;
+        const uint64_t scale2 = pk2(sl2, sl2), neg2 = pk2(neg_m, neg_m);
+        uint64_t sum = pk2(0.f, 0.f);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t w[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            float x0, x1;
+            upk2(fma2(pk2(sc[h * 64 + 2 * i], sc[h * 64 + 2 * i + 1]), scale2, neg2), x0, x1);
+            x0 = ex2_approx(x0);
+            x1 = ex2_approx(x1);
+            sum = add2(sum, pk2(x0, x1));
+            w[i] = pack_bf16(x0, x1);
+          }
+          tmem_st32_issue(t_s + h * 32, w);
+          tmem_wait_st();
+          tc_fence_before();
+          mbar_arrive(p_full(x, h));
+        }
+        float l0, l1;
+        upk2(sum, l0, l1);
+        l += l0 + l1;
+      }
+      const bool have = j0 < nt;                                 // this half had a tile
+      if (have && ok) ok = mbar_wait_f(o_done(x), (uint32_t)(n_o & 1), failed);
+      n_o += have;
+      tc_fence_after();
+      // rows of one item that lie in both halves are added up here: half x writes the columns [x HD / 2, + HD / 2)
+      float w_own = 1.f, w_other = 0.f;
+      if (!two) {
+        stats[x][row] = make_float2(m, l);
+        both_halves();
+        const float2 o = stats[x ^ 1][row];
+        const float m_all = fmaxf(m, o.x), base = m_all == -INFINITY ? 0.f : m_all;
+        w_own = ex2_approx(m - base);
+        w_other = ex2_approx(o.x - base);
+        l = l * w_own + o.y * w_other;
+        m = m_all;
+      }
+      const bool other_has = !two && (x ^ 1) < nt;
+      const bool whole = u.t0 == 0 && u.t1 == u.r.tiles;
+      const int slot = (2 * (int)blockIdx.x + (u.t0 == 0 ? 1 : 0)) * 2 + (two ? x : 0);
+      const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
+      const bool odd = ok && odd_values[n_piece % kRing] != 0;
+      const int head = u.kvh * a.group + row % a.group;
+      bf16* out = (bf16*)a.out + (u.r.start + node) * a.out_stride + (size_t)head * HD;
+      float* part = a.partials + slot * partial_floats(BM, HD);
+      constexpr int kCols = HD / 2;
+      for (int part_of = 0; part_of < (two ? 2 : 1); ++part_of) {
+        const int c0 = (two ? part_of : x) * kCols;
+        if (!any_mine || !ok) continue;
+        float o[kCols];
+        if (have) {
+#pragma unroll
+          for (int c = 0; c < kCols; c += 8) tmem_ld8_issue(t_o + c0 + c, o + c);
+          tmem_wait_ld();
+        }
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) o[c] = have ? o[c] * w_own : 0.f;
+        if (other_has) {
+          const uint32_t t_other = t_row + kOCol + (x ^ 1) * 128 + c0;
+          float r[kCols];
+#pragma unroll
+          for (int c = 0; c < kCols; c += 8) tmem_ld8_issue(t_other + c, r + c);
+          tmem_wait_ld();
+#pragma unroll
+          for (int c = 0; c < kCols; ++c) o[c] = fmaf(r[c], w_other, o[c]);
+        }
+        if (odd && mine) {
+          // values that were set to zero, for the rows that see them (rare: nothing here is made to be fast)
+          for (int t = u.t0; t < u.t1; ++t) {
+            const bool nodes = t >= u.r.n_pre;
+            const int key0 = nodes ? (t - u.r.n_pre) * BN : (u.r.first + t) * BN;
+            if (!nodes && !(a.window > 0 && key0 <= u.r.prefix + u.r.n - 1 - a.window)) continue;
+            for (int k = key0; k < key0 + BN; ++k) {
+              const bf16* src;
+              if (nodes) {
+                if (k >= u.r.nk || !((mask[k >> 5] >> (k & 31)) & 1u)) continue;
+                src = (const bf16*)a.v + (u.r.start + k) * a.v_stride + (size_t)u.kvh * HD;
+              } else {
+                if (k < u.r.lo || k >= u.r.prefix || k <= after) continue;
+                const int page = a.block_table[(size_t)u.s * a.max_blocks + (k >> ta.block_shift)];
+                if (page < 0 || page >= a.pages) continue;
+                src = (const bf16*)a.cache + page * a.page_stride + a.v_off + ((size_t)u.kvh * a.block_size + (k & (a.block_size - 1))) * HD;
+              }
+#pragma unroll
+              for (int c = 0; c < kCols; ++c) {
+                const float v = __bfloat162float(src[c0 + c]);
+                if (!(fabsf(v) <= 3.4e38f)) o[c] += v;
+              }
+            }
+          }
+        }
+        if (!mine) continue;
+        if (whole) {
+#pragma unroll
+          for (int c = 0; c < kCols; ++c) o[c] *= inv;
+          if (ta.wide_out) {
+#pragma unroll
+            for (int c = 0; c < kCols; c += 8) {
+              uint4 w;
+              w.x = pack_bf16(o[c], o[c + 1]);
+              w.y = pack_bf16(o[c + 2], o[c + 3]);
+              w.z = pack_bf16(o[c + 4], o[c + 5]);
+              w.w = pack_bf16(o[c + 6], o[c + 7]);
+              *reinterpret_cast<uint4*>(out + c0 + c) = w;
+            }
+          } else {
+#pragma unroll
+            for (int c = 0; c < kCols; ++c) out[c0 + c] = __float2bfloat16_rn(o[c]);
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < kCols; c += 4)
+            *reinterpret_cast<float4*>(part + ((size_t)((c0 + c) / 4) * BM + row) * 4) = make_float4(o[c], o[c + 1], o[c + 2], o[c + 3]);
+        }
+      }
+      if (!whole && mine && (two || x == 0)) {
+        part[(size_t)HD * BM + row] = m;
+        part[(size_t)HD * BM + BM + row] = l;
+        if (row == 0)
+          a.notes[slot] = make_int4(u.s, u.kvh, item * rows_item, (min(ta.nodes_per_item, u.r.n - item * ta.nodes_per_item) * a.group) | (u.t1 < u.r.tiles ? kGoesOn : 0));
+      }
+      // the next piece's first P V overwrites the outputs, of both halves where they were added up
+      tc_fence_before();
+      if (!two) both_halves();
+      g0 += nt;
+      p += nt;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (*failed && tid == 0 && ta.error_flag) atomicExch(ta.error_flag, 3);
+  if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
+}
+
+// A map of [outer][middle][HD] bfloat16 with boxes of 64 x box_middle x box_outer.
+static bool make_map(CUtensorMap* m, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box) {
+  EncodeTiledFn encode = encode_tiled_fn();
+  const cuuint32_t ones[4] = {1, 1, 1, 1};
+  return encode && encode(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+}  // namespace tree
+}  // namespace lmsf
+
+LMSF_API long long lmsf_attention_tree_tc_workspace(int sms, int hd) {
+  return 4ll * sms * ((long long)lmsf::tree::partial_floats(lmsf::tree::BM, hd) * 4 + 16);
+}
+
+// As lmsf_attention_tree, for bfloat16; all rows 16-byte aligned but out's.
+LMSF_API int lmsf_attention_tree_tc(const void* q, long long q_stride, const void* k, long long k_stride, const void* v, long long v_stride,
+                                    void* out, long long out_stride, const void* cache, long long page_stride, long long v_off, int pages,
+                                    const int* block_table, int max_blocks, int block_size, const int* cu_q, const int* prefix_len,
+                                    const unsigned* mask, int words, const int* positions, int window, float scale, int n_seqs, int n_rows,
+                                    int n_q_heads, int n_kv_heads, int hd, void* workspace, int sms, int* error_flag, void* stream) {
+  using namespace lmsf;
+  using namespace lmsf::tree;
+  if (n_seqs <= 0 || n_rows <= 0) return 0;
+  if (hd != HD) LMSF_REFUSE("attention_tree: built for head size %d, called with %d", HD, hd);
+  if (n_kv_heads < 1 || n_q_heads < 1 || n_q_heads % n_kv_heads) LMSF_REFUSE("attention_tree: %d query heads of %d kv heads", n_q_heads, n_kv_heads);
+  if (n_seqs > kMaxSeqs) LMSF_REFUSE("attention_tree: %d requests are more than one launch takes (%d)", n_seqs, kMaxSeqs);
+  if (words < 1 || max_blocks < 1 || block_size < 8 || (block_size & (block_size - 1)))
+    LMSF_REFUSE("attention_tree: words=%d, max_blocks=%d, block_size=%d", words, max_blocks, block_size);
+  if (window > 0 && !positions) LMSF_REFUSE("attention_tree: a window needs the nodes' positions");
+  const int group = n_q_heads / n_kv_heads;
+  if (group > BM || !(scale > 0.f) || pages < 1) LMSF_REFUSE("attention_tree: group of %d heads, scale %g, %d pages", group, scale, pages);
+  if (((unsigned long long)q | (unsigned long long)k | (unsigned long long)v | (unsigned long long)cache) % 16 ||
+      (q_stride | k_stride | v_stride | page_stride) % 8)
+    LMSF_REFUSE("attention_tree: q, k, v and the cache need 16-byte aligned rows");
+  const long long tiles = ((long long)max_blocks * block_size + BN - 1) / BN + (32ll * words + BN - 1) / BN + 1;
+  TcArgs ta;
+  ta.nodes_per_item = BM / group;
+  const int rows_item = ta.nodes_per_item * group;
+  if ((((long long)n_rows * group + rows_item - 1) / rows_item + n_seqs) * n_kv_heads * tiles > 0x7fffffffll)
+    LMSF_REFUSE("attention_tree: %d rows of %d heads over %d pages are too much work for one launch", n_rows, n_q_heads, max_blocks);
+  ta.a = Args{q, q_stride, k, k_stride, v, v_stride, out, out_stride, cache, page_stride, v_off, pages, block_table, max_blocks, block_size,
+              cu_q, prefix_len, mask, words, positions, window, scale, n_seqs, n_rows, n_q_heads, n_kv_heads, group, hd, nullptr, nullptr};
+  ta.a.notes = (int4*)workspace;
+  ta.a.partials = (float*)(ta.a.notes + 4 * sms);
+  ta.block_shift = 0;
+  while ((1 << ta.block_shift) < block_size) ++ta.block_shift;
+  ta.rows_box = block_size < BN ? block_size : BN;
+  ta.wide_out = (unsigned long long)out % 16 == 0 && out_stride % 8 == 0;
+  ta.error_flag = error_flag;
+  CUtensorMap maps[4];
+  const cuuint64_t e = 2, d = HD;
+  {
+    const cuuint64_t dims[3] = {d, (cuuint64_t)n_q_heads, (cuuint64_t)n_rows}, strides[2] = {d * e, (cuuint64_t)q_stride * e};
+    const cuuint32_t box[3] = {64, (cuuint32_t)group, (cuuint32_t)ta.nodes_per_item};
+    if (!make_map(&maps[0], q, 3, dims, strides, box)) LMSF_REFUSE("attention_tree: no tensor map of the queries");
+  }
+  for (int i = 0; i < 2; ++i) {
+    const cuuint64_t dims[3] = {d, (cuuint64_t)n_kv_heads, (cuuint64_t)n_rows}, strides[2] = {d * e, (cuuint64_t)(i ? v_stride : k_stride) * e};
+    const cuuint32_t box[3] = {64, 1, 32};
+    if (!make_map(&maps[1 + i], i ? v : k, 3, dims, strides, box)) LMSF_REFUSE("attention_tree: no tensor map of the drafted tokens' keys");
+  }
+  {
+    const cuuint64_t dims[4] = {d, (cuuint64_t)block_size, 2 * (cuuint64_t)n_kv_heads, (cuuint64_t)pages};
+    const cuuint64_t strides[3] = {d * e, (cuuint64_t)block_size * d * e, (cuuint64_t)page_stride * e};
+    const cuuint32_t box[4] = {64, (cuuint32_t)ta.rows_box, 1, 1};
+    if (!make_map(&maps[3], cache, 4, dims, strides, box)) LMSF_REFUSE("attention_tree: no tensor map of the cache");
+  }
+  const size_t smem = kOffWork + sizeof(int) * (n_seqs + 1) + 1024;
+  static bool raised[64] = {};
+  int dev = 0;
+  cudaError_t rc = cudaGetDevice(&dev);
+  if (rc != cudaSuccess) return (int)rc;
+  if (dev < 64 && !raised[dev]) {
+    rc = cudaFuncSetAttribute(attention_tree_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kOffWork + 4 * (kMaxSeqs + 1) + 1024);
+    if (rc != cudaSuccess) return (int)rc;
+    raised[dev] = true;
+  }
+  cudaStream_t st = (cudaStream_t)stream;
+  const int status = launch_pdl(attention_tree_tc_kernel, dim3(sms), dim3(kThreadsTotal), smem, st, ta, maps[0], maps[1], maps[2], maps[3]);
+  if (status) return status;
+  return launch_pdl(join_kernel<bf16, BM, 2>, dim3(sms, 2 * BM / 32), dim3(256), 0, st, ta.a);
+}

@@ -7,6 +7,7 @@ VARIANTS = {
     # one build per head size that the tensor-core attention kernels take
     "attention_mma.cu": [(f"LMSF_HEAD_DIM={hd}",) for hd in range(16, 257, 16)],
     "attention_tc.cu": [("LMSF_HEAD_DIM=64",), ("LMSF_HEAD_DIM=128",)],
+    "attention_tree_tc.cu": [(f"LMSF_HEAD_DIM={hd}",) for hd in (64, 80, 96, 112, 128)],
 }
 
 

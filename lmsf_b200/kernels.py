@@ -1060,12 +1060,34 @@ def tree_layout(cu_q: torch.Tensor, token_seq: torch.Tensor, positions: torch.Te
 
 _ATTENTION_TREE_ARGS = [c_void_p, c_longlong] * 4 + [c_void_p, c_longlong, c_longlong, c_int, c_void_p, c_int, c_int, c_void_p,
                         c_void_p, c_void_p, c_int, c_void_p, c_int, c_float, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int, c_void_p]
+_ATTENTION_TREE_TC_ARGS = _ATTENTION_TREE_ARGS[:-4] + [c_void_p, c_int, c_void_p, c_void_p]
 _TREE_WORKSPACE = {}
+TREE_TC_HEAD_DIMS = (64, 80, 96, 112, 128)
+USE_TC_TREE = True             # bfloat16 trees run on the tcgen05 kernel where it takes them (csrc/attention_tree_tc.cu)
+
+
+def attention_tree_tc_supported(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: torch.Tensor, scale: float, group: int) -> bool:
+    """Whether `attention_tree` runs on the tensor cores: bfloat16, a head size of TREE_TC_HEAD_DIMS, groups up to 128, pages of a power
+    of two of at least 8 tokens, a positive scale, rows of q, k, v and the cache on 16-byte boundaries."""
+    bs = cache.shape[3]
+    return (q.dtype == torch.bfloat16 and cache.shape[4] in TREE_TC_HEAD_DIMS and group <= 128 and bs >= 8 and bs & (bs - 1) == 0
+            and cache.shape[0] > 0 and scale > 0.0 and (q.stride(0) | k.stride(0) | v.stride(0)) % 8 == 0
+            and (q.data_ptr() | k.data_ptr() | v.data_ptr() | cache.data_ptr()) % 16 == 0)
+
+
+def _tree_workspace(source: str, name: str, sms: int, head_dim: int, defines: Tuple[str, ...] = ()) -> int:
+    key = (name, sms, head_dim)
+    need = _TREE_WORKSPACE.get(key)
+    if need is None:
+        f = getattr(load_library(source, defines), name)
+        f.restype, f.argtypes = c_longlong, [c_int, c_int]
+        need = _TREE_WORKSPACE[key] = f(sms, head_dim)
+    return need
 
 
 def attention_tree(out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor,
                    block_size: int, cu_q: torch.Tensor, prefix_len: torch.Tensor, mask: torch.Tensor, scale: float, n_q_heads: int,
-                   n_kv_heads: int, head_dim: int, positions: Optional[torch.Tensor] = None, window: int = 0):
+                   n_kv_heads: int, head_dim: int, positions: Optional[torch.Tensor] = None, window: int = 0, error_flag: Optional[torch.Tensor] = None):
     """Attention of drafted trees: row t of request s sees the request's prefix_len[s] cached keys, read from the pages of `cache`
     [pages, 2, n_kv_heads, block_size, head_dim], and those of the request's own rows whose bits are set in mask[t] (int32 [N,
     words]: bit j is the request's j-th row; `tree_layout` makes it), whose keys and values are in k and v.  Nothing is written to the cache: `tree_accept` moves there what is kept.
@@ -1099,20 +1121,23 @@ def attention_tree(out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch
     dev = _same_device("attention_tree", q, out, k, v, cache, block_table, cu_q, prefix_len, mask, positions)
     if N == 0 or S == 0:
         return
-    key = (dev.index, head_dim)
     sms = sm_count(dev)
-    need = _TREE_WORKSPACE.get(key)
-    if need is None:
-        w = load_library("attention_tree.cu").lmsf_attention_tree_workspace
-        w.restype, w.argtypes = c_longlong, [c_int, c_int]
-        need = _TREE_WORKSPACE[key] = w(sms, head_dim)
-    f = _func("attention_tree.cu", "lmsf_attention_tree", _ATTENTION_TREE_ARGS)
-    with _On(dev):
-        space = torch.empty(need, dtype=torch.uint8, device=dev)
-        rc = f(q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), out.data_ptr(), out.stride(0),
-               cache.data_ptr(), cache.stride(0), cache.stride(1), cache.shape[0], *tables, window, scale, S, N, n_q_heads, n_kv_heads,
-               head_dim, code, space.data_ptr(), sms, _stream())
-    _check(rc, "attention_tree.cu", "lmsf_attention_tree")
+    args = (q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), out.data_ptr(), out.stride(0), cache.data_ptr(),
+            cache.stride(0), cache.stride(1), cache.shape[0], *tables, window, scale, S, N, n_q_heads, n_kv_heads, head_dim)
+    if USE_TC_TREE and attention_tree_tc_supported(q, k, v, cache, scale, n_q_heads // n_kv_heads):
+        source, d = "attention_tree_tc.cu", (f"LMSF_HEAD_DIM={head_dim}",)
+        f = _func(source, "lmsf_attention_tree_tc", _ATTENTION_TREE_TC_ARGS, d)
+        with _On(dev):
+            space = torch.empty(_tree_workspace(source, "lmsf_attention_tree_tc_workspace", sms, head_dim, d), dtype=torch.uint8, device=dev)
+            rc = f(*args, space.data_ptr(), sms, _error_word(error_flag, dev), _stream())
+        _check(rc, source, "lmsf_attention_tree_tc", d)
+    else:
+        source = "attention_tree.cu"
+        f = _func(source, "lmsf_attention_tree", _ATTENTION_TREE_ARGS)
+        with _On(dev):
+            space = torch.empty(_tree_workspace(source, "lmsf_attention_tree_workspace", sms, head_dim), dtype=torch.uint8, device=dev)
+            rc = f(*args, code, space.data_ptr(), sms, _stream())
+        _check(rc, source, "lmsf_attention_tree")
     add_launches(1)
 
 

@@ -123,13 +123,14 @@ def attention_case(seed, lens, prefix, heads, kvh, hd, bs, dtype, window=0, mask
                 positions=pos + [0] * spare_rows, window=window, dtype=dt, n=sum(lens))
 
 
-def call_attention(c, out=None, **kw):
+def call_attention(c, out=None):
     from lmsf_b200 import kernels
     if out is None:
         out = torch.full((c["q"].shape[0], c["heads"] * c["hd"]), 7.0, dtype=c["dtype"], device=D)
-    S = len(c["prefix"])
+    S, f = len(c["prefix"]), flag()
     kernels.attention_tree(out, c["q"], c["k"], c["v"], c["cache"], ints(c["table"]).reshape(S, -1), c["bs"], ints(c["cu"]), ints(c["prefix"]),
-                           c["mask"].to(D), c["scale"], c["heads"], c["kvh"], c["hd"], positions=ints(c["positions"]), window=c["window"], **kw)
+                           c["mask"].to(D), c["scale"], c["heads"], c["kvh"], c["hd"], positions=ints(c["positions"]), window=c["window"], error_flag=f)
+    assert f.item() == 0
     return out
 
 
@@ -153,11 +154,15 @@ SHAPES = [  # lens, prefix, heads, kv heads, head size, page
 
 
 @pytest.mark.parametrize("lens,prefix,heads,kvh,hd,bs", SHAPES)
-@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "bf16 on the CUDA cores"])
 @pytest.mark.parametrize("masks,window", [("tree", 0), ("any", 0), ("tree", 37), ("any", 150)])
-def test_attention(lens, prefix, heads, kvh, hd, bs, dtype, masks, window):
+def test_attention(lens, prefix, heads, kvh, hd, bs, dtype, masks, window, monkeypatch):
     """Lengths of none and one, pages that end inside a tile, odd sizes and groups, rows that see no drafted token or nothing at all (no cached
     tokens and an empty mask), NaN everywhere that nobody looks."""
+    from lmsf_b200 import kernels
+    if dtype.startswith("bf16 "):
+        monkeypatch.setattr(kernels, "USE_TC_TREE", False)
+        dtype = "bf16"
     c = attention_case(sum(lens) + hd, lens, prefix, heads, kvh, hd, bs, dtype, window, masks, spare_rows=3)
     check_attention(c, call_attention(c))
 
