@@ -41,7 +41,7 @@ __global__ void __launch_bounds__(kThreads) attention_tree_kernel(Args a, bool w
   int begin, end;
   share_of_block(offs[a.n_seqs], begin, end);
   const int b = blockIdx.x;
-  if (tid < 2) a.notes[2 * b + tid] = make_int4(-1, 0, 0, 0);
+  if (tid == 0) a.notes[b] = make_int4(-1, 0, 0, 0);
   __syncthreads();
   const T* q = (const T*)a.q;
   for (int p = begin; p < end;) {
@@ -212,7 +212,7 @@ __global__ void __launch_bounds__(kThreads) attention_tree_kernel(Args a, bool w
           o[(size_t)quads * 4 * kRows + kRows + row] = l[i];
         }
       }
-      if (tid == 0) a.notes[slot] = make_int4(u.s, u.kvh, row0, rows | (ends ? 0 : kGoesOn));
+      if (begins && tid == 0) a.notes[b] = make_int4(u.s, u.kvh, row0, rows | (block_of_tile(offs[a.n_seqs], p + u.r.tiles - 1) << 8));
     }
     p += u.t1 - u.t0;
   }
@@ -232,7 +232,8 @@ static int launch(const Args& a, int blocks, bool wide, cudaStream_t st) {
   }
   int rc = launch_pdl(attention_tree_kernel<T, HDP>, dim3(blocks), dim3(kThreads), smem, st, a, wide);
   if (rc) return rc;
-  return launch_pdl(join_kernel<T, kRows, 1>, dim3(blocks, 1), dim3(256), 0, st, a);
+  const bool wide_out = ((unsigned long long)a.out | (unsigned long long)(a.out_stride * sizeof(T)) | (unsigned long long)(a.hd * sizeof(T))) % 16 == 0;
+  return launch_pdl(join_kernel<T, kRows, 1, HDP>, dim3(blocks, 1), dim3(256), 0, st, a, wide_out);
 }
 
 }  // namespace tree
@@ -242,7 +243,7 @@ static int launch(const Args& a, int blocks, bool wide, cudaStream_t st) {
 LMSF_API int lmsf_attention_tree_blocks(int sms) { return 2 * sms; }
 LMSF_API long long lmsf_attention_tree_workspace(int sms, int hd) {
   const long long blocks = lmsf_attention_tree_blocks(sms);
-  return 2 * blocks * ((long long)lmsf::tree::partial_floats(lmsf::tree::kRows, hd) * 4 + 16);
+  return blocks * (2 * (long long)lmsf::tree::partial_floats(lmsf::tree::kRows, hd) * 4 + 16);
 }
 
 // q, out [n_rows, heads x hd]; k, v [n_rows, kv heads x hd]; strides in elements.  workspace: lmsf_attention_tree_workspace
@@ -269,7 +270,7 @@ LMSF_API int lmsf_attention_tree(const void* q, long long q_stride, const void* 
          cu_q, prefix_len, mask, words, positions, window, scale, n_seqs, n_rows, n_q_heads, n_kv_heads, (int)group, hd, nullptr, nullptr};
   const int blocks = lmsf_attention_tree_blocks(sms);
   a.notes = (int4*)workspace;
-  a.partials = (float*)(a.notes + 2 * blocks);
+  a.partials = (float*)(a.notes + blocks);
   const int size = dtype == LMSF_F32 ? 4 : 2;
   const unsigned long long bits = (unsigned long long)q | (unsigned long long)k | (unsigned long long)v | (unsigned long long)cache |
                                   (unsigned long long)(size * (q_stride | k_stride | v_stride | page_stride | v_off | hd));

@@ -31,7 +31,7 @@ struct Args {
   const int* positions; int window;        // window > 0: a node at position p sees cached keys > p - window
   float scale;
   int n_seqs, n_rows, n_q_heads, n_kv, group, hd;
-  float* partials; int4* notes;            // workspace: two partials and two notes for every block
+  float* partials; int4* notes;            // workspace: for every block and item two partials and a note
 };
 
 struct Request { int start, n, nk, prefix, lo, first, n_pre, tiles, items; };
@@ -124,59 +124,80 @@ __device__ __forceinline__ Piece piece_at(const Args& a, const int* offs, int ro
 // Partial number (2 block + which) * kItems + item: which = 0 for the unit that the block's share begins inside, 1 for the one that it ends
 // inside.  Columns in fours: [hd / 4, rounded up][kRows][4], so that threads that own a row each write and read whole lines;
 // then [kRows] maxima (in log2 units) and [kRows] sums.
-// Its note: x = request, or -1: none; y = kv head; z = first row among the request's rows of that kv head;
-// w = rows | kGoesOn if the unit goes on in the next block.
-constexpr int kGoesOn = 0x10000;
+// Its note, of which = 1 alone: x = request, or -1: none; y = kv head; z = first row among the request's rows of that kv head;
+// w = rows | the last block that has a part of the unit << 8.
 __host__ __device__ __forceinline__ size_t partial_floats(int rows, int hd) { return (size_t)rows * ((hd + 3) / 4 * 4 + 2); }
 
+// The block that has tile p of all `work` tiles (share_of_block's rule).
+__device__ __forceinline__ int block_of_tile(int work, int p) {
+  const int blocks = min((int)gridDim.x, work);
+  int b = (int)((long long)p * blocks / work);
+  while ((long long)work * (b + 1) / blocks <= p) ++b;
+  return b;
+}
+
 // Adds the partials of the units that were cut: block (b, y) of the grid acts if a unit begins in b's last piece and goes on; y is
-// an item and 32 of its rows.  A thread has one row and every eighth group of four columns, and keeps the sums of up to four
-// groups in registers while it goes over the partials.
-template <typename T, int kRows, int kItems>
-__global__ void __launch_bounds__(256) join_kernel(Args a) {
-  constexpr int kGroups = 4;
+// an item and 32 of its rows.  Lane = row, and a warp has every eighth group of four columns, so that partials are read in whole
+// lines; the results pass through shared memory, so that rows are written in whole lines too.  All of a partial's values are
+// requested before the first is used: with two or three partials a unit the kernel is one round trip to L2.
+template <typename T, int kRows, int kItems, int kMaxHd>
+__global__ void __launch_bounds__(256) join_kernel(Args a, bool wide) {
+  constexpr int kGroups = kMaxHd / 32;           // groups of four columns of a thread
+  __shared__ __align__(16) T tile[32][kMaxHd + 16 / sizeof(T)];
   pdl_launch_dependents();
   pdl_wait();
-  const int b = blockIdx.x, item = blockIdx.y / (kRows / 32), row = (blockIdx.y % (kRows / 32)) * 32 + (threadIdx.x & 31), warp = threadIdx.x >> 5;
-  const int4 note = a.notes[(2 * b + 1) * kItems + item];
-  if (note.x < 0 || !(note.w & kGoesOn) || row >= (note.w & 0xffff)) return;
-  // the unit goes on in the first partials of the blocks behind, up to the one that ends it
-  int last = b + 1;
-  while (last < (int)gridDim.x - 1 && (a.notes[2 * last * kItems + item].w & kGoesOn)) ++last;
-  const int quads = (a.hd + 3) / 4;
+  const int b = blockIdx.x, item = blockIdx.y / (kRows / 32), row0 = (blockIdx.y % (kRows / 32)) * 32, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int4 note = a.notes[b * kItems + item];
+  const int rows = min((note.w & 0xff) - row0, 32), last = note.w >> 8;
+  if (note.x < 0 || rows <= 0) return;
+  const int quads = (a.hd + 3) / 4, row = row0 + min(lane, rows - 1);
   const size_t stride = partial_floats(kRows, a.hd);
   auto part = [&](int i) { return a.partials + stride * ((size_t)(i == b ? 2 * b + 1 : 2 * i) * kItems + item); };
   const size_t at_m = (size_t)quads * 4 * kRows + row, at_l = at_m + kRows;
-  float m = -INFINITY;
-  for (int i = b; i <= last; ++i) m = fmaxf(m, part(i)[at_m]);
-  const float base = m == -INFINITY ? 0.f : m;
-  const int r = note.z + row, node = r / a.group, head = note.y * a.group + r % a.group;
-  T* out = (T*)a.out + (min(max(a.cu_q[note.x], 0), a.n_rows) + node) * a.out_stride + (size_t)head * a.hd;
-  for (int q0 = warp; q0 < quads; q0 += 8 * kGroups) {
-    float4 sum[kGroups] = {};
-    float l = 0.f;
-    for (int i = b; i <= last; ++i) {
-      const float* p = part(i);
-      const float w = exp2f(p[at_m] - base);
-      l += p[at_l] * w;
+  const int start = min(max(a.cu_q[note.x], 0), a.n_rows);
+  float m = -INFINITY, l = 0.f;
+  float4 sum[kGroups] = {};
+#pragma unroll 2
+  for (int i = b; i <= last; ++i) {              // running maximum again: one pass over the partials
+    const float* p = part(i);
+    const float mi = p[at_m], li = p[at_l];
+    float4 x[kGroups];
 #pragma unroll
-      for (int k = 0; k < kGroups; ++k) {
-        const int q = q0 + 8 * k;
-        if (q < quads) {
-          const float4 x = *reinterpret_cast<const float4*>(p + ((size_t)q * kRows + row) * 4);
-          sum[k].x += x.x * w; sum[k].y += x.y * w; sum[k].z += x.z * w; sum[k].w += x.w * w;
-        }
+    for (int k = 0; k < kGroups; ++k)
+      if (warp + 8 * k < quads) x[k] = *reinterpret_cast<const float4*>(p + ((size_t)(warp + 8 * k) * kRows + row) * 4);
+    const float now = fmaxf(m, mi), base = now == -INFINITY ? 0.f : now, keep = exp2f(m - base), w = exp2f(mi - base);
+    m = now;
+    l = l * keep + li * w;
+#pragma unroll
+    for (int k = 0; k < kGroups; ++k)
+      if (warp + 8 * k < quads) {
+        sum[k].x = sum[k].x * keep + x[k].x * w;
+        sum[k].y = sum[k].y * keep + x[k].y * w;
+        sum[k].z = sum[k].z * keep + x[k].z * w;
+        sum[k].w = sum[k].w * keep + x[k].w * w;
       }
-    }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-    for (int k = 0; k < kGroups; ++k) {
-      const int c = 4 * (q0 + 8 * k);
+  for (int k = 0; k < kGroups; ++k)
+    if (warp + 8 * k < quads) {
       const float v[4] = {sum[k].x * inv, sum[k].y * inv, sum[k].z * inv, sum[k].w * inv};
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (c + e < a.hd) out[c + e] = from_f32<T>(v[e]);
+      st4(&tile[lane][4 * (warp + 8 * k)], v);
     }
+  __syncthreads();
+  constexpr int kVec = 16 / sizeof(T);
+  auto out_of = [&](int i) {
+    const int r = note.z + row0 + i, node = r / a.group, head = note.y * a.group + r % a.group;
+    return (T*)a.out + (start + node) * a.out_stride + (size_t)head * a.hd;
+  };
+  if (wide) {                                    // rows of the output, and the head size, in 16-byte words
+    const int words = a.hd / kVec;
+    for (int i = threadIdx.x; i < rows * words; i += 256) {
+      const int r = i / words, c = (i % words) * kVec;
+      *reinterpret_cast<uint4*>(out_of(r) + c) = *reinterpret_cast<const uint4*>(&tile[r][c]);
+    }
+  } else {
+    for (int i = threadIdx.x; i < rows * a.hd; i += 256) out_of(i / a.hd)[i % a.hd] = tile[i / a.hd][i % a.hd];
   }
 }
 

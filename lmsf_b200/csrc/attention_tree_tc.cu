@@ -107,6 +107,15 @@ __device__ __forceinline__ uint32_t bits(int lo, int hi) {
   return upto & ~below;
 }
 
+// Rows [lo, hi) of a tile are seen by some row of the piece's request; none of the others is multiplied, but for those that share a step
+// of 16 with them.
+__device__ __forceinline__ void rows_seen(const Piece& u, int t, int& key0, int& lo, int& hi) {
+  const bool nodes = t >= u.r.n_pre;
+  key0 = nodes ? (t - u.r.n_pre) * BN : (u.r.first + t) * BN;
+  lo = nodes ? 0 : max(u.r.lo - key0, 0);
+  hi = min((nodes ? u.r.nk : u.r.prefix) - key0, BN);
+}
+
 __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(const TcArgs ta, const __grid_constant__ CUtensorMap q_map,
                                                                              const __grid_constant__ CUtensorMap k_map,
                                                                              const __grid_constant__ CUtensorMap v_map,
@@ -165,13 +174,14 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
   pdl_wait();
   const int rows_item = ta.nodes_per_item * a.group;
   add_up_work<BN>(a, rows_item, 2, offs, scratch);
-  if (tid < 4) a.notes[4 * blockIdx.x + tid] = make_int4(-1, 0, 0, 0);
+  if (tid < 2) a.notes[2 * blockIdx.x + tid] = make_int4(-1, 0, 0, 0);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_base_mem;
   int begin, end;
-  share_of_block(offs[a.n_seqs], begin, end);
+  const int work = offs[a.n_seqs];
+  share_of_block(work, begin, end);
   auto piece = [&](int p) { return piece_at<BN>(a, offs, rows_item, 2, p, end); };
 
   if (warp >= 8) {
@@ -264,12 +274,14 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
             if (!two || x == 1) umma_commit(leader, k_empty((g0 + j) % kStages));
           }
         };
-        auto issue_pv = [&](int x, int j, bool first, int h) {
+        // (steps [ks0, ks1) of the tile's eight)
+        auto issue_pv = [&](int x, int j, bool first, int h, int ks0, int ks1) {
           const uint64_t dv = dv0 + (uint64_t)((((g0 + j) % kStages) * kTileBytes) >> 4);
 #pragma unroll
           for (int k4 = 0; k4 < BN / 32; ++k4) {
             const int ks = h * (BN / 32) + k4;
-            umma_ts(leader, tmem + kOCol + x * 128, tmem + x * BN + ks * 8, dv + ((ks * 16 * 128) >> 4), idesc_o, (!first || ks > 0) ? 1u : 0u);
+            umma_ts(leader && ks >= ks0 && ks < ks1, tmem + kOCol + x * 128, tmem + x * BN + ks * 8, dv + ((ks * 16 * 128) >> 4), idesc_o,
+                    (!first || ks > ks0) ? 1u : 0u);
           }
         };
         int k_ready = -1;
@@ -298,6 +310,8 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
         }
         for (int j = 0; j < nt && ok; ++j) {
           const int g = g0 + j, s = g % kStages;
+          int key0, lo, hi;
+          rows_seen(u, u.t0 + j, key0, lo, hi);
           ok = mbar_wait_f(v_full(s), (uint32_t)((g / kStages) & 1), failed) && mbar_wait_f(v_fixed(s), (uint32_t)((g / kStages) & 1), failed);
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
@@ -308,7 +322,7 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
               if (ok) ok = mbar_wait_f(p_full(x, h), (uint32_t)(n_p[x] & 1), failed);
               if (!ok) continue;
               tc_fence_after();
-              issue_pv(x, j, first, h);
+              issue_pv(x, j, first, h, lo / 16, (hi + 15) / 16);
             }
             if (!ok) continue;
             ++n_p[x];
@@ -348,38 +362,63 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
           const int s = g % kStages;
           ok = mbar_wait_f(v_full(s), (uint32_t)((g / kStages) & 1), failed);
           if (!ok) break;
-          const bool nodes = t >= u.r.n_pre;
-          const int key0 = nodes ? (t - u.r.n_pre) * BN : (u.r.first + t) * BN;
-          const int lo = nodes ? 0 : u.r.lo - key0, hi = (nodes ? u.r.nk : u.r.prefix) - key0;       // rows [lo, hi) are seen
-          const bool some = nodes || (a.window > 0 && key0 <= u.r.prefix + u.r.n - 1 - a.window);    // but perhaps not by every row
+          int key0, lo, hi;
+          rows_seen(u, t, key0, lo, hi);
+          const bool some = t >= u.r.n_pre || (a.window > 0 && key0 <= u.r.prefix + u.r.n - 1 - a.window);   // seen, but perhaps not by every row
           const uint32_t missing = v_holes[g % kRing];
           if (some || lo > 0 || hi < BN || missing) {
-            const uint32_t v = sV + s * kTileBytes;
-            bool odd = false;
-#pragma unroll 4
-            for (int i = lane; i < kHB * BN * 8; i += 32) {
-              const int row = (i >> 3) % BN;
-              const uint32_t at = v + i * 16;
-              if (row < lo || row >= hi || ((missing >> (row / ta.rows_box)) & 1u)) {
-                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
-              } else if (some) {
-                uint32_t w[4];
-                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
-                bool bad = false;
+            // eight lanes a row, four rows at a time, and the 64-wide blocks of the head one after the other
+            const uint32_t v = sV + s * kTileBytes + (lane & 7) * 16;
+            const int r_lane = lane >> 3, lo16 = lo & ~15, hi16 = (hi + 15) & ~15;
+            auto clear = [&](int from, int to) {
+              for (int r = from + r_lane; r < to; r += 4)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  const bool high = (w[e] & 0x7f800000u) == 0x7f800000u, low = (w[e] & 0x7f80u) == 0x7f80u;
-                  if (high) w[e] &= 0xffffu;
-                  if (low) w[e] &= 0xffff0000u;
-                  bad |= high | low;
-                }
-                if (bad) {
-                  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
-                  odd = true;
-                }
+                for (int hb = 0; hb < kHB; ++hb)
+                  asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(v + (hb * BN + r) * 128), "r"(0) : "memory");
+            };
+            clear(lo16, lo);
+            clear(hi, hi16);
+            for (int left = (int)missing; left; left &= left - 1) {
+              const int box = __ffs(left) - 1;
+              clear(max(box * ta.rows_box, lo), min((box + 1) * ta.rows_box, hi));
+            }
+            __syncwarp();
+            if (some) {
+              // 0 x is 0 but for infinities and NaN: a sum of them says whether there is one among the values
+              __nv_bfloat162 odd2 = __float2bfloat162_rn(0.f);
+              const __nv_bfloat162 zero2 = odd2;
+              for (int r = lo + r_lane; r < hi; r += 16) {
+                uint32_t w[4][kHB][4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                  for (int hb = 0; hb < kHB; ++hb)
+                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[i][hb][0]), "=r"(w[i][hb][1]), "=r"(w[i][hb][2]), "=r"(w[i][hb][3])
+                                 : "r"(v + (hb * BN + min(r + 4 * i, hi - 1)) * 128) : "memory");
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                  for (int hb = 0; hb < kHB; ++hb)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) odd2 = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&w[i][hb][e]), zero2, odd2);
+              }
+              const bool odd = __hisnan(__low2bfloat16(odd2)) || __hisnan(__high2bfloat16(odd2));
+              if (__any_sync(0xffffffffu, odd)) {
+                if (lane == 0) odd_values[n_piece % kRing] = 1;
+                for (int r = lo + r_lane; r < hi; r += 4)
+                  for (int hb = 0; hb < kHB; ++hb) {
+                    const uint32_t at = v + (hb * BN + r) * 128;
+                    uint32_t w[4];
+                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                      if ((w[e] & 0x7f800000u) == 0x7f800000u) w[e] &= 0xffffu;
+                      if ((w[e] & 0x7f80u) == 0x7f80u) w[e] &= 0xffff0000u;
+                    }
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+                  }
               }
             }
-            if (__any_sync(0xffffffffu, odd) && lane == 0) odd_values[n_piece % kRing] = 1;
             fence_async_smem();
           }
           __syncwarp();
@@ -603,8 +642,9 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
       if (!whole && mine && (two || x == 0)) {
         part[(size_t)HD * BM + row] = m;
         part[(size_t)HD * BM + BM + row] = l;
-        if (row == 0)
-          a.notes[slot] = make_int4(u.s, u.kvh, item * rows_item, (min(ta.nodes_per_item, u.r.n - item * ta.nodes_per_item) * a.group) | (u.t1 < u.r.tiles ? kGoesOn : 0));
+        if (row == 0 && u.t0 == 0)
+          a.notes[2 * blockIdx.x + (two ? x : 0)] = make_int4(u.s, u.kvh, item * rows_item, min(ta.nodes_per_item, u.r.n - item * ta.nodes_per_item) * a.group
+                                                              | (block_of_tile(work, p + u.r.tiles - 1) << 8));
       }
       // the next piece's first P V overwrites the outputs, of both halves where they were added up
       tc_fence_before();
@@ -631,7 +671,7 @@ static bool make_map(CUtensorMap* m, const void* base, int rank, const cuuint64_
 }  // namespace lmsf
 
 LMSF_API long long lmsf_attention_tree_tc_workspace(int sms, int hd) {
-  return 4ll * sms * ((long long)lmsf::tree::partial_floats(lmsf::tree::BM, hd) * 4 + 16);
+  return sms * (4 * (long long)lmsf::tree::partial_floats(lmsf::tree::BM, hd) * 4 + 2 * 16);
 }
 
 // As lmsf_attention_tree, for bfloat16; all rows 16-byte aligned but out's.
@@ -663,7 +703,7 @@ LMSF_API int lmsf_attention_tree_tc(const void* q, long long q_stride, const voi
   ta.a = Args{q, q_stride, k, k_stride, v, v_stride, out, out_stride, cache, page_stride, v_off, pages, block_table, max_blocks, block_size,
               cu_q, prefix_len, mask, words, positions, window, scale, n_seqs, n_rows, n_q_heads, n_kv_heads, group, hd, nullptr, nullptr};
   ta.a.notes = (int4*)workspace;
-  ta.a.partials = (float*)(ta.a.notes + 4 * sms);
+  ta.a.partials = (float*)(ta.a.notes + 2 * sms);
   ta.block_shift = 0;
   while ((1 << ta.block_shift) < block_size) ++ta.block_shift;
   ta.rows_box = block_size < BN ? block_size : BN;
@@ -700,5 +740,5 @@ LMSF_API int lmsf_attention_tree_tc(const void* q, long long q_stride, const voi
   cudaStream_t st = (cudaStream_t)stream;
   const int status = launch_pdl(attention_tree_tc_kernel, dim3(sms), dim3(kThreadsTotal), smem, st, ta, maps[0], maps[1], maps[2], maps[3]);
   if (status) return status;
-  return launch_pdl(join_kernel<bf16, BM, 2>, dim3(sms, 2 * BM / 32), dim3(256), 0, st, ta.a);
+  return launch_pdl(join_kernel<bf16, BM, 2, 128>, dim3(sms, 2 * BM / 32), dim3(256), 0, st, ta.a, (bool)ta.wide_out);
 }
