@@ -16,7 +16,7 @@
 // make NaN of them; the rows that do see them get them added at the end.
 // Tensor memory: S of half x (128 columns, P over the first 64 of them as bfloat16 pairs) at 128 x, its output at 256 + 128 x.
 // Weights are rounded to bfloat16 for P V (2^-8 relative, the operand type of the product); sums, maxima, outputs are float32.
-// Every wait is bounded; when one runs out the block raises the error word (code 3), leaves its waits and ends in good order.
+// Every wait is bounded (the two halves meet at an mbarrier too); when one runs out the block raises the error word (code 3) and ends.
 #include <cstring>
 
 #include "attention_tree.cuh"
@@ -45,8 +45,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescale = 8.0f;               // the output is rescaled when the maximum grew by more than this (log2 units)
 constexpr int kThreadsTotal = 384, kHalf = 128;
 constexpr int kRegsSoftmax = 224, kRegsOther = 56;
-constexpr int kRing = 8;                       // notes of tiles and of pieces that warps leave one another
-static_assert(kStages + 3 <= kRing, "notes are read before they are written again");
+constexpr int kRing = 16;                      // notes of tiles and of pieces that warps leave one another
+static_assert(kStages + 4 <= kRing, "notes are read before they are written again");
 
 struct TcArgs {
   Args a;
@@ -98,7 +98,11 @@ __device__ __forceinline__ void tma_load_box_3d(uint32_t dst, const CUtensorMap*
       "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
       ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(mbar) : "memory");
 }
-__device__ __forceinline__ void both_halves() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+// the same value, which the compiler takes for another: what follows from it is worked out here and not kept from further up
+__device__ __forceinline__ int again(int v) {
+  asm volatile("" : "+r"(v));
+  return v;
+}
 // bits [lo, hi) of a word
 __device__ __forceinline__ uint32_t bits(int lo, int hi) {
   lo = min(max(lo, 0), 32);
@@ -107,13 +111,21 @@ __device__ __forceinline__ uint32_t bits(int lo, int hi) {
   return upto & ~below;
 }
 
+// What the warps of a block need to know of a piece, left in shared memory by warp 11 a piece ahead.  They read it where they need it:
+// held in registers it would not fit beside a row's scores, nor into what the other warps keep.
+struct __align__(16) PieceNote { int s, kvh, item, t0, nt, start, n, nk, prefix, lo, first, n_pre, tiles, two, p, pad; };
+typedef const volatile PieceNote* NotePtr;
 // Rows [lo, hi) of a tile are seen by some row of the piece's request; none of the others is multiplied, but for those that share a step
 // of 16 with them.
-__device__ __forceinline__ void rows_seen(const Piece& u, int t, int& key0, int& lo, int& hi) {
-  const bool nodes = t >= u.r.n_pre;
-  key0 = nodes ? (t - u.r.n_pre) * BN : (u.r.first + t) * BN;
-  lo = nodes ? 0 : max(u.r.lo - key0, 0);
-  hi = min((nodes ? u.r.nk : u.r.prefix) - key0, BN);
+__device__ __forceinline__ void rows_seen(NotePtr u, int t, int& key0, int& lo, int& hi) {
+  const bool nodes = t >= u->n_pre;
+  key0 = nodes ? (t - u->n_pre) * BN : (u->first + t) * BN;
+  lo = nodes ? 0 : max(u->lo - key0, 0);
+  hi = min((nodes ? u->nk : u->prefix) - key0, BN);
+}
+// Seen by some row, but perhaps not by every one: drafted tokens, and cached ones at the edge of a window.
+__device__ __forceinline__ bool seen_by_some(const Args& a, NotePtr u, int t, int key0) {
+  return t >= u->n_pre || (a.window > 0 && key0 <= u->prefix + u->n - 1 - a.window);
 }
 
 __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(const TcArgs ta, const __grid_constant__ CUtensorMap q_map,
@@ -122,8 +134,10 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
                                                                              const __grid_constant__ CUtensorMap cache_map) {
   const Args& a = ta.a;
   extern __shared__ unsigned char smem_raw[];
-  // k_full[kStages], k_empty, v_full, v_fixed, v_empty [kStages each], s_full[2], p_full[2][half of P], o_done[2], q_full[2], q_free[2]
-  __shared__ __align__(8) uint64_t bars[5 * kStages + 12];
+  // k_full[kStages], k_empty, v_full, v_fixed, v_empty [kStages each], s_full[2], p_full[2][half of P], o_done[2], q_full[2], q_free[2],
+  // noted[kRing], met
+  __shared__ __align__(8) uint64_t bars[5 * kStages + 13 + kRing];
+  __shared__ PieceNote notes[kRing];
   __shared__ uint32_t tmem_base_mem;
   __shared__ int failed_mem, scratch[32];
   __shared__ uint32_t k_holes[kRing], v_holes[kRing];    // boxes of the tile whose page is not there
@@ -143,6 +157,8 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
   auto o_done = [&](int x) { return bar0 + 8u * (5 * kStages + 6 + x); };
   auto q_full = [&](int x) { return bar0 + 8u * (5 * kStages + 8 + x); };
   auto q_free = [&](int x) { return bar0 + 8u * (5 * kStages + 10 + x); };
+  const uint32_t met = bar0 + 8u * (5 * kStages + 12 + kRing);
+  auto noted = [&](int i) { return bar0 + 8u * (5 * kStages + 12 + i % kRing); };
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   pdl_launch_dependents();
@@ -164,6 +180,8 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
       mbar_init(q_full(x), 1);
       mbar_init(q_free(x), 1);
     }
+    for (int i = 0; i < kRing; ++i) mbar_init(noted(i), 1);
+    mbar_init(met, 8);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     failed_mem = 0;
   }
@@ -182,7 +200,11 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
   int begin, end;
   const int work = offs[a.n_seqs];
   share_of_block(work, begin, end);
-  auto piece = [&](int p) { return piece_at<BN>(a, offs, rows_item, 2, p, end); };
+  // the note of the block's i-th piece
+  auto note_of = [&](int i, bool& ok) -> NotePtr {
+    if (ok) ok = mbar_wait_f(noted(i), (uint32_t)((i / kRing) & 1), failed);
+    return &notes[i % kRing];
+  };
 
   if (warp >= 8) {
     regs_dec<kRegsOther>();
@@ -197,26 +219,28 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
       const int n_box = BN / ta.rows_box;
       int g = 0;                                                 // tiles of the block so far
       bool ok = true;
-      for (int p = begin; p < end && ok;) {
-        const Piece u = piece(p);
-        const int* table = a.block_table + (size_t)u.s * a.max_blocks;
-        const int head_row = (is_v ? a.n_kv : 0) + u.kvh;
+      for (int i = 0, p = begin; p < end && ok; ++i) {
+        NotePtr u = note_of(i, ok);
+        if (!ok) break;
+        const int t0 = u->t0, t1 = t0 + u->nt, n_pre = u->n_pre;
+        const int* table = a.block_table + (size_t)u->s * a.max_blocks;
+        const int head_row = (is_v ? a.n_kv : 0) + u->kvh;
         // the first key of this lane's box, and its page: -2 where nobody sees the box, -1 where it is not there
-        auto box_key = [&](int t) { return (u.r.first + t) * BN + lane * ta.rows_box; };
+        const int key_base = u->first * BN + lane * ta.rows_box;
         auto fetch = [&](int t) {
-          const int key = box_key(t);
-          if (t >= u.t1 || t >= u.r.n_pre || lane >= n_box || key >= u.r.prefix || key + ta.rows_box <= u.r.lo) return -2;
+          const int key = key_base + t * BN;
+          if (t >= t1 || t >= n_pre || lane >= n_box || key >= u->prefix || key + ta.rows_box <= u->lo) return -2;
           const int page = table[key >> ta.block_shift];         // (the prefix ends inside the table)
           return page >= 0 && page < a.pages ? page : -1;
         };
-        int page = fetch(u.t0);
-        for (int t = u.t0; t < u.t1; ++t, ++g) {
+        int page = fetch(t0);
+        for (int t = t0; t < t1; ++t, ++g) {
           const int s = g % kStages;
           if (g >= kStages && !mbar_wait_f(empty(s), (uint32_t)((g / kStages - 1) & 1), failed)) { ok = false; break; }
           const int next = fetch(t + 1);
           const uint32_t dst = ring + s * kTileBytes;
-          if (t >= u.r.n_pre) {                                  // drafted tokens: boxes of 32 rows
-            const int j0 = (t - u.r.n_pre) * BN, boxes = (min(BN, u.r.nk - j0) + 31) / 32;
+          if (t >= n_pre) {                                      // drafted tokens: boxes of 32 rows
+            const int j0 = (t - n_pre) * BN, boxes = (min(BN, u->nk - j0) + 31) / 32;
             if (lane == 0) {
               holes[g % kRing] = 0u;
               mbar_arrive_expect_tx(full(s), (uint32_t)(boxes * 32 * 128 * kHB));
@@ -225,7 +249,7 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
             if (lane < boxes) {
 #pragma unroll
               for (int hb = 0; hb < kHB; ++hb)
-                tma_load_box_3d(dst + hb * (BN * 128) + lane * (32 * 128), own_map, hb * 64, u.kvh, u.r.start + j0 + lane * 32, full(s));
+                tma_load_box_3d(dst + hb * (BN * 128) + lane * (32 * 128), own_map, hb * 64, u->kvh, u->start + j0 + lane * 32, full(s));
             }
           } else {
             const uint32_t here = __ballot_sync(0xffffffffu, page >= 0), missing = __ballot_sync(0xffffffffu, page == -1);
@@ -235,7 +259,7 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
             }
             __syncwarp();
             if (page >= 0) {
-              const int slot = box_key(t) & (a.block_size - 1);
+              const int slot = (key_base + t * BN) & (a.block_size - 1);
 #pragma unroll
               for (int hb = 0; hb < kHB; ++hb)
                 tma_load_box(dst + hb * (BN * 128) + lane * ta.rows_box * 128, &cache_map, hb * 64, slot, head_row, page, full(s));
@@ -243,7 +267,7 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
           }
           page = next;
         }
-        p += u.t1 - u.t0;
+        p += t1 - t0;
       }
       // no copy of this block may be in flight when it ends
       for (int i = max(0, g - kStages); i < g; ++i) mbar_wait_drain(full(i % kStages), (uint32_t)((i / kStages) & 1));
@@ -256,10 +280,11 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
       const uint64_t dq0 = smem_desc(sQ, 16, 1024), dk0 = smem_desc(sK, 16, 1024), dv0 = smem_desc(sV, BN * 128, 1024);
       int g0 = 0, n_p[2] = {0, 0}, n_q[2] = {0, 0};              // tiles of the block before the piece; P's and queries of a half so far
       bool ok = true;
-      for (int p = begin; p < end && ok;) {
-        const Piece u = piece(p);
-        const bool two = u.item + 1 < u.r.items;
-        const int nt = u.t1 - u.t0;
+      for (int i = 0, p = begin; p < end && ok; ++i) {
+        NotePtr u = note_of(i, ok);
+        if (!ok) break;
+        const bool two = u->two != 0;
+        const int nt = u->nt, t0 = u->t0;
         auto issue_s = [&](int x, int j) {
           const uint64_t dq = dq0 + (uint64_t)(((two ? x : 0) * kTileBytes) >> 4), dk = dk0 + (uint64_t)((((g0 + j) % kStages) * kTileBytes) >> 4);
 #pragma unroll
@@ -269,10 +294,8 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
           }
           umma_commit(leader, s_full(x));
           if (leader) mbar_arrive(s_full(x));
-          if (two || x == (j & 1)) {
-            if (j == nt - 1) umma_commit(leader, q_free(two ? x : 0));             // the piece's last scores from these queries
-            if (!two || x == 1) umma_commit(leader, k_empty((g0 + j) % kStages));
-          }
+          if (j == nt - 1) umma_commit(leader, q_free(two ? x : 0));               // the piece's last scores from these queries
+          if (!two || x == 1) umma_commit(leader, k_empty((g0 + j) % kStages));
         };
         // (steps [ks0, ks1) of the tile's eight)
         auto issue_pv = [&](int x, int j, bool first, int h, int ks0, int ks1) {
@@ -311,7 +334,7 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
         for (int j = 0; j < nt && ok; ++j) {
           const int g = g0 + j, s = g % kStages;
           int key0, lo, hi;
-          rows_seen(u, u.t0 + j, key0, lo, hi);
+          rows_seen(u, t0 + j, key0, lo, hi);
           ok = mbar_wait_f(v_full(s), (uint32_t)((g / kStages) & 1), failed) && mbar_wait_f(v_fixed(s), (uint32_t)((g / kStages) & 1), failed);
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
@@ -340,46 +363,62 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
         p += nt;
       }
     } else {
-      // ------------------------------------------------------------------ queries, and the tiles of v that are not for everybody
-      int g = 0, n_q[2] = {0, 0}, n_piece = 0;
+      // ------------------------------------------------------------------ notes, queries, and the tiles of v that are not for everybody
+      int g = 0, n_q[2] = {0, 0};
       bool ok = true;
-      for (int p = begin; p < end && ok; ++n_piece) {
-        const Piece u = piece(p);
-        const int items = min(2, u.r.items - u.item);
-        for (int x = 0; x < items && ok; ++x) {
+      auto leave_note = [&](int i, int p) {
+        if (p >= end) return;
+        const Piece u = piece_at<BN>(a, offs, rows_item, 2, p, end);
+        if (lane == 0) {
+          volatile PieceNote* n = &notes[i % kRing];
+          n->s = u.s; n->kvh = u.kvh; n->item = u.item; n->t0 = u.t0; n->nt = u.t1 - u.t0; n->start = u.r.start; n->n = u.r.n; n->nk = u.r.nk;
+          n->prefix = u.r.prefix; n->lo = u.r.lo; n->first = u.r.first; n->n_pre = u.r.n_pre; n->tiles = u.r.tiles;
+          n->two = u.item + 1 < u.r.items; n->p = p;
+          mbar_arrive(noted(i));
+        }
+        __syncwarp();
+      };
+      leave_note(0, begin);
+      for (int i = 0, p = begin; p < end && ok; ++i) {
+        NotePtr u = &notes[i % kRing];                           // (written by this warp)
+        const int nt = u->nt, t0 = u->t0;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          if (!ok || (x == 1 && !u->two)) continue;
           if (n_q[x] > 0) ok = mbar_wait_f(q_free(x), (uint32_t)((n_q[x] - 1) & 1), failed);
-          if (!ok) break;
+          if (!ok) continue;
           if (lane == 0) {
             mbar_arrive_expect_tx(q_full(x), (uint32_t)(rows_item * 128 * kHB));
 #pragma unroll
             for (int hb = 0; hb < kHB; ++hb)
-              tma_load_box_3d(sQ + x * kTileBytes + hb * (BM * 128), &q_map, hb * 64, u.kvh * a.group, u.r.start + (u.item + x) * ta.nodes_per_item, q_full(x));
+              tma_load_box_3d(sQ + x * kTileBytes + hb * (BM * 128), &q_map, hb * 64, u->kvh * a.group, u->start + (u->item + x) * ta.nodes_per_item, q_full(x));
           }
           ++n_q[x];
         }
-        if (lane == 0) odd_values[n_piece % kRing] = 0;
-        for (int t = u.t0; t < u.t1 && ok; ++t, ++g) {
+        if (lane == 0) odd_values[i % kRing] = 0;
+        leave_note(i + 1, p + nt);
+        for (int t = t0; t < t0 + nt && ok; ++t, ++g) {
           const int s = g % kStages;
           ok = mbar_wait_f(v_full(s), (uint32_t)((g / kStages) & 1), failed);
           if (!ok) break;
           int key0, lo, hi;
           rows_seen(u, t, key0, lo, hi);
-          const bool some = t >= u.r.n_pre || (a.window > 0 && key0 <= u.r.prefix + u.r.n - 1 - a.window);   // seen, but perhaps not by every row
+          const bool some = seen_by_some(a, u, t, key0);
           const uint32_t missing = v_holes[g % kRing];
           if (some || lo > 0 || hi < BN || missing) {
             // eight lanes a row, four rows at a time, and the 64-wide blocks of the head one after the other
             const uint32_t v = sV + s * kTileBytes + (lane & 7) * 16;
-            const int r_lane = lane >> 3, lo16 = lo & ~15, hi16 = (hi + 15) & ~15;
+            const int r_lane = lane >> 3;
             auto clear = [&](int from, int to) {
               for (int r = from + r_lane; r < to; r += 4)
 #pragma unroll
                 for (int hb = 0; hb < kHB; ++hb)
                   asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(v + (hb * BN + r) * 128), "r"(0) : "memory");
             };
-            clear(lo16, lo);
-            clear(hi, hi16);
-            for (int left = (int)missing; left; left &= left - 1) {
-              const int box = __ffs(left) - 1;
+            clear(lo & ~15, lo);
+            clear(hi, (hi + 15) & ~15);
+            for (uint32_t left = missing; left; left &= left - 1) {
+              const int box = __ffs((int)left) - 1;
               clear(max(box * ta.rows_box, lo), min((box + 1) * ta.rows_box, hi));
             }
             __syncwarp();
@@ -388,23 +427,22 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
               __nv_bfloat162 odd2 = __float2bfloat162_rn(0.f);
               const __nv_bfloat162 zero2 = odd2;
               for (int r = lo + r_lane; r < hi; r += 16) {
-                uint32_t w[4][kHB][4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                for (int hb = 0; hb < kHB; ++hb) {
+                  uint32_t w[4][4];
 #pragma unroll
-                  for (int hb = 0; hb < kHB; ++hb)
-                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[i][hb][0]), "=r"(w[i][hb][1]), "=r"(w[i][hb][2]), "=r"(w[i][hb][3])
-                                 : "r"(v + (hb * BN + min(r + 4 * i, hi - 1)) * 128) : "memory");
+                  for (int k = 0; k < 4; ++k)
+                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[k][0]), "=r"(w[k][1]), "=r"(w[k][2]), "=r"(w[k][3])
+                                 : "r"(v + (hb * BN + min(r + 4 * k, hi - 1)) * 128) : "memory");
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                  for (int k = 0; k < 4; ++k)
 #pragma unroll
-                  for (int hb = 0; hb < kHB; ++hb)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) odd2 = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&w[i][hb][e]), zero2, odd2);
+                    for (int e = 0; e < 4; ++e) odd2 = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&w[k][e]), zero2, odd2);
+                }
               }
               const bool odd = __hisnan(__low2bfloat16(odd2)) || __hisnan(__high2bfloat16(odd2));
               if (__any_sync(0xffffffffu, odd)) {
-                if (lane == 0) odd_values[n_piece % kRing] = 1;
+                if (lane == 0) odd_values[i % kRing] = 1;
                 for (int r = lo + r_lane; r < hi; r += 4)
                   for (int hb = 0; hb < kHB; ++hb) {
                     const uint32_t at = v + (hb * BN + r) * 128;
@@ -424,8 +462,9 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
           __syncwarp();
           if (lane == 0) mbar_arrive(v_fixed(s));
         }
-        p += u.t1 - u.t0;
+        p += nt;
       }
+#pragma unroll
       for (int x = 0; x < 2; ++x)
         if (n_q[x] > 0) {
           mbar_wait_drain(q_full(x), (uint32_t)((n_q[x] - 1) & 1));
@@ -436,23 +475,42 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
     // ------------------------------------------------------------------ softmax of half x
     regs_inc<kRegsSoftmax>();
     const int x = warp >> 2, row = tid & 127;
-    const uint32_t t_row = tmem + ((uint32_t)((warp & 3) * 32) << 16), t_s = t_row + x * BN, t_o = t_row + kOCol + x * 128;
+    const uint32_t t_s = tmem + ((uint32_t)((warp & 3) * 32) << 16) + x * BN, t_o = t_s + kOCol;
     const float sl2 = a.scale * kLog2e;
-    int n_s = 0, n_o = 0, g0 = 0, n_piece = 0;                   // scores and outputs of this half so far; tiles and pieces of the block
-    bool ok = true;                                              // false: no more waits, but every barrier of the two halves is kept
-    for (int p = begin; p < end; ++n_piece) {
-      const Piece u = piece(p);
-      const bool two = u.item + 1 < u.r.items;
-      const int item = u.item + (two ? x : 0), node = row < rows_item ? item * ta.nodes_per_item + row / a.group : u.r.n;
-      const bool mine = node < u.r.n, any_mine = __any_sync(0xffffffffu, mine);
-      const int after = mine && a.window > 0 ? a.positions[u.r.start + node] - a.window : -1;
-      const unsigned* mask = a.mask + (size_t)(u.r.start + (mine ? node : 0)) * a.words;
-      const int nt = u.t1 - u.t0, step = two ? 1 : 2, j0 = two ? 0 : x;
+    int n_s = 0, n_o = 0, n_met = 0;                             // scores and outputs of this half so far, meetings of the two
+    bool ok = true;
+    auto meet = [&]() {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(met);
+      ok = mbar_wait_f(met, (uint32_t)(n_met & 1), failed);
+      ++n_met;
+    };
+    for (int i_piece = 0, p = begin; p < end; ++i_piece) {
+      NotePtr u = note_of(i_piece, ok);
+      if (!ok) break;
+      const bool two = u->two != 0;
+      int node = u->n;                                           // of this thread's row; the tree's size: none
+      if (row < rows_item) node = (u->item + (two ? x : 0)) * ta.nodes_per_item + row / a.group;
+      const bool mine = node < u->n, any_mine = __any_sync(0xffffffffu, mine);
+      const int after = mine && a.window > 0 ? a.positions[u->start + node] - a.window : -1;
+      auto mask_word = [&](int i) { return a.mask[(size_t)(u->start + node) * a.words + i]; };
+      const int nt = u->nt, step = two ? 1 : 2, j0 = two ? 0 : x;
       float m = -INFINITY, l = 0.f;
       for (int j = j0; j < nt; j += step, ++n_s) {
+        int key0, lo, hi;
+        rows_seen(u, u->t0 + j, key0, lo, hi);
+        const bool nodes = u->t0 + j >= u->n_pre;
+        // what the row sees of the tile, as bits; the words of a mask are requested before the scores are awaited
+        uint32_t sees[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (nodes) sees[i] = mine && 32 * i < hi ? mask_word((key0 >> 5) + i) & bits(0, hi - 32 * i) : 0u;
+          else sees[i] = bits(max(lo, after + 1 - key0) - 32 * i, hi - 32 * i);
+        }
         // S of the tile is complete, and with it every product issued before it: P V of this half's tile before too
-        if (ok) ok = mbar_wait_f(s_full(x), (uint32_t)(n_s & 1), failed);
-        if (!ok || !any_mine) {                                  // a warp without rows: its P is never looked at
+        ok = mbar_wait_f(s_full(x), (uint32_t)(n_s & 1), failed);
+        if (!ok) break;
+        if (!any_mine) {                                  // a warp without rows: its P is never looked at
           mbar_arrive(p_full(x, 0));
           mbar_arrive(p_full(x, 1));
           continue;
@@ -461,31 +519,17 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
         float sc[BN];
 #pragma unroll
         for (int c = 0; c < BN; c += 32) tmem_ld32_issue(t_s + c, sc + c);
-        const int t = u.t0 + j;
-        const bool nodes = t >= u.r.n_pre;
-        const int key0 = nodes ? (t - u.r.n_pre) * BN : (u.r.first + t) * BN;
-        const uint32_t missing = k_holes[(g0 + j) % kRing];
-        uint32_t sees[4];
-        if (nodes) {
+        const uint32_t missing = k_holes[(p - begin + j) % kRing];
+        if (missing) {
+          for (int b = 0; b < BN / ta.rows_box; ++b)
+            if ((missing >> b) & 1u) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int k = key0 + 32 * i;
-            sees[i] = mine && k < u.r.nk ? mask[k >> 5] & bits(0, u.r.nk - k) : 0u;
-          }
-        } else {
-          const int from = max(u.r.lo, after + 1) - key0, to = u.r.prefix - key0;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) sees[i] = bits(from - 32 * i, to - 32 * i);
-          if (missing) {
-            for (int b = 0; b < BN / ta.rows_box; ++b)
-              if ((missing >> b) & 1u) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) sees[i] &= ~bits(b * ta.rows_box - 32 * i, (b + 1) * ta.rows_box - 32 * i);
-              }
-          }
+              for (int i = 0; i < 4; ++i) sees[i] &= ~bits(b * ta.rows_box - 32 * i, (b + 1) * ta.rows_box - 32 * i);
+            }
         }
+        const bool all = (sees[0] & sees[1] & sees[2] & sees[3]) == 0xffffffffu;
         tmem_wait_ld();
-        if (__any_sync(0xffffffffu, (sees[0] & sees[1] & sees[2] & sees[3]) != 0xffffffffu)) {
+        if (__any_sync(0xffffffffu, !all)) {
 #pragma unroll
           for (int i = 0; i < BN; ++i)
             if (!((sees[i >> 5] >> (i & 31)) & 1u)) sc[i] = -INFINITY;
@@ -508,7 +552,7 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
           l *= alpha;
         }
         if (j > j0 && __any_sync(0xffffffffu, grow)) {
-#pragma unroll
+#pragma unroll 1
           for (int c = 0; c < HD; c += 16) {
             float r[16];
             tmem_ld8_issue(t_o + c, r);
@@ -546,69 +590,67 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
         l += l0 + l1;
       }
       const bool have = j0 < nt;                                 // this half had a tile
-      if (have && ok) ok = mbar_wait_f(o_done(x), (uint32_t)(n_o & 1), failed);
+      // (the tiles' loop needs all registers: what comes now keeps nothing across it)
+      const int x_now = again(x), row_now = again(row);
+      if (ok && have) ok = mbar_wait_f(o_done(x_now), (uint32_t)(n_o & 1), failed);
+      if (!ok) break;
       n_o += have;
       tc_fence_after();
-      // rows of one item that lie in both halves are added up here: half x writes the columns [x HD / 2, + HD / 2)
+      // rows of one item that lie in both halves are added up here: half x_now writes the columns [x_now HD / 2, + HD / 2)
       float w_own = 1.f, w_other = 0.f;
       if (!two) {
-        stats[x][row] = make_float2(m, l);
-        both_halves();
-        const float2 o = stats[x ^ 1][row];
+        stats[x_now][row_now] = make_float2(m, l);
+        meet();
+        if (!ok) break;
+        const float2 o = stats[x_now ^ 1][row_now];
         const float m_all = fmaxf(m, o.x), base = m_all == -INFINITY ? 0.f : m_all;
         w_own = ex2_approx(m - base);
         w_other = ex2_approx(o.x - base);
         l = l * w_own + o.y * w_other;
         m = m_all;
       }
-      const bool other_has = !two && (x ^ 1) < nt;
-      const bool whole = u.t0 == 0 && u.t1 == u.r.tiles;
-      const int slot = (2 * (int)blockIdx.x + (u.t0 == 0 ? 1 : 0)) * 2 + (two ? x : 0);
-      const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
-      const bool odd = ok && odd_values[n_piece % kRing] != 0;
-      const int head = u.kvh * a.group + row % a.group;
-      bf16* out = (bf16*)a.out + (u.r.start + node) * a.out_stride + (size_t)head * HD;
+      const bool other_has = !two && (x_now ^ 1) < nt;
+      const bool whole = nt == u->tiles;
+      const bool odd = odd_values[i_piece % kRing] != 0;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      bf16* out = (bf16*)a.out + (u->start + node) * a.out_stride + (size_t)(u->kvh * a.group + row_now % a.group) * HD;
+      const int slot = (2 * (int)blockIdx.x + (u->t0 == 0 ? 1 : 0)) * 2 + (two ? x_now : 0);
       float* part = a.partials + slot * partial_floats(BM, HD);
-      constexpr int kCols = HD / 2;
-      for (int part_of = 0; part_of < (two ? 2 : 1); ++part_of) {
-        const int c0 = (two ? part_of : x) * kCols;
-        if (!any_mine || !ok) continue;
-        float o[kCols];
-        if (have) {
+      constexpr int kCols = HD / 2, kChunk = 8;
+      const int c_begin = two ? 0 : x_now * kCols, c_end = two ? HD : c_begin + kCols;
+#pragma unroll 1
+      for (int c0 = c_begin; c0 < c_end && any_mine; c0 += kChunk) {
+        float o[kChunk], r[kChunk];
 #pragma unroll
-          for (int c = 0; c < kCols; c += 8) tmem_ld8_issue(t_o + c0 + c, o + c);
-          tmem_wait_ld();
+        for (int c = 0; c < kChunk; c += 8) {
+          if (have) tmem_ld8_issue(t_o + c0 + c, o + c);
+          if (other_has) tmem_ld8_issue((t_o ^ 128u) + c0 + c, r + c);
         }
+        tmem_wait_ld();
 #pragma unroll
-        for (int c = 0; c < kCols; ++c) o[c] = have ? o[c] * w_own : 0.f;
-        if (other_has) {
-          const uint32_t t_other = t_row + kOCol + (x ^ 1) * 128 + c0;
-          float r[kCols];
-#pragma unroll
-          for (int c = 0; c < kCols; c += 8) tmem_ld8_issue(t_other + c, r + c);
-          tmem_wait_ld();
-#pragma unroll
-          for (int c = 0; c < kCols; ++c) o[c] = fmaf(r[c], w_other, o[c]);
-        }
+        for (int c = 0; c < kChunk; ++c) o[c] = (have ? o[c] * w_own : 0.f) + (other_has ? r[c] * w_other : 0.f);
         if (odd && mine) {
           // values that were set to zero, for the rows that see them (rare: nothing here is made to be fast)
-          for (int t = u.t0; t < u.t1; ++t) {
-            const bool nodes = t >= u.r.n_pre;
-            const int key0 = nodes ? (t - u.r.n_pre) * BN : (u.r.first + t) * BN;
-            if (!nodes && !(a.window > 0 && key0 <= u.r.prefix + u.r.n - 1 - a.window)) continue;
-            for (int k = key0; k < key0 + BN; ++k) {
+#pragma unroll 1
+          for (int t = u->t0; t < u->t0 + nt; ++t) {
+            int key0, lo, hi;
+            rows_seen(u, t, key0, lo, hi);
+            if (!seen_by_some(a, u, t, key0)) continue;
+            const bool nodes = t >= u->n_pre;
+#pragma unroll 1
+            for (int k = key0 + lo; k < key0 + hi; ++k) {
               const bf16* src;
               if (nodes) {
-                if (k >= u.r.nk || !((mask[k >> 5] >> (k & 31)) & 1u)) continue;
-                src = (const bf16*)a.v + (u.r.start + k) * a.v_stride + (size_t)u.kvh * HD;
+                if (!((mask_word(k >> 5) >> (k & 31)) & 1u)) continue;
+                src = (const bf16*)a.v + (u->start + k) * a.v_stride + (size_t)u->kvh * HD;
               } else {
-                if (k < u.r.lo || k >= u.r.prefix || k <= after) continue;
-                const int page = a.block_table[(size_t)u.s * a.max_blocks + (k >> ta.block_shift)];
+                if (k <= after) continue;
+                const int page = a.block_table[(size_t)u->s * a.max_blocks + (k >> ta.block_shift)];
                 if (page < 0 || page >= a.pages) continue;
-                src = (const bf16*)a.cache + page * a.page_stride + a.v_off + ((size_t)u.kvh * a.block_size + (k & (a.block_size - 1))) * HD;
+                src = (const bf16*)a.cache + page * a.page_stride + a.v_off + ((size_t)u->kvh * a.block_size + (k & (a.block_size - 1))) * HD;
               }
 #pragma unroll
-              for (int c = 0; c < kCols; ++c) {
+              for (int c = 0; c < kChunk; ++c) {
                 const float v = __bfloat162float(src[c0 + c]);
                 if (!(fabsf(v) <= 3.4e38f)) o[c] += v;
               }
@@ -618,10 +660,10 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
         if (!mine) continue;
         if (whole) {
 #pragma unroll
-          for (int c = 0; c < kCols; ++c) o[c] *= inv;
+          for (int c = 0; c < kChunk; ++c) o[c] *= inv;
           if (ta.wide_out) {
 #pragma unroll
-            for (int c = 0; c < kCols; c += 8) {
+            for (int c = 0; c < kChunk; c += 8) {
               uint4 w;
               w.x = pack_bf16(o[c], o[c + 1]);
               w.y = pack_bf16(o[c + 2], o[c + 3]);
@@ -631,25 +673,27 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
             }
           } else {
 #pragma unroll
-            for (int c = 0; c < kCols; ++c) out[c0 + c] = __float2bfloat16_rn(o[c]);
+            for (int c = 0; c < kChunk; ++c) out[c0 + c] = __float2bfloat16_rn(o[c]);
           }
         } else {
 #pragma unroll
-          for (int c = 0; c < kCols; c += 4)
-            *reinterpret_cast<float4*>(part + ((size_t)((c0 + c) / 4) * BM + row) * 4) = make_float4(o[c], o[c + 1], o[c + 2], o[c + 3]);
+          for (int c = 0; c < kChunk; c += 4)
+            *reinterpret_cast<float4*>(part + ((size_t)((c0 + c) / 4) * BM + row_now) * 4) = make_float4(o[c], o[c + 1], o[c + 2], o[c + 3]);
         }
       }
-      if (!whole && mine && (two || x == 0)) {
-        part[(size_t)HD * BM + row] = m;
-        part[(size_t)HD * BM + BM + row] = l;
-        if (row == 0 && u.t0 == 0)
-          a.notes[2 * blockIdx.x + (two ? x : 0)] = make_int4(u.s, u.kvh, item * rows_item, min(ta.nodes_per_item, u.r.n - item * ta.nodes_per_item) * a.group
-                                                              | (block_of_tile(work, p + u.r.tiles - 1) << 8));
+      if (!whole && mine && (two || x_now == 0)) {
+        part[(size_t)HD * BM + row_now] = m;
+        part[(size_t)HD * BM + BM + row_now] = l;
+        if (row_now == 0 && u->t0 == 0) {
+          const int item = u->item + (two ? x_now : 0);
+          a.notes[2 * blockIdx.x + (two ? x_now : 0)] = make_int4(u->s, u->kvh, item * rows_item, min(ta.nodes_per_item, u->n - item * ta.nodes_per_item) * a.group
+                                                              | (block_of_tile(offs[a.n_seqs], u->p + u->tiles - 1) << 8));
+        }
       }
       // the next piece's first P V overwrites the outputs, of both halves where they were added up
       tc_fence_before();
-      if (!two) both_halves();
-      g0 += nt;
+      if (!two) meet();
+      if (!ok) break;
       p += nt;
     }
   }
