@@ -31,13 +31,14 @@ __global__ void __launch_bounds__(kThreads) attention_tree_kernel(Args a, bool w
   float* kv = qs + kRows * kPitch;                               // [kKeys][kPitch]
   float* ps = kv + kKeys * kPitch;                               // [kRows][kKeys + 4]
   int* there = (int*)(ps + kRows * (kKeys + 4));                 // [kKeys] whether any row may see the key
-  int* offs = there + kKeys;                                     // [n_seqs + 1]
+  Lengths* lens = (Lengths*)(there + kKeys);                     // [n_seqs]
+  int* offs = (int*)(lens + a.n_seqs);                           // [n_seqs + 1]
   __shared__ int scratch[32];
   constexpr int kPP = kKeys + 4;
   pdl_launch_dependents();
   pdl_wait();
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-  add_up_work<kKeys>(a, kRows, 1, offs, scratch);
+  add_up_work<kKeys>(a, kRows, 1, lens, offs, scratch);
   int begin, end;
   share_of_block(offs[a.n_seqs], begin, end);
   const int b = blockIdx.x;
@@ -45,7 +46,7 @@ __global__ void __launch_bounds__(kThreads) attention_tree_kernel(Args a, bool w
   __syncthreads();
   const T* q = (const T*)a.q;
   for (int p = begin; p < end;) {
-    const Piece u = piece_at<kKeys>(a, offs, kRows, 1, p, end);
+    const Piece u = piece_at<kKeys>(a, lens, offs, 1, p, end);
     const int row0 = u.item * kRows, rows = min(kRows, u.r.n * a.group - row0);
     const int* table = a.block_table + (size_t)u.s * a.max_blocks;
     __syncthreads();
@@ -220,7 +221,7 @@ __global__ void __launch_bounds__(kThreads) attention_tree_kernel(Args a, bool w
 
 template <typename T, int HDP>
 static int launch(const Args& a, int blocks, bool wide, cudaStream_t st) {
-  const size_t smem = sizeof(float) * ((size_t)(kRows + kKeys) * (HDP + 4) + kRows * (kKeys + 4) + kKeys) + sizeof(int) * (a.n_seqs + 1);
+  const size_t smem = sizeof(float) * ((size_t)(kRows + kKeys) * (HDP + 4) + kRows * (kKeys + 4) + kKeys) + work_bytes(a.n_seqs);
   static bool raised[64] = {};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);

@@ -17,7 +17,7 @@
 namespace lmsf {
 namespace tree {
 
-constexpr int kMaxSeqs = 4096;             // requests of a step (their work is added up in shared memory)
+constexpr int kMaxSeqs = 1024;             // requests of a step (what is known of each lies in shared memory)
 
 struct Args {
   const void* q; long long q_stride;
@@ -35,36 +35,49 @@ struct Args {
 };
 
 struct Request { int start, n, nk, prefix, lo, first, n_pre, tiles, items; };
+struct __align__(16) Lengths { int start, n, prefix, items; };
 
-// kKeys keys a tile; an item has `rows` rows.
+// An item has `rows` rows.
+__device__ __forceinline__ Lengths lengths(const Args& a, int s, int rows) {
+  Lengths l;
+  const int from = a.cu_q[s], to = a.cu_q[s + 1], prefix = a.prefix_len[s];
+  l.start = min(max(from, 0), a.n_rows);
+  l.n = min(max(to - l.start, 0), a.n_rows - l.start);
+  l.prefix = (int)min((long long)max(prefix, 0), (long long)a.max_blocks * a.block_size);
+  l.items = (l.n * a.group + rows - 1) / rows;
+  return l;
+}
+// kKeys keys a tile.
 template <int kKeys>
-__device__ __forceinline__ Request request(const Args& a, int s, int rows) {
+__device__ __forceinline__ Request request(const Args& a, const Lengths& l) {
   Request r;
-  r.start = min(max(a.cu_q[s], 0), a.n_rows);
-  r.n = min(max(a.cu_q[s + 1] - r.start, 0), a.n_rows - r.start);
+  r.start = l.start;
+  r.n = l.n;
+  r.prefix = l.prefix;
+  r.items = l.items;
   r.nk = min(r.n, 32 * a.words);                                 // a node behind the mask's last bit is seen by nobody
-  r.prefix = (int)min((long long)max(a.prefix_len[s], 0), (long long)a.max_blocks * a.block_size);
   r.lo = a.window > 0 ? min(max(r.prefix - a.window + 1, 0), r.prefix) : 0;    // a node's position is the prefix or behind it
   r.first = r.lo / kKeys;
   r.n_pre = (r.prefix + kKeys - 1) / kKeys - r.first;
   if (r.lo >= r.prefix) r.n_pre = 0;
   r.tiles = max(1, r.n_pre + (r.nk + kKeys - 1) / kKeys);        // (rows that see nothing are still written)
-  r.items = (r.n * a.group + rows - 1) / rows;
   return r;
 }
 
-// offs[s] = tiles before request s, for 0 <= s <= n_seqs; by all threads of the block (a multiple of 32, at most 1024).
+// What a block keeps of the step in shared memory: all[s], and offs[s] = tiles before request s, for 0 <= s <= n_seqs.
+__host__ __device__ __forceinline__ size_t work_bytes(int n_seqs) { return (size_t)n_seqs * sizeof(Lengths) + (size_t)(n_seqs + 1) * sizeof(int); }
+// By all threads of the block (a multiple of 32, at most 1024).
 template <int kKeys>
-__device__ __forceinline__ void add_up_work(const Args& a, int rows, int items_per_unit, int* offs, int* scratch) {
+__device__ __forceinline__ void add_up_work(const Args& a, int rows, int items_per_unit, Lengths* all, int* offs, int* scratch) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = blockDim.x >> 5;
   const int per = (a.n_seqs + blockDim.x - 1) / blockDim.x;
   const int s0 = min(tid * per, a.n_seqs), s1 = min(s0 + per, a.n_seqs);
   int sum = 0;
   for (int s = s0; s < s1; ++s) {
-    const Request r = request<kKeys>(a, s, rows);
-    const int w = r.tiles * ((r.items + items_per_unit - 1) / items_per_unit) * a.n_kv;
+    const Lengths l = lengths(a, s, rows);
+    all[s] = l;
     offs[s] = sum;
-    sum += w;
+    sum += request<kKeys>(a, l).tiles * ((l.items + items_per_unit - 1) / items_per_unit) * a.n_kv;
   }
   int x = sum;
 #pragma unroll
@@ -78,9 +91,9 @@ __device__ __forceinline__ void add_up_work(const Args& a, int rows, int items_p
   for (int w = 0; w < warp; ++w) base += scratch[w];
   for (int s = s0; s < s1; ++s) offs[s] += base;
   if (tid == 0) {
-    int all = 0;
-    for (int w = 0; w < nw; ++w) all += scratch[w];
-    offs[a.n_seqs] = all;
+    int total = 0;
+    for (int w = 0; w < nw; ++w) total += scratch[w];
+    offs[a.n_seqs] = total;
   }
   __syncthreads();
 }
@@ -109,15 +122,15 @@ __device__ __forceinline__ int request_at(const int* offs, int n_seqs, int p) {
 // A block's share of one unit: tiles [t0, t1) of the unit's.
 struct Piece { int s, kvh, item, t0, t1; Request r; };
 template <int kKeys>
-__device__ __forceinline__ Piece piece_at(const Args& a, const int* offs, int rows, int items_per_unit, int p, int end) {
+__device__ __forceinline__ Piece piece_at(const Args& a, const Lengths* all, const int* offs, int items_per_unit, int p, int end) {
   Piece x;
   x.s = request_at(offs, a.n_seqs, p);
-  x.r = request<kKeys>(a, x.s, rows);
+  x.r = request<kKeys>(a, all[x.s]);
   const int units = (x.r.items + items_per_unit - 1) / items_per_unit, rem = p - offs[x.s], u = rem / x.r.tiles;
-  x.t0 = rem % x.r.tiles;
+  x.t0 = rem - u * x.r.tiles;
   x.t1 = min(x.r.tiles, x.t0 + (end - p));
   x.kvh = u / units;
-  x.item = (u % units) * items_per_unit;                         // the unit's first item: its neighbours read the same keys
+  x.item = (u - x.kvh * units) * items_per_unit;                         // the unit's first item: its neighbours read the same keys
   return x;
 }
 

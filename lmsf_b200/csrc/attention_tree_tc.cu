@@ -9,12 +9,15 @@
 //   * a unit of two items: both take every tile, each its own queries;
 //   * a unit of one item: the two halves of the block take the tiles in turn with the same queries, each with an output and a maximum of
 //     its own, and add up at the end, so that one half's products run beside the other's softmax here too.
-// Warps: 0-3 and 4-7 softmax of half 0 and 1, a row per thread; 8 and 9 bring tiles of k and v by tensor-map copies (a box per page, or
-// 32 rows of the step's own k and v for drafted tokens); 10 issues the products; 11 brings the queries and goes over those
-// tiles of v that some row must not see all of: rows that nobody sees are cleared, and in a tile whose rows not every row sees
-// (drafted tokens, the edge of a window) values that are no numbers are set to zero and remembered, since their zero weights would
-// make NaN of them; the rows that do see them get them added at the end.
-// Tensor memory: S of half x (128 columns, P over the first 64 of them as bfloat16 pairs) at 128 x, its output at 256 + 128 x.
+// Warps: 0-3 and 4-7 softmax of half 0 and 1, a row per thread; 8 works out the pieces and brings queries and tiles of k by tensor-map copies (a
+// box per page, or 32 rows of the step's own k for drafted tokens); 9 brings tiles of v and goes over those that some row must not see
+// all of: rows that nobody sees are cleared, and in a tile whose rows not every row sees (drafted tokens, the edge of a window)
+// values that are no numbers are set to zero and remembered, since their zero weights would make NaN of them; the rows that do
+// see them get them added at the end; 10 issues the products, the halves in turn, so that one half's products run beside the other's softmax
+// (a warp for each half let both halves do the same at the same time).
+// Tensor memory: S of half x (128 columns, P over the first 64 of them as bfloat16 pairs) at 128 x, its output at 256 + 128 x.  (Steps of
+// 64 keys, whose scores would have two places to be in, were slower: a product of 64 columns takes the tensor cores as long as one
+// of 128, whose left operand has as many rows to be read.)
 // Weights are rounded to bfloat16 for P V (2^-8 relative, the operand type of the product); sums, maxima, outputs are float32.
 // Every wait is bounded (the two halves meet at an mbarrier too); when one runs out the block raises the error word (code 3) and ends.
 #include <cstring>
@@ -35,7 +38,7 @@ using namespace lmsf::tc;
 
 constexpr int HD = LMSF_HEAD_DIM;
 static_assert(HD % 16 == 0 && HD >= 64 && HD <= 128, "head sizes 64 to 128 in steps of 16");
-constexpr int BM = 128, BN = 128;
+constexpr int BM = 128, BN = 128;              // rows of an item, keys of a tile
 constexpr int kHB = (HD + 63) / 64;            // 64-wide blocks of the head dimension
 constexpr int kTileBytes = kHB * BN * 128;     // one tile of q, k or v
 constexpr int kStages = HD > 64 ? 2 : 4;       // tiles of k in flight, and of v
@@ -44,9 +47,10 @@ constexpr uint32_t kTmemCols = 512, kOCol = 256;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescale = 8.0f;               // the output is rescaled when the maximum grew by more than this (log2 units)
 constexpr int kThreadsTotal = 384, kHalf = 128;
-constexpr int kRegsSoftmax = 224, kRegsOther = 56;
+constexpr int kRegsSoftmax = 216, kRegsOther = 72;
 constexpr int kRing = 16;                      // notes of tiles and of pieces that warps leave one another
 static_assert(kStages + 4 <= kRing, "notes are read before they are written again");
+static_assert(kStages <= 4, "warp 9 may be this far ahead of the notes");
 
 struct TcArgs {
   Args a;
@@ -93,15 +97,29 @@ __device__ __forceinline__ void tmem_st8_issue(uint32_t taddr, const float* r) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n"
                ::"r"(taddr), "f"(r[0]), "f"(r[1]), "f"(r[2]), "f"(r[3]), "f"(r[4]), "f"(r[5]), "f"(r[6]), "f"(r[7]) : "memory");
 }
+// Waits let the warp sleep until the barrier's phase is over (10 us at a time, a second or so in all).  Without the hint a wait comes back and
+// looks again after a moment, and the looks of the warps that wait take the softmax warps beside them a third of their issue slots.
+constexpr uint32_t kSleepNs = 10000;
+constexpr int kSleeps = 1 << 17;
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* failed) {
+  uint32_t done = 0;
+  for (int it = 0; it < kSleeps && !done; ++it) {
+    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\nselp.b32 %0, 1, 0, p;\n}\n"
+                 : "=r"(done) : "r"(bar), "r"(parity), "r"(kSleepNs) : "memory");
+    if (!done && *failed) return false;
+  }
+  if (!done) *failed = 1;
+  return done != 0;
+}
+// the same without the early way out: a block's own copies land before it ends
+__device__ __forceinline__ void bar_drain(uint32_t bar, uint32_t parity) {
+  int never = 0;
+  bar_wait(bar, parity, &never);
+}
 __device__ __forceinline__ void tma_load_box_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t mbar) {
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
       ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(mbar) : "memory");
-}
-// the same value, which the compiler takes for another: what follows from it is worked out here and not kept from further up
-__device__ __forceinline__ int again(int v) {
-  asm volatile("" : "+r"(v));
-  return v;
 }
 // bits [lo, hi) of a word
 __device__ __forceinline__ uint32_t bits(int lo, int hi) {
@@ -113,7 +131,7 @@ __device__ __forceinline__ uint32_t bits(int lo, int hi) {
 
 // What the warps of a block need to know of a piece, left in shared memory by warp 11 a piece ahead.  They read it where they need it:
 // held in registers it would not fit beside a row's scores, nor into what the other warps keep.
-struct __align__(16) PieceNote { int s, kvh, item, t0, nt, start, n, nk, prefix, lo, first, n_pre, tiles, two, p, pad; };
+struct __align__(16) PieceNote { int s, kvh, item, t0, nt, start, n, nk, prefix, lo, first, n_pre, tiles, two, last, pad; };   // last: the block that ends the unit
 typedef const volatile PieceNote* NotePtr;
 // Rows [lo, hi) of a tile are seen by some row of the piece's request; none of the others is multiplied, but for those that share a step
 // of 16 with them.
@@ -123,6 +141,11 @@ __device__ __forceinline__ void rows_seen(NotePtr u, int t, int& key0, int& lo, 
   lo = nodes ? 0 : max(u->lo - key0, 0);
   hi = min((nodes ? u->nk : u->prefix) - key0, BN);
 }
+// What the warps need to know of a tile: boxes of k that are not there, which steps of 16 keys somebody sees (from, to), and whether every
+// row sees every key.
+constexpr uint32_t kAllSeen = 0x80000000u;
+__device__ __forceinline__ int from16(uint32_t note) { return (note >> 16) & 15; }
+__device__ __forceinline__ int to16(uint32_t note) { return (note >> 20) & 15; }
 // Seen by some row, but perhaps not by every one: drafted tokens, and cached ones at the edge of a window.
 __device__ __forceinline__ bool seen_by_some(const Args& a, NotePtr u, int t, int key0) {
   return t >= u->n_pre || (a.window > 0 && key0 <= u->prefix + u->n - 1 - a.window);
@@ -134,18 +157,19 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
                                                                              const __grid_constant__ CUtensorMap cache_map) {
   const Args& a = ta.a;
   extern __shared__ unsigned char smem_raw[];
-  // k_full[kStages], k_empty, v_full, v_fixed, v_empty [kStages each], s_full[2], p_full[2][half of P], o_done[2], q_full[2], q_free[2],
-  // noted[kRing], met
-  __shared__ __align__(8) uint64_t bars[5 * kStages + 13 + kRing];
+  // k_full[kStages], k_empty, v_full, v_fixed, v_empty [kStages each], s_full[2], p_full[2][half of P], o_done[2], q_full, q_free, met,
+  // noted[kRing]
+  __shared__ __align__(8) uint64_t bars[5 * kStages + 11 + kRing];
   __shared__ PieceNote notes[kRing];
   __shared__ uint32_t tmem_base_mem;
   __shared__ int failed_mem, scratch[32];
-  __shared__ uint32_t k_holes[kRing], v_holes[kRing];    // boxes of the tile whose page is not there
+  __shared__ uint32_t tile_notes[kRing], v_holes[kRing]; // of a tile of k; boxes of a tile of v that are not there
   __shared__ int odd_values[kRing];                      // of a piece: values that are no numbers were set to zero
   __shared__ float2 stats[2][kHalf];                     // maximum and sum of a half's rows (a unit of one item)
   volatile int* failed = &failed_mem;
   const uint32_t smem = (smem_addr(smem_raw) + 1023u) & ~1023u;
-  int* offs = (int*)(smem_raw + (smem - smem_addr(smem_raw)) + kOffWork);
+  Lengths* lens = (Lengths*)(smem_raw + (smem - smem_addr(smem_raw)) + kOffWork);
+  int* offs = (int*)(lens + a.n_seqs);
   const uint32_t sQ = smem, sK = smem + kOffK, sV = smem + kOffV, bar0 = smem_addr(&bars[0]);
   auto k_full = [&](int s) { return bar0 + 8u * s; };
   auto k_empty = [&](int s) { return bar0 + 8u * (kStages + s); };
@@ -155,14 +179,14 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
   auto s_full = [&](int x) { return bar0 + 8u * (5 * kStages + x); };
   auto p_full = [&](int x, int h) { return bar0 + 8u * (5 * kStages + 2 + 2 * x + h); };
   auto o_done = [&](int x) { return bar0 + 8u * (5 * kStages + 6 + x); };
-  auto q_full = [&](int x) { return bar0 + 8u * (5 * kStages + 8 + x); };
-  auto q_free = [&](int x) { return bar0 + 8u * (5 * kStages + 10 + x); };
-  const uint32_t met = bar0 + 8u * (5 * kStages + 12 + kRing);
-  auto noted = [&](int i) { return bar0 + 8u * (5 * kStages + 12 + i % kRing); };
+  const uint32_t q_full = bar0 + 8u * (5 * kStages + 8), q_free = q_full + 8u, met = q_full + 16u;
+  auto noted = [&](int i) { return bar0 + 8u * (5 * kStages + 11 + i % kRing); };
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   pdl_launch_dependents();
   if (tid == 0) {
+    // s_full and o_done take the products' completion and an arrival of the thread that issued them: what that thread had seen before (a
+    // tile's note, odd values) is then seen by those who wait there.  p_full takes an arrival of every warp of the half.
     for (int s = 0; s < kStages; ++s) {
       mbar_init(k_full(s), 1);
       mbar_init(k_empty(s), 1);
@@ -171,19 +195,21 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
       mbar_init(v_empty(s), 1);
     }
     for (int x = 0; x < 2; ++x) {
-      // the products' completion and an arrival of the thread that issued them: what that thread had seen before (notes of the
-      // tile) is then seen by those who wait here
       mbar_init(s_full(x), 2);
       mbar_init(o_done(x), 2);
-      mbar_init(p_full(x, 0), kHalf);
-      mbar_init(p_full(x, 1), kHalf);
-      mbar_init(q_full(x), 1);
-      mbar_init(q_free(x), 1);
+      mbar_init(p_full(x, 0), kHalf / 32);
+      mbar_init(p_full(x, 1), kHalf / 32);
     }
+    mbar_init(q_full, 1);
+    mbar_init(q_free, 1);
     for (int i = 0; i < kRing; ++i) mbar_init(noted(i), 1);
     mbar_init(met, 8);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     failed_mem = 0;
+  }
+  if (warp == 8 && lane < 4) {
+    const CUtensorMap* m = lane == 0 ? &q_map : lane == 1 ? &k_map : lane == 2 ? &v_map : &cache_map;
+    asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
   }
   if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_base_mem)), "r"(kTmemCols));
@@ -191,7 +217,7 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
   }
   pdl_wait();
   const int rows_item = ta.nodes_per_item * a.group;
-  add_up_work<BN>(a, rows_item, 2, offs, scratch);
+  add_up_work<BN>(a, rows_item, 2, lens, offs, scratch);
   if (tid < 2) a.notes[2 * blockIdx.x + tid] = make_int4(-1, 0, 0, 0);
   tc_fence_before();
   __syncthreads();
@@ -202,178 +228,56 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
   share_of_block(work, begin, end);
   // the note of the block's i-th piece
   auto note_of = [&](int i, bool& ok) -> NotePtr {
-    if (ok) ok = mbar_wait_f(noted(i), (uint32_t)((i / kRing) & 1), failed);
+    if (ok) ok = bar_wait(noted(i), (uint32_t)((i / kRing) & 1), failed);
     return &notes[i % kRing];
   };
 
   if (warp >= 8) {
     regs_dec<kRegsOther>();
-    if (warp == 8 || warp == 9) {
-      // ------------------------------------------------------------------ producers: warp 8 of k, warp 9 of v
-      const bool is_v = warp == 9;
-      const uint32_t ring = is_v ? sV : sK;
-      const CUtensorMap* own_map = is_v ? &v_map : &k_map;
-      uint32_t* holes = is_v ? v_holes : k_holes;
-      auto full = [&](int s) { return is_v ? v_full(s) : k_full(s); };
-      auto empty = [&](int s) { return is_v ? v_empty(s) : k_empty(s); };
-      const int n_box = BN / ta.rows_box;
+    const int n_box = BN / ta.rows_box;
+    // the page of a lane's box of tile t, whose first key is key: -2 where nobody sees the box, -1 where it is not there
+    auto page_of = [&](NotePtr u, int t) {
+      const int key = (u->first + t) * BN + lane * ta.rows_box;
+      if (t >= u->t0 + u->nt || t >= u->n_pre || lane >= n_box || key >= u->prefix || key + ta.rows_box <= u->lo) return -2;
+      const int page = a.block_table[(size_t)u->s * a.max_blocks + (key >> ta.block_shift)];       // (the prefix ends inside the table)
+      return page >= 0 && page < a.pages ? page : -1;
+    };
+    // tile t of k or v into `dst`, by the whole warp
+    auto bring = [&](NotePtr u, int t, int page, bool is_v, uint32_t dst, uint32_t bar) {
+      if (t >= u->n_pre) {                                       // drafted tokens: boxes of 32 rows
+        const int j0 = (t - u->n_pre) * BN, boxes = (min(BN, u->nk - j0) + 31) / 32;
+        if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(boxes * 32 * 128 * kHB));
+        __syncwarp();
+        if (lane < boxes) {
+#pragma unroll
+          for (int hb = 0; hb < kHB; ++hb)
+            tma_load_box_3d(dst + hb * (BN * 128) + lane * (32 * 128), is_v ? &v_map : &k_map, hb * 64, u->kvh, u->start + j0 + lane * 32, bar);
+        }
+      } else {
+        const uint32_t here = __ballot_sync(0xffffffffu, page >= 0);
+        if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(__popc(here) * ta.rows_box * 128 * kHB));
+        __syncwarp();
+        if (page >= 0) {
+          const int slot = ((u->first + t) * BN + lane * ta.rows_box) & (a.block_size - 1);
+#pragma unroll
+          for (int hb = 0; hb < kHB; ++hb)
+            tma_load_box(dst + hb * (BN * 128) + lane * ta.rows_box * 128, &cache_map, hb * 64, slot, (is_v ? a.n_kv : 0) + u->kvh, page, bar);
+        }
+      }
+    };
+    if (warp == 8) {
+      // ------------------------------------------------------------------ notes, queries, tiles of k
       int g = 0;                                                 // tiles of the block so far
-      bool ok = true;
-      for (int i = 0, p = begin; p < end && ok; ++i) {
-        NotePtr u = note_of(i, ok);
-        if (!ok) break;
-        const int t0 = u->t0, t1 = t0 + u->nt, n_pre = u->n_pre;
-        const int* table = a.block_table + (size_t)u->s * a.max_blocks;
-        const int head_row = (is_v ? a.n_kv : 0) + u->kvh;
-        // the first key of this lane's box, and its page: -2 where nobody sees the box, -1 where it is not there
-        const int key_base = u->first * BN + lane * ta.rows_box;
-        auto fetch = [&](int t) {
-          const int key = key_base + t * BN;
-          if (t >= t1 || t >= n_pre || lane >= n_box || key >= u->prefix || key + ta.rows_box <= u->lo) return -2;
-          const int page = table[key >> ta.block_shift];         // (the prefix ends inside the table)
-          return page >= 0 && page < a.pages ? page : -1;
-        };
-        int page = fetch(t0);
-        for (int t = t0; t < t1; ++t, ++g) {
-          const int s = g % kStages;
-          if (g >= kStages && !mbar_wait_f(empty(s), (uint32_t)((g / kStages - 1) & 1), failed)) { ok = false; break; }
-          const int next = fetch(t + 1);
-          const uint32_t dst = ring + s * kTileBytes;
-          if (t >= n_pre) {                                      // drafted tokens: boxes of 32 rows
-            const int j0 = (t - n_pre) * BN, boxes = (min(BN, u->nk - j0) + 31) / 32;
-            if (lane == 0) {
-              holes[g % kRing] = 0u;
-              mbar_arrive_expect_tx(full(s), (uint32_t)(boxes * 32 * 128 * kHB));
-            }
-            __syncwarp();
-            if (lane < boxes) {
-#pragma unroll
-              for (int hb = 0; hb < kHB; ++hb)
-                tma_load_box_3d(dst + hb * (BN * 128) + lane * (32 * 128), own_map, hb * 64, u->kvh, u->start + j0 + lane * 32, full(s));
-            }
-          } else {
-            const uint32_t here = __ballot_sync(0xffffffffu, page >= 0), missing = __ballot_sync(0xffffffffu, page == -1);
-            if (lane == 0) {
-              holes[g % kRing] = missing;
-              mbar_arrive_expect_tx(full(s), (uint32_t)(__popc(here) * ta.rows_box * 128 * kHB));
-            }
-            __syncwarp();
-            if (page >= 0) {
-              const int slot = (key_base + t * BN) & (a.block_size - 1);
-#pragma unroll
-              for (int hb = 0; hb < kHB; ++hb)
-                tma_load_box(dst + hb * (BN * 128) + lane * ta.rows_box * 128, &cache_map, hb * 64, slot, head_row, page, full(s));
-            }
-          }
-          page = next;
-        }
-        p += t1 - t0;
-      }
-      // no copy of this block may be in flight when it ends
-      for (int i = max(0, g - kStages); i < g; ++i) mbar_wait_drain(full(i % kStages), (uint32_t)((i / kStages) & 1));
-      // nor an arrival on its barriers
-      for (int i = max(0, g - kStages); i < g && ok; ++i) ok = mbar_wait_f(empty(i % kStages), (uint32_t)((i / kStages) & 1), failed);
-    } else if (warp == 10) {
-      // ------------------------------------------------------------------ tensor-core issue
-      constexpr uint32_t idesc_s = instr_desc(BM, BN, 0), idesc_o = instr_desc(BM, HD, 1);
-      const bool leader = elect_one();
-      const uint64_t dq0 = smem_desc(sQ, 16, 1024), dk0 = smem_desc(sK, 16, 1024), dv0 = smem_desc(sV, BN * 128, 1024);
-      int g0 = 0, n_p[2] = {0, 0}, n_q[2] = {0, 0};              // tiles of the block before the piece; P's and queries of a half so far
-      bool ok = true;
-      for (int i = 0, p = begin; p < end && ok; ++i) {
-        NotePtr u = note_of(i, ok);
-        if (!ok) break;
-        const bool two = u->two != 0;
-        const int nt = u->nt, t0 = u->t0;
-        auto issue_s = [&](int x, int j) {
-          const uint64_t dq = dq0 + (uint64_t)(((two ? x : 0) * kTileBytes) >> 4), dk = dk0 + (uint64_t)((((g0 + j) % kStages) * kTileBytes) >> 4);
-#pragma unroll
-          for (int ks = 0; ks < HD / 16; ++ks) {
-            const uint32_t off = (ks / 4) * (BN * 128) + (ks % 4) * 32;
-            umma(leader, tmem + x * BN, dq + (off >> 4), dk + (off >> 4), idesc_s, ks > 0);
-          }
-          umma_commit(leader, s_full(x));
-          if (leader) mbar_arrive(s_full(x));
-          if (j == nt - 1) umma_commit(leader, q_free(two ? x : 0));               // the piece's last scores from these queries
-          if (!two || x == 1) umma_commit(leader, k_empty((g0 + j) % kStages));
-        };
-        // (steps [ks0, ks1) of the tile's eight)
-        auto issue_pv = [&](int x, int j, bool first, int h, int ks0, int ks1) {
-          const uint64_t dv = dv0 + (uint64_t)((((g0 + j) % kStages) * kTileBytes) >> 4);
-#pragma unroll
-          for (int k4 = 0; k4 < BN / 32; ++k4) {
-            const int ks = h * (BN / 32) + k4;
-            umma_ts(leader && ks >= ks0 && ks < ks1, tmem + kOCol + x * 128, tmem + x * BN + ks * 8, dv + ((ks * 16 * 128) >> 4), idesc_o,
-                    (!first || ks > ks0) ? 1u : 0u);
-          }
-        };
-        int k_ready = -1;
-        auto k_wait = [&](int j) {
-          if (k_ready >= j) return true;
-          const int g = g0 + j;
-          if (!mbar_wait_f(k_full(g % kStages), (uint32_t)((g / kStages) & 1), failed)) return false;
-          tc_fence_after();
-          k_ready = j;
-          return true;
-        };
-        const int step = two ? 1 : 2;                            // tiles between two of a half
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-          if ((x == 0 || two) && ok) {
-            ok = mbar_wait_f(q_full(x), (uint32_t)(n_q[x] & 1), failed);
-            ++n_q[x];
-          }
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const int j = two ? 0 : x;
-          if (ok && j < nt) {
-            ok = k_wait(j);
-            if (ok) issue_s(x, j);
-          }
-        }
-        for (int j = 0; j < nt && ok; ++j) {
-          const int g = g0 + j, s = g % kStages;
-          int key0, lo, hi;
-          rows_seen(u, t0 + j, key0, lo, hi);
-          ok = mbar_wait_f(v_full(s), (uint32_t)((g / kStages) & 1), failed) && mbar_wait_f(v_fixed(s), (uint32_t)((g / kStages) & 1), failed);
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            if (!ok || (!two && x != (j & 1))) continue;
-            const bool first = j < step;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              if (ok) ok = mbar_wait_f(p_full(x, h), (uint32_t)(n_p[x] & 1), failed);
-              if (!ok) continue;
-              tc_fence_after();
-              issue_pv(x, j, first, h, lo / 16, (hi + 15) / 16);
-            }
-            if (!ok) continue;
-            ++n_p[x];
-            if (!two || x == 1) umma_commit(leader, v_empty(s));
-            if (j + step < nt) {
-              ok = k_wait(j + step);
-              if (ok) issue_s(x, j + step);
-            } else {
-              umma_commit(leader, o_done(x));
-              if (leader) mbar_arrive(o_done(x));
-            }
-          }
-        }
-        g0 += nt;
-        p += nt;
-      }
-    } else {
-      // ------------------------------------------------------------------ notes, queries, and the tiles of v that are not for everybody
-      int g = 0, n_q[2] = {0, 0};
       bool ok = true;
       auto leave_note = [&](int i, int p) {
         if (p >= end) return;
-        const Piece u = piece_at<BN>(a, offs, rows_item, 2, p, end);
+        const Piece u = piece_at<BN>(a, lens, offs, 2, p, end);
         if (lane == 0) {
           volatile PieceNote* n = &notes[i % kRing];
           n->s = u.s; n->kvh = u.kvh; n->item = u.item; n->t0 = u.t0; n->nt = u.t1 - u.t0; n->start = u.r.start; n->n = u.r.n; n->nk = u.r.nk;
           n->prefix = u.r.prefix; n->lo = u.r.lo; n->first = u.r.first; n->n_pre = u.r.n_pre; n->tiles = u.r.tiles;
-          n->two = u.item + 1 < u.r.items; n->p = p;
+          n->two = u.item + 1 < u.r.items;
+          n->last = u.t0 == 0 && u.t1 < u.r.tiles ? block_of_tile(work, p + u.r.tiles - 1) : 0;
           mbar_arrive(noted(i));
         }
         __syncwarp();
@@ -381,25 +285,87 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
       leave_note(0, begin);
       for (int i = 0, p = begin; p < end && ok; ++i) {
         NotePtr u = &notes[i % kRing];                           // (written by this warp)
-        const int nt = u->nt, t0 = u->t0;
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          if (!ok || (x == 1 && !u->two)) continue;
-          if (n_q[x] > 0) ok = mbar_wait_f(q_free(x), (uint32_t)((n_q[x] - 1) & 1), failed);
-          if (!ok) continue;
-          if (lane == 0) {
-            mbar_arrive_expect_tx(q_full(x), (uint32_t)(rows_item * 128 * kHB));
-#pragma unroll
-            for (int hb = 0; hb < kHB; ++hb)
-              tma_load_box_3d(sQ + x * kTileBytes + hb * (BM * 128), &q_map, hb * 64, u->kvh * a.group, u->start + (u->item + x) * ta.nodes_per_item, q_full(x));
-          }
-          ++n_q[x];
-        }
-        if (lane == 0) odd_values[i % kRing] = 0;
-        leave_note(i + 1, p + nt);
+        const int t0 = u->t0, nt = u->nt;
+        // before this warp waits for a piece's scores to free the queries, the note of the piece behind is there: warp 9 runs ahead with v
+        if (i > 0) leave_note(i + 1, p + nt);
+        int page = page_of(u, t0);
         for (int t = t0; t < t0 + nt && ok; ++t, ++g) {
           const int s = g % kStages;
-          ok = mbar_wait_f(v_full(s), (uint32_t)((g / kStages) & 1), failed);
+          if (g >= kStages && !bar_wait(k_empty(s), (uint32_t)((g / kStages - 1) & 1), failed)) { ok = false; break; }
+          const int next = page_of(u, t + 1);
+          const uint32_t missing = __ballot_sync(0xffffffffu, page == -1);
+          if (lane == 0) {
+            int key0, lo, hi;
+            rows_seen(u, t, key0, lo, hi);
+            const bool all = lo == 0 && hi == BN && !missing && !seen_by_some(a, u, t, key0);
+            tile_notes[g % kRing] = missing | ((uint32_t)(lo / 16) << 16) | ((uint32_t)((hi + 15) / 16) << 20) | (all ? kAllSeen : 0u);
+          }
+          __syncwarp();
+          bring(u, t, page, false, sK + s * kTileBytes, k_full(s));
+          page = next;
+          if (t == t0) {                                         // the queries, as soon as the piece before has issued its last scores
+            if (i > 0 && !bar_wait(q_free, (uint32_t)((i - 1) & 1), failed)) { ok = false; ++g; break; }
+            if (lane == 0) {
+              const int items = u->two ? 2 : 1;
+              mbar_arrive_expect_tx(q_full, (uint32_t)(items * rows_item * 128 * kHB));
+              for (int x = 0; x < items; ++x)
+#pragma unroll
+                for (int hb = 0; hb < kHB; ++hb)
+                  tma_load_box_3d(sQ + x * kTileBytes + hb * (BM * 128), &q_map, hb * 64, u->kvh * a.group, u->start + (u->item + x) * ta.nodes_per_item, q_full);
+            }
+            __syncwarp();
+            if (i == 0) leave_note(1, p + nt);
+          }
+        }
+        p += nt;
+        if (p >= end && ok) {                                    // the last queries, and the arrival behind them
+          bar_drain(q_full, (uint32_t)(i & 1));
+          ok = bar_wait(q_free, (uint32_t)(i & 1), failed);
+        }
+      }
+      // no copy of this block may be in flight when it ends, nor an arrival on its barriers
+      for (int i = max(0, g - kStages); i < g; ++i) bar_drain(k_full(i % kStages), (uint32_t)((i / kStages) & 1));
+      for (int i = max(0, g - kStages); i < g && ok; ++i) ok = bar_wait(k_empty(i % kStages), (uint32_t)((i / kStages) & 1), failed);
+      if (!ok) bar_drain(q_full, 0u), bar_drain(q_full, 1u);
+    } else if (warp == 9) {
+      // ------------------------------------------------------------------ tiles of v, and those of them that are not for everybody
+      // a tile is brought when the one whose place it takes has been multiplied, and gone over when it has landed; the two are a
+      // ring apart and lie in different pieces at times
+      int gp = 0, ip = 0, tp = 0, page = -2;                     // the next tile to bring: its number, its piece, its place in the unit
+      bool ok = true;
+      NotePtr up = nullptr;
+      const int total = end - begin;
+      auto bring_next = [&]() {
+        if (gp >= total) return;
+        const int s = gp % kStages;
+        if (gp >= kStages) ok = bar_wait(v_empty(s), (uint32_t)((gp / kStages - 1) & 1), failed);
+        if (ok && (!up || tp >= up->t0 + up->nt)) {
+          if (up) ++ip;
+          up = note_of(ip, ok);
+          if (ok) {
+            tp = up->t0;
+            page = page_of(up, tp);
+          }
+        }
+        if (!ok) return;
+        const int next = page_of(up, tp + 1);
+        const uint32_t missing = __ballot_sync(0xffffffffu, page == -1);
+        if (lane == 0) v_holes[gp % kRing] = missing;
+        bring(up, tp, page, true, sV + s * kTileBytes, v_full(s));
+        page = next;
+        ++tp;
+        ++gp;
+      };
+      for (int k = 0; k + 1 < kStages && ok; ++k) bring_next();
+      int g = 0;
+      for (int i = 0; g < total && ok; ++i) {
+        NotePtr u = note_of(i, ok);
+        if (!ok) break;
+        const int t0 = u->t0, nt = u->nt;
+        if (lane == 0) odd_values[i % kRing] = 0;
+        for (int t = t0; t < t0 + nt && ok; ++t, ++g) {
+          const int s = g % kStages;
+          ok = bar_wait(v_full(s), (uint32_t)((g / kStages) & 1), failed);
           if (!ok) break;
           int key0, lo, hi;
           rows_seen(u, t, key0, lo, hi);
@@ -461,15 +427,90 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
           }
           __syncwarp();
           if (lane == 0) mbar_arrive(v_fixed(s));
+          bring_next();
         }
+      }
+      for (int i = max(0, gp - kStages); i < gp; ++i) bar_drain(v_full(i % kStages), (uint32_t)((i / kStages) & 1));
+      for (int i = max(0, gp - kStages); i < gp && ok; ++i) ok = bar_wait(v_empty(i % kStages), (uint32_t)((i / kStages) & 1), failed);
+    } else if (warp == 10) {
+      // ------------------------------------------------------------------ products
+      constexpr uint32_t idesc_s = instr_desc(BM, BN, 0), idesc_o = instr_desc(BM, HD, 1);
+      const bool leader = elect_one();
+      const uint64_t dq0 = smem_desc(sQ, 16, 1024), dk0 = smem_desc(sK, 16, 1024), dv0 = smem_desc(sV, BN * 128, 1024);
+      int g0 = 0, n_p[2] = {0, 0};                               // tiles of the block before the piece; P's of a half so far
+      bool ok = true;
+      for (int i = 0, p = begin; p < end && ok; ++i) {
+        NotePtr u = note_of(i, ok);
+        if (!ok) break;
+        const bool two = u->two != 0;
+        const int nt = u->nt, every = two ? 1 : 2;               // every: tiles between two of a half
+        auto issue_s = [&](int x, int j) {
+          const int s = (g0 + j) % kStages;
+          const uint64_t dq = dq0 + (uint64_t)(((two ? x : 0) * kTileBytes) >> 4), dk = dk0 + (uint64_t)((s * kTileBytes) >> 4);
+#pragma unroll
+          for (int ks = 0; ks < HD / 16; ++ks) {
+            const uint32_t off = (ks / 4) * (BN * 128) + (ks % 4) * 32;
+            umma(leader, tmem + x * BN, dq + (off >> 4), dk + (off >> 4), idesc_s, ks > 0);
+          }
+          umma_commit(leader, s_full(x));
+          if (leader) mbar_arrive(s_full(x));
+          if (!two || x == 1) {
+            umma_commit(leader, k_empty(s));
+            if (j == nt - 1) umma_commit(leader, q_free);        // (a tile's scores are issued in the tiles' order)
+          }
+        };
+        int k_ready = -1;                                        // tiles of k up to this one are there
+        auto k_wait = [&](int j) {
+          if (k_ready >= j) return;
+          const int g = g0 + j;
+          ok = bar_wait(k_full(g % kStages), (uint32_t)((g / kStages) & 1), failed);
+          tc_fence_after();
+          k_ready = j;
+        };
+        ok = bar_wait(q_full, (uint32_t)(i & 1), failed);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const int j = two ? 0 : x;
+          if (ok && j < nt) k_wait(j);
+          if (ok && j < nt) issue_s(x, j);
+        }
+        for (int j = 0; j < nt && ok; ++j) {
+          const int g = g0 + j, s = g % kStages;
+          const uint32_t note = *(volatile uint32_t*)&tile_notes[g % kRing];
+          const uint64_t dv = dv0 + (uint64_t)((s * kTileBytes) >> 4);
+          ok = bar_wait(v_full(s), (uint32_t)((g / kStages) & 1), failed) && bar_wait(v_fixed(s), (uint32_t)((g / kStages) & 1), failed);
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            if (!ok || (!two && x != (j & 1))) continue;
+            const uint32_t phase = (uint32_t)(n_p[x] & 1);
+            const bool first = j < every;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              if (ok) ok = bar_wait(p_full(x, h), phase, failed);
+              if (!ok) continue;
+              tc_fence_after();
+#pragma unroll
+              for (int k4 = 0; k4 < BN / 32; ++k4) {             // of the steps of 16 keys those that somebody sees
+                const int ks = h * (BN / 32) + k4;
+                umma_ts(leader && ks >= from16(note) && ks < to16(note), tmem + kOCol + x * 128, tmem + x * BN + ks * 8, dv + ((ks * 16 * 128) >> 4), idesc_o,
+                        (!first || ks > from16(note)) ? 1u : 0u);
+              }
+            }
+            if (!ok) continue;
+            ++n_p[x];
+            if (!two || x == 1) umma_commit(leader, v_empty(s));
+            if (j + every < nt) {
+              k_wait(j + every);
+              if (ok) issue_s(x, j + every);
+            } else {
+              umma_commit(leader, o_done(x));
+              if (leader) mbar_arrive(o_done(x));
+            }
+          }
+        }
+        g0 += nt;
         p += nt;
       }
-#pragma unroll
-      for (int x = 0; x < 2; ++x)
-        if (n_q[x] > 0) {
-          mbar_wait_drain(q_full(x), (uint32_t)((n_q[x] - 1) & 1));
-          if (ok) ok = mbar_wait_f(q_free(x), (uint32_t)((n_q[x] - 1) & 1), failed);
-        }
     }
   } else {
     // ------------------------------------------------------------------ softmax of half x
@@ -482,7 +523,7 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
     auto meet = [&]() {
       __syncwarp();
       if (lane == 0) mbar_arrive(met);
-      ok = mbar_wait_f(met, (uint32_t)(n_met & 1), failed);
+      ok = bar_wait(met, (uint32_t)(n_met & 1), failed);
       ++n_met;
     };
     for (int i_piece = 0, p = begin; p < end; ++i_piece) {
@@ -494,42 +535,48 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
       const bool mine = node < u->n, any_mine = __any_sync(0xffffffffu, mine);
       const int after = mine && a.window > 0 ? a.positions[u->start + node] - a.window : -1;
       auto mask_word = [&](int i) { return a.mask[(size_t)(u->start + node) * a.words + i]; };
-      const int nt = u->nt, step = two ? 1 : 2, j0 = two ? 0 : x;
+      const int nt = u->nt, every = two ? 1 : 2;
       float m = -INFINITY, l = 0.f;
-      for (int j = j0; j < nt; j += step, ++n_s) {
-        int key0, lo, hi;
-        rows_seen(u, u->t0 + j, key0, lo, hi);
-        const bool nodes = u->t0 + j >= u->n_pre;
-        // what the row sees of the tile, as bits; the words of a mask are requested before the scores are awaited
-        uint32_t sees[4];
+      const int j0 = two ? 0 : x;
+      const bool have = j0 < nt;                                 // this half has a tile
+      for (int j = j0; j < nt; j += every, ++n_s) {
+        const int t = u->t0 + j;
+        uint32_t sees[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+        if (t >= u->n_pre) {                                     // what the row sees of the drafted tokens, requested before the scores are awaited
+          const int w0 = (t - u->n_pre) * (BN / 32), n_words = (u->nk + 31) / 32;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (nodes) sees[i] = mine && 32 * i < hi ? mask_word((key0 >> 5) + i) & bits(0, hi - 32 * i) : 0u;
-          else sees[i] = bits(max(lo, after + 1 - key0) - 32 * i, hi - 32 * i);
+          for (int i = 0; i < 4; ++i) sees[i] = mine && w0 + i < n_words ? mask_word(w0 + i) : 0u;
         }
         // S of the tile is complete, and with it every product issued before it: P V of this half's tile before too
-        ok = mbar_wait_f(s_full(x), (uint32_t)(n_s & 1), failed);
+        ok = bar_wait(s_full(x), (uint32_t)(n_s & 1), failed);
         if (!ok) break;
-        if (!any_mine) {                                  // a warp without rows: its P is never looked at
-          mbar_arrive(p_full(x, 0));
-          mbar_arrive(p_full(x, 1));
+        if (!any_mine) {                                         // a warp without rows: its P is never looked at
+          if (lane == 0) {
+            mbar_arrive(p_full(x, 0));
+            mbar_arrive(p_full(x, 1));
+          }
           continue;
         }
         tc_fence_after();
         float sc[BN];
 #pragma unroll
         for (int c = 0; c < BN; c += 32) tmem_ld32_issue(t_s + c, sc + c);
-        const uint32_t missing = k_holes[(p - begin + j) % kRing];
-        if (missing) {
-          for (int b = 0; b < BN / ta.rows_box; ++b)
-            if ((missing >> b) & 1u) {
+        const uint32_t note = *(volatile uint32_t*)&tile_notes[(p - begin + j) % kRing];
+        if (note & kAllSeen) {
+          tmem_wait_ld();
+        } else {                                                 // what the row sees of the tile's keys, as bits
+          int key0, lo, hi;
+          rows_seen(u, t, key0, lo, hi);
+          lo = max(lo, after + 1 - key0);
 #pragma unroll
-              for (int i = 0; i < 4; ++i) sees[i] &= ~bits(b * ta.rows_box - 32 * i, (b + 1) * ta.rows_box - 32 * i);
+          for (int i = 0; i < 4; ++i) {
+            sees[i] &= t >= u->n_pre ? bits(0, hi - 32 * i) : bits(lo - 32 * i, hi - 32 * i);
+            for (uint32_t left = note & 0xffffu; left; left &= left - 1) {
+              const int box = (__ffs((int)left) - 1) * ta.rows_box - 32 * i;
+              sees[i] &= ~bits(box, box + ta.rows_box);
             }
-        }
-        const bool all = (sees[0] & sees[1] & sees[2] & sees[3]) == 0xffffffffu;
-        tmem_wait_ld();
-        if (__any_sync(0xffffffffu, !all)) {
+          }
+          tmem_wait_ld();
 #pragma unroll
           for (int i = 0; i < BN; ++i)
             if (!((sees[i >> 5] >> (i & 31)) & 1u)) sc[i] = -INFINITY;
@@ -563,7 +610,6 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
             tmem_st8_issue(t_o + c, r);
             tmem_st8_issue(t_o + c + 8, r + 8);
           }
-          tmem_wait_st();
         }
         const float neg_m = m == -INFINITY ? 0.f : -m;
         const uint64_t scale2 = pk2(sl2, sl2), neg2 = pk2(neg_m, neg_m);
@@ -583,53 +629,39 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
           tmem_st32_issue(t_s + h * 32, w);
           tmem_wait_st();
           tc_fence_before();
-          mbar_arrive(p_full(x, h));
+          __syncwarp();
+          if (lane == 0) mbar_arrive(p_full(x, h));
         }
         float l0, l1;
         upk2(sum, l0, l1);
         l += l0 + l1;
       }
-      const bool have = j0 < nt;                                 // this half had a tile
-      // (the tiles' loop needs all registers: what comes now keeps nothing across it)
-      const int x_now = again(x), row_now = again(row);
-      if (ok && have) ok = mbar_wait_f(o_done(x_now), (uint32_t)(n_o & 1), failed);
+      if (ok && have) ok = bar_wait(o_done(x), (uint32_t)(n_o & 1), failed);
       if (!ok) break;
       n_o += have;
       tc_fence_after();
-      // rows of one item that lie in both halves are added up here: half x_now writes the columns [x_now HD / 2, + HD / 2)
+      // rows of one item that lie in both halves are added up here: half x writes the columns [x HD / 2, + HD / 2)
       float w_own = 1.f, w_other = 0.f;
       if (!two) {
-        stats[x_now][row_now] = make_float2(m, l);
+        stats[x][row] = make_float2(m, l);
         meet();
         if (!ok) break;
-        const float2 o = stats[x_now ^ 1][row_now];
+        const float2 o = stats[x ^ 1][row];
         const float m_all = fmaxf(m, o.x), base = m_all == -INFINITY ? 0.f : m_all;
         w_own = ex2_approx(m - base);
         w_other = ex2_approx(o.x - base);
         l = l * w_own + o.y * w_other;
         m = m_all;
       }
-      const bool other_has = !two && (x_now ^ 1) < nt;
       const bool whole = nt == u->tiles;
-      const bool odd = odd_values[i_piece % kRing] != 0;
       const float inv = l == 0.f ? 0.f : 1.f / l;
-      bf16* out = (bf16*)a.out + (u->start + node) * a.out_stride + (size_t)(u->kvh * a.group + row_now % a.group) * HD;
-      const int slot = (2 * (int)blockIdx.x + (u->t0 == 0 ? 1 : 0)) * 2 + (two ? x_now : 0);
-      float* part = a.partials + slot * partial_floats(BM, HD);
-      constexpr int kCols = HD / 2, kChunk = 8;
-      const int c_begin = two ? 0 : x_now * kCols, c_end = two ? HD : c_begin + kCols;
-#pragma unroll 1
-      for (int c0 = c_begin; c0 < c_end && any_mine; c0 += kChunk) {
-        float o[kChunk], r[kChunk];
-#pragma unroll
-        for (int c = 0; c < kChunk; c += 8) {
-          if (have) tmem_ld8_issue(t_o + c0 + c, o + c);
-          if (other_has) tmem_ld8_issue((t_o ^ 128u) + c0 + c, r + c);
-        }
-        tmem_wait_ld();
-#pragma unroll
-        for (int c = 0; c < kChunk; ++c) o[c] = (have ? o[c] * w_own : 0.f) + (other_has ? r[c] * w_other : 0.f);
-        if (odd && mine) {
+      const int slot = (2 * (int)blockIdx.x + (u->t0 == 0 ? 1 : 0)) * 2 + (two ? x : 0);
+      float* part = a.partials + slot * partial_floats(BM, HD) + row * 4;
+      bf16* out = (bf16*)a.out + (u->start + node) * a.out_stride + (size_t)(u->kvh * a.group + row % a.group) * HD;
+      // columns [c0, c0 + kN) of the row's output, summed over this block's keys
+      auto put = [&](int c0, auto& o) {
+        constexpr int kN = sizeof(o) / 4;
+        if (odd_values[i_piece % kRing] && mine) {
           // values that were set to zero, for the rows that see them (rare: nothing here is made to be fast)
 #pragma unroll 1
           for (int t = u->t0; t < u->t0 + nt; ++t) {
@@ -650,20 +682,20 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
                 src = (const bf16*)a.cache + page * a.page_stride + a.v_off + ((size_t)u->kvh * a.block_size + (k & (a.block_size - 1))) * HD;
               }
 #pragma unroll
-              for (int c = 0; c < kChunk; ++c) {
+              for (int c = 0; c < kN; ++c) {
                 const float v = __bfloat162float(src[c0 + c]);
                 if (!(fabsf(v) <= 3.4e38f)) o[c] += v;
               }
             }
           }
         }
-        if (!mine) continue;
+        if (!mine) return;
         if (whole) {
 #pragma unroll
-          for (int c = 0; c < kChunk; ++c) o[c] *= inv;
+          for (int c = 0; c < kN; ++c) o[c] *= inv;
           if (ta.wide_out) {
 #pragma unroll
-            for (int c = 0; c < kChunk; c += 8) {
+            for (int c = 0; c < kN; c += 8) {
               uint4 w;
               w.x = pack_bf16(o[c], o[c + 1]);
               w.y = pack_bf16(o[c + 2], o[c + 3]);
@@ -673,21 +705,48 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
             }
           } else {
 #pragma unroll
-            for (int c = 0; c < kChunk; ++c) out[c0 + c] = __float2bfloat16_rn(o[c]);
+            for (int c = 0; c < kN; ++c) out[c0 + c] = __float2bfloat16_rn(o[c]);
           }
         } else {
 #pragma unroll
-          for (int c = 0; c < kChunk; c += 4)
-            *reinterpret_cast<float4*>(part + ((size_t)((c0 + c) / 4) * BM + row_now) * 4) = make_float4(o[c], o[c + 1], o[c + 2], o[c + 3]);
+          for (int c = 0; c < kN; c += 4)
+            *reinterpret_cast<float4*>(part + (size_t)(c0 + c) * BM) = make_float4(o[c], o[c + 1], o[c + 2], o[c + 3]);
+        }
+      };
+      if (any_mine && two) {
+        constexpr int kN = HD % 32 == 0 ? 32 : 16;
+#pragma unroll 1
+        for (int c0 = 0; c0 < HD; c0 += kN) {
+          float o[kN];
+#pragma unroll
+          for (int c = 0; c < kN; c += 8) tmem_ld8_issue(t_o + c0 + c, o + c);
+          tmem_wait_ld();
+          put(c0, o);
+        }
+      } else if (any_mine) {
+        constexpr int kN = HD % 32 == 0 ? 16 : 8;
+        const bool other_has = (x ^ 1) < nt;
+#pragma unroll 1
+        for (int c0 = x * (HD / 2); c0 < (x + 1) * (HD / 2); c0 += kN) {
+          float o[kN], r[kN];
+#pragma unroll
+          for (int c = 0; c < kN; c += 8) {
+            tmem_ld8_issue(t_o + c0 + c, o + c);
+            tmem_ld8_issue((t_o ^ 128u) + c0 + c, r + c);
+          }
+          tmem_wait_ld();
+#pragma unroll
+          for (int c = 0; c < kN; ++c) o[c] = (have ? o[c] * w_own : 0.f) + (other_has ? r[c] * w_other : 0.f);
+          put(c0, o);
         }
       }
-      if (!whole && mine && (two || x_now == 0)) {
-        part[(size_t)HD * BM + row_now] = m;
-        part[(size_t)HD * BM + BM + row_now] = l;
-        if (row_now == 0 && u->t0 == 0) {
-          const int item = u->item + (two ? x_now : 0);
-          a.notes[2 * blockIdx.x + (two ? x_now : 0)] = make_int4(u->s, u->kvh, item * rows_item, min(ta.nodes_per_item, u->n - item * ta.nodes_per_item) * a.group
-                                                              | (block_of_tile(offs[a.n_seqs], u->p + u->tiles - 1) << 8));
+      if (!whole && mine && (two || x == 0)) {
+        part[(size_t)HD * BM - 3 * row] = m;
+        part[(size_t)HD * BM + BM - 3 * row] = l;
+        if (row == 0 && u->t0 == 0) {
+          const int item = u->item + (two ? x : 0);
+          a.notes[2 * blockIdx.x + (two ? x : 0)] = make_int4(u->s, u->kvh, item * rows_item, min(ta.nodes_per_item, u->n - item * ta.nodes_per_item) * a.group
+                                                              | (u->last << 8));
         }
       }
       // the next piece's first P V overwrites the outputs, of both halves where they were added up
@@ -771,13 +830,13 @@ LMSF_API int lmsf_attention_tree_tc(const void* q, long long q_stride, const voi
     const cuuint32_t box[4] = {64, (cuuint32_t)ta.rows_box, 1, 1};
     if (!make_map(&maps[3], cache, 4, dims, strides, box)) LMSF_REFUSE("attention_tree: no tensor map of the cache");
   }
-  const size_t smem = kOffWork + sizeof(int) * (n_seqs + 1) + 1024;
+  const size_t smem = kOffWork + work_bytes(n_seqs) + 1024;
   static bool raised[64] = {};
   int dev = 0;
   cudaError_t rc = cudaGetDevice(&dev);
   if (rc != cudaSuccess) return (int)rc;
   if (dev < 64 && !raised[dev]) {
-    rc = cudaFuncSetAttribute(attention_tree_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kOffWork + 4 * (kMaxSeqs + 1) + 1024);
+    rc = cudaFuncSetAttribute(attention_tree_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kOffWork + work_bytes(kMaxSeqs) + 1024));
     if (rc != cudaSuccess) return (int)rc;
     raised[dev] = true;
   }

@@ -26,6 +26,7 @@ BASE_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "--shared", "-Xcompiler", "-fPIC
               "--expt-relaxed-constexpr", "-Xcudafe", "--diag_suppress=177"]
 
 _loaded: Dict[Tuple[str, Tuple[str, ...]], ctypes.CDLL] = {}
+_modules: Dict[str, object] = {}
 _lock = threading.Lock()
 
 
@@ -34,6 +35,19 @@ class BuildError(RuntimeError):
 
 
 HOST_FLAGS = ["-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden"]
+# Host sources that look at torch's tensors: built against the headers of the torch that loads them.
+TORCH_SOURCES = ("tree_calls.cpp",)
+
+
+def _torch_flags() -> list:
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(os.path.abspath(torch.__file__))
+    cuda = os.environ.get("CUDA_HOME") or os.path.dirname(os.path.dirname(_nvcc()))
+    return [f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-isystem", sysconfig.get_paths()["include"],
+            "-isystem", os.path.join(root, "include"), "-isystem", os.path.join(root, "include", "torch", "csrc", "api", "include"),
+            "-isystem", os.path.join(cuda, "include"), "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
 
 
 def _gxx() -> str:
@@ -87,6 +101,9 @@ def _key(source: str, defines: Tuple[str, ...]) -> str:
             h.update(name.encode())
             h.update(f.read())
     flags = HOST_FLAGS if source.endswith(".cpp") else [*ARCH_FLAGS, *BASE_FLAGS]
+    if source in TORCH_SOURCES:              # a library per torch and Python (no paths: a copy of the tree finds its libraries elsewhere)
+        import torch
+        flags = [*flags, torch.__version__, sys.implementation.cache_tag or ""]
     h.update(" ".join([*flags, *defines]).encode())
     return h.hexdigest()[:16]
 
@@ -104,7 +121,7 @@ def compile_source(source: str, defines: Tuple[str, ...] = (), verbose: bool = T
         return out
     if source.endswith(".cpp"):      # host code: the C++ compiler alone
         cmd = [_gxx(), *HOST_FLAGS, *extra_flags, *[f"-D{d}" for d in defines], "-I", CSRC_DIR,
-               os.path.join(CSRC_DIR, source), "-o", out + f".tmp{os.getpid()}"]
+               os.path.join(CSRC_DIR, source), "-o", out + f".tmp{os.getpid()}", *(_torch_flags() if source in TORCH_SOURCES else [])]
     else:
         cmd = [_nvcc(), *ARCH_FLAGS, *BASE_FLAGS, *extra_flags, *[f"-D{d}" for d in defines], "-I", CSRC_DIR,
                os.path.join(CSRC_DIR, source), "-o", out + f".tmp{os.getpid()}", "-lcudart"]
@@ -141,6 +158,21 @@ def load_library(source: str, defines: Tuple[str, ...] = ()) -> ctypes.CDLL:
             lib = ctypes.CDLL(compile_source(source, tuple(defines)))
             _loaded[key] = lib
         return lib
+
+
+def load_module(source: str):
+    """The Python module that `source`, one of TORCH_SOURCES, defines (compiled on first use)."""
+    import importlib.machinery
+    import importlib.util
+    with _lock:
+        mod = _modules.get(source)
+        if mod is None:
+            name = "lmsf_" + os.path.splitext(source)[0]
+            loader = importlib.machinery.ExtensionFileLoader(name, compile_source(source))
+            mod = importlib.util.module_from_spec(importlib.util.spec_from_loader(name, loader))
+            loader.exec_module(mod)
+            _modules[source] = mod
+        return mod
 
 
 def all_sources() -> Iterable[str]:

@@ -8,14 +8,13 @@ are an error.
 from __future__ import annotations
 
 import ctypes
-import math
 import os
 from ctypes import c_float, c_int, c_longlong, c_void_p
 from typing import Optional, Sequence, Tuple
 
 import torch
 
-from .csrc.build import load_library
+from .csrc.build import load_library, load_module
 
 F32, BF16 = 0, 1
 
@@ -967,53 +966,37 @@ def attention_prefill_tc(out: torch.Tensor, q: torch.Tensor, cache: torch.Tensor
 # ----------------------------------------------------------------------------- trees of drafted tokens
 
 TREE_MAX_NODES = 256           # nodes of one tree (tree.cu)
-TREE_MAX_SEQS = 4096           # requests of one launch of attention_tree (attention_tree.cuh)
+TREE_MAX_SEQS = 1024           # requests of one launch of attention_tree (attention_tree.cuh)
 
 
-def _same_device(what: str, first: torch.Tensor, *others: Optional[torch.Tensor]) -> torch.device:
-    """The CUDA device that all of them are on."""
-    dev = first.device
-    if dev.type != "cuda":
-        raise KernelError("lmsf_b200 kernels run on CUDA tensors only; got a tensor on " + str(dev))
-    for t in others:
-        if t is not None and t.device != dev:
-            raise KernelError(f"{what}: tensors on {dev} and {t.device}")
-    return dev
+_TREE_CALLS = None
 
 
-def _ints(t: torch.Tensor, shape, name: str) -> int:
-    """The address of a contiguous int32 tensor of this shape."""
-    if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous():
-        raise KernelError(f"{name} must be a contiguous int32 tensor {list(shape)}, not {t.dtype} {list(t.shape)}")
-    return t.data_ptr()
+def _tree_calls():
+    """The module that checks and launches (csrc/tree_calls.cpp), and the launchers' addresses."""
+    global _TREE_CALLS
+    if _TREE_CALLS is None:
+        mod = load_module("tree_calls.cpp")
+        mod.set_error(KernelError)
+        address = lambda source, name, defines=(): ctypes.cast(getattr(load_library(source, defines), name), c_void_p).value  # noqa: E731
+        _TREE_CALLS = (mod, address)
+    return _TREE_CALLS
 
 
-def _error_word(error_flag: Optional[torch.Tensor], device: torch.device) -> int:
-    """The address of the caller's error word, or of the device's own."""
-    if error_flag is None:
-        if (device.index or 0) not in _ERROR_WORDS and torch.cuda.is_current_stream_capturing():
+def _flag_of(error_flag: Optional[torch.Tensor], t: torch.Tensor) -> Optional[torch.Tensor]:
+    """The caller's error word, or that of t's device (None: t is on no device, which the checks then say)."""
+    if error_flag is not None:
+        return error_flag
+    i = t.get_device()
+    w = _ERROR_WORDS.get(i)
+    if w is None and i >= 0:
+        if torch.cuda.is_current_stream_capturing():
             raise KernelError("the device's error word has to be made before a capture: call kernels.error_word(device) once")
-        error_flag = error_word(device)
-    return _i32(error_flag, "error_flag")
+        w = error_word(t.device)
+    return w
 
 
-class _On:
-    """Makes a device the current one for a launch, where it is not already."""
-    __slots__ = ("guard",)
-
-    def __init__(self, device: torch.device):
-        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
-
-
-_TREE_LAYOUT_ARGS = [c_void_p] * 9 + [c_int] * 6 + [c_void_p, c_void_p]
+_LAUNCHERS = {}
 
 
 def tree_layout(cu_q: torch.Tensor, token_seq: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor, mask: Optional[torch.Tensor],
@@ -1030,59 +1013,37 @@ def tree_layout(cu_q: torch.Tensor, token_seq: torch.Tensor, positions: torch.Te
     set for its ancestors and itself, of which with window > 0 the nearest `window` only; None: not made.  Rows behind the last request's are left as they
     were.  A tree has at most 32 * words and at most 256 nodes; a longer one, a parent that is not before its node, and rows beyond N are cut off
     and reported in the device's error word (or error_flag) as code 5."""
-    S = tree_len.shape[0]
-    N = token_seq.shape[0]
-    if slots.dtype != torch.int64 or slots.shape != (N,) or not slots.is_contiguous():
-        raise KernelError("tree_layout: slots must be contiguous int64 [rows]")
-    if block_table.dim() != 2 or block_table.shape[0] != S:
-        raise KernelError("tree_layout: the block table has one row per request")
-    words = 0
-    if mask is not None:
-        if mask.dim() != 2 or mask.dtype != torch.int32 or mask.shape[0] != N or not mask.is_contiguous():
-            raise KernelError("tree_layout: the mask must be contiguous int32 [rows, words]")
-        words = mask.shape[1]
-        if not 1 <= words <= TREE_MAX_NODES // 32:
-            raise KernelError(f"tree_layout: a mask has 1 to {TREE_MAX_NODES // 32} words a row, not {words}")
-    elif window:
-        raise KernelError("tree_layout: a window shows in the mask")
-    if block_size < 1 or window < 0:
-        raise KernelError(f"tree_layout: block_size={block_size}, window={window}")
-    args = (_ints(cu_q, (S + 1,), "cu_q"), _ints(token_seq, (N,), "token_seq"), _ints(positions, (N,), "positions"), slots.data_ptr(),
-            mask.data_ptr() if mask is not None else None, _ints(parents, (N,), "parents") if parents is not None else None,
-            _ints(tree_len, (S,), "tree_len"), _ints(prefix_len, (S,), "prefix_len"),
-            _ints(block_table, (S, block_table.shape[1]), "block_table"), block_table.shape[1], block_size, S, N, words, window)
-    dev = _same_device("tree_layout", cu_q, token_seq, positions, slots, mask, parents, tree_len, prefix_len, block_table, error_flag)
-    f = _func("tree.cu", "lmsf_tree_layout", _TREE_LAYOUT_ARGS)
-    with _On(dev):
-        rc = f(*args, _error_word(error_flag, dev), _stream())
+    mod, address = _TREE_CALLS or _tree_calls()
+    f = _LAUNCHERS.get("tree_layout") or _LAUNCHERS.setdefault("tree_layout", address("tree.cu", "lmsf_tree_layout"))
+    rc = mod.tree_layout(f, cu_q, token_seq, positions, slots, mask, parents, tree_len, prefix_len, block_table, block_size, window,
+                         _flag_of(error_flag, cu_q))
     _check(rc, "tree.cu", "lmsf_tree")
 
 
-_ATTENTION_TREE_ARGS = [c_void_p, c_longlong] * 4 + [c_void_p, c_longlong, c_longlong, c_int, c_void_p, c_int, c_int, c_void_p,
-                        c_void_p, c_void_p, c_int, c_void_p, c_int, c_float, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int, c_void_p]
-_ATTENTION_TREE_TC_ARGS = _ATTENTION_TREE_ARGS[:-4] + [c_void_p, c_int, c_void_p, c_void_p]
-_TREE_WORKSPACE = {}
 TREE_TC_HEAD_DIMS = (64, 80, 96, 112, 128)
 USE_TC_TREE = True             # bfloat16 trees run on the tcgen05 kernel where it takes them (csrc/attention_tree_tc.cu)
 
 
-def attention_tree_tc_supported(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: torch.Tensor, scale: float, group: int) -> bool:
-    """Whether `attention_tree` runs on the tensor cores: bfloat16, a head size of TREE_TC_HEAD_DIMS, groups up to 128, pages of a power
-    of two of at least 8 tokens, a positive scale, rows of q, k, v and the cache on 16-byte boundaries."""
-    bs = cache.shape[3]
-    return (q.dtype == torch.bfloat16 and cache.shape[4] in TREE_TC_HEAD_DIMS and group <= 128 and bs >= 8 and bs & (bs - 1) == 0
-            and cache.shape[0] > 0 and scale > 0.0 and (q.stride(0) | k.stride(0) | v.stride(0)) % 8 == 0
-            and (q.data_ptr() | k.data_ptr() | v.data_ptr() | cache.data_ptr()) % 16 == 0)
+def _attention_tree_launchers(head_dim: int, tc: bool, device: int) -> Tuple[int, int, int, int, int]:
+    """(address of the tensor-core kernel's launcher or 0, of the other's, their workspaces in bytes, SMs of the device)."""
+    key = (head_dim, tc, device)
+    got = _LAUNCHERS.get(key)
+    if got is None:
+        if not 1 <= head_dim <= 256:
+            raise KernelError(f"attention_tree: head size {head_dim} is not between 1 and 256")
+        _, address = _tree_calls()
+        sms = sm_count(torch.device("cuda", device))
 
+        def need(source, name, defines=()):
+            f = getattr(load_library(source, defines), name)
+            f.restype, f.argtypes = c_longlong, [c_int, c_int]
+            return f(sms, head_dim)
 
-def _tree_workspace(source: str, name: str, sms: int, head_dim: int, defines: Tuple[str, ...] = ()) -> int:
-    key = (name, sms, head_dim)
-    need = _TREE_WORKSPACE.get(key)
-    if need is None:
-        f = getattr(load_library(source, defines), name)
-        f.restype, f.argtypes = c_longlong, [c_int, c_int]
-        need = _TREE_WORKSPACE[key] = f(sms, head_dim)
-    return need
+        d = (f"LMSF_HEAD_DIM={head_dim}",)
+        got = _LAUNCHERS[key] = (address("attention_tree_tc.cu", "lmsf_attention_tree_tc", d) if tc else 0, address("attention_tree.cu", "lmsf_attention_tree"),
+                                 need("attention_tree_tc.cu", "lmsf_attention_tree_tc_workspace", d) if tc else 0,
+                                 need("attention_tree.cu", "lmsf_attention_tree_workspace"), sms)
+    return got
 
 
 def attention_tree(out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor,
@@ -1097,59 +1058,19 @@ def attention_tree(out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch
     positions[t] (int32 [N], no less than prefix_len) sees only cached keys behind positions[t] - window; its own
     request's rows are the mask's matter.  The lengths are read on the device alone: a captured call serves any lengths
     that fit its tensors.  Scores, softmax and sums are float32; in bfloat16 the weights are rounded to bfloat16 for their product with v."""
-    N, S = q.shape[0], prefix_len.shape[0]
-    if n_q_heads < 1 or n_kv_heads < 1 or n_q_heads % n_kv_heads:
-        raise KernelError(f"attention_tree: {n_q_heads} query heads of {n_kv_heads} kv heads")
-    if q.shape != (N, n_q_heads * head_dim) or out.shape != q.shape or k.shape != (N, n_kv_heads * head_dim) or v.shape != k.shape:
-        raise KernelError("attention_tree: q and out must be [rows, heads * head_dim], k and v [rows, kv heads * head_dim]")
-    if N and (q.stride(1) != 1 or out.stride(1) != 1 or k.stride(1) != 1 or v.stride(1) != 1):
-        raise KernelError("attention_tree: q, k, v and out need a contiguous last dimension")
-    code = dtype_code(q.dtype)
-    if not (out.dtype == k.dtype == v.dtype == cache.dtype == q.dtype):
-        raise KernelError("attention_tree: q, k, v, out and the cache must share one dtype")
-    if cache.dim() != 5 or tuple(cache.shape[1:]) != (2, n_kv_heads, block_size, head_dim) or not cache.is_contiguous():
-        raise KernelError(f"attention_tree: cache of shape {tuple(cache.shape)} does not match [pages, 2, {n_kv_heads}, {block_size}, {head_dim}]")
-    if block_table.dim() != 2 or block_table.shape[0] != S or mask.dim() != 2 or mask.shape[0] != N or mask.shape[1] < 1:
-        raise KernelError("attention_tree: the block table has one row per request, the mask at least a word for every row")
-    if window < 0 or (window and positions is None):
-        raise KernelError("attention_tree: a window is positive and needs positions")
-    if not math.isfinite(scale):
-        raise KernelError(f"attention_tree: a scale of {scale}")
-    tables = (_ints(block_table, block_table.shape, "block_table"), block_table.shape[1], block_size, _ints(cu_q, (S + 1,), "cu_q"),
-              _ints(prefix_len, (S,), "prefix_len"), _ints(mask, mask.shape, "mask"), mask.shape[1],
-              _ints(positions, (N,), "positions") if positions is not None else None)
-    dev = _same_device("attention_tree", q, out, k, v, cache, block_table, cu_q, prefix_len, mask, positions)
-    if N == 0 or S == 0:
-        return
-    sms = sm_count(dev)
-    args = (q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), out.data_ptr(), out.stride(0), cache.data_ptr(),
-            cache.stride(0), cache.stride(1), cache.shape[0], *tables, window, scale, S, N, n_q_heads, n_kv_heads, head_dim)
-    if USE_TC_TREE and attention_tree_tc_supported(q, k, v, cache, scale, n_q_heads // n_kv_heads):
-        source, d = "attention_tree_tc.cu", (f"LMSF_HEAD_DIM={head_dim}",)
-        f = _func(source, "lmsf_attention_tree_tc", _ATTENTION_TREE_TC_ARGS, d)
-        with _On(dev):
-            space = torch.empty(_tree_workspace(source, "lmsf_attention_tree_tc_workspace", sms, head_dim, d), dtype=torch.uint8, device=dev)
-            rc = f(*args, space.data_ptr(), sms, _error_word(error_flag, dev), _stream())
-        _check(rc, source, "lmsf_attention_tree_tc", d)
-    else:
-        source = "attention_tree.cu"
-        f = _func(source, "lmsf_attention_tree", _ATTENTION_TREE_ARGS)
-        with _On(dev):
-            space = torch.empty(_tree_workspace(source, "lmsf_attention_tree_workspace", sms, head_dim), dtype=torch.uint8, device=dev)
-            rc = f(*args, code, space.data_ptr(), sms, _stream())
-        _check(rc, source, "lmsf_attention_tree")
-    add_launches(1)
-
-
-_ADJUST_ARGS = [c_void_p, c_longlong, c_void_p, c_longlong, c_int, c_int, c_void_p, c_int, c_void_p, c_longlong, c_int, c_void_p, c_void_p,
-                c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p,
-                c_int, c_int, c_void_p, c_void_p]
-
-
-def _floats(t: torch.Tensor, shape, name: str) -> int:
-    if t.dtype != torch.float32 or t.shape != shape or not t.is_contiguous():
-        raise KernelError(f"{name} must be a contiguous float32 tensor {list(shape)}, not {t.dtype} {list(t.shape)}")
-    return t.data_ptr()
+    mod, _ = _TREE_CALLS or _tree_calls()
+    device = q.get_device()
+    # bfloat16 of these head sizes; the other conditions (group, pages, alignment, a positive scale) are looked at in the call
+    tc = USE_TC_TREE and head_dim in TREE_TC_HEAD_DIMS and q.dtype is torch.bfloat16
+    launchers = _LAUNCHERS.get((head_dim, tc, device)) or (_attention_tree_launchers(head_dim, tc, device) if device >= 0 else (0, 0, 0, 0, 0))
+    rc = mod.attention_tree(*launchers, out, q, k, v, cache, block_table, block_size, cu_q, prefix_len, mask, scale, n_q_heads, n_kv_heads, head_dim,
+                            positions, window, _flag_of(error_flag, q))
+    if rc == 0:
+        add_launches(2)
+    elif rc == -2:
+        _check(-1, "attention_tree.cu", "lmsf_attention_tree")
+    elif rc != -3:
+        _check(rc, "attention_tree_tc.cu" if tc else "attention_tree.cu", "lmsf_attention_tree_tc", (f"LMSF_HEAD_DIM={head_dim}",) if tc else ())
 
 
 def adjust_logits(out: torch.Tensor, logits: torch.Tensor, row_req: Optional[torch.Tensor] = None, history=None, penalties=None, tree=None,
@@ -1169,57 +1090,13 @@ def adjust_logits(out: torch.Tensor, logits: torch.Tensor, row_req: Optional[tor
       -inf, whatever the logit was; which[r] < 0: everything is allowed.
 
     A request or a mask beyond the tensors is reported in the device's error word (or error_flag) as code 5; its row passes without them."""
-    rows, vocab = logits.shape
-    if logits.dtype != torch.float32 or out.dtype != torch.float32 or out.shape != logits.shape:
-        raise KernelError("adjust_logits: logits and out must be float32 [rows, vocab]")
-    if rows and vocab and (logits.stride(1) != 1 or out.stride(1) != 1 or (rows > 1 and (logits.stride(0) < vocab or out.stride(0) < vocab))):
-        raise KernelError("adjust_logits: logits and out need a contiguous last dimension and rows apart")
-    if out.data_ptr() == logits.data_ptr() and rows > 1 and out.stride(0) != logits.stride(0):
-        raise KernelError("adjust_logits: out is logits itself or lies apart from it")
-    if (history is not None or tree is not None) and penalties is None:
-        raise KernelError("adjust_logits: occurrences are counted for penalties")
-    R = penalties[0].shape[0] if penalties is not None else bias[0].shape[0] - 1 if bias is not None else 0
-    args = [None] * 3
-    h = [None, 0, 0, None, None]
-    t = [None, None, None, 0]
-    if penalties is not None:
-        args = [_floats(x, (R,), f"adjust_logits: {name}") for x, name in zip(penalties, ("presence", "frequency", "repetition"))]
-        if history is not None:
-            tokens, length, prompt = history
-            if tokens.dtype != torch.int32 or tokens.dim() != 2 or tokens.shape[0] != R or (tokens.shape[1] and tokens.stride(1) != 1):
-                raise KernelError("adjust_logits: the history must be int32 [requests, width] with a contiguous last dimension")
-            h = [tokens.data_ptr(), tokens.stride(0), tokens.shape[1], _ints(length, (R,), "history length"), _ints(prompt, (R,), "prompt length")]
-        if tree is not None:
-            tokens, mask, cu_q = tree
-            if mask.dim() != 2:
-                raise KernelError("adjust_logits: the tree's mask must be int32 [rows, words]")
-            t = [_ints(tokens, (rows,), "tree tokens"), _ints(mask, (rows, mask.shape[1]), "tree mask"), _ints(cu_q, (R + 1,), "cu_q"), mask.shape[1]]
-    b = [None, None, None, 0]
-    if bias is not None:
-        start, token, value = bias
-        n = token.shape[0]
-        b = [_ints(start, (R + 1,), "bias start"), _ints(token, (n,), "bias token"), _floats(value, (n,), "bias value"), n]
-    m = [None, None, 0, 0]
-    if allowed is not None:
-        bits, which = allowed
-        words = (vocab + 31) // 32
-        if bits.dim() != 2:
-            raise KernelError("adjust_logits: the masks must be int32 [masks, words]")
-        m = [_ints(bits, (bits.shape[0], words), "masks"), _ints(which, (rows,), "mask of a row"), bits.shape[0], words]
-    if row_req is None and R and R != rows:
-        raise KernelError(f"adjust_logits: options of {R} requests for {rows} rows need row_req")
-    req = _ints(row_req, (rows,), "row_req") if row_req is not None else None
-    dev = _same_device("adjust_logits", logits, out, row_req, error_flag, *(history or ()), *(penalties or ()), *(tree or ()), *(bias or ()), *(allowed or ()))
-    if rows == 0 or vocab == 0:
-        return
-    f = _func("adjust_logits.cu", "lmsf_adjust_logits", _ADJUST_ARGS)
-    with _On(dev):
-        rc = f(out.data_ptr(), max(out.stride(0), vocab), logits.data_ptr(), max(logits.stride(0), vocab), rows, vocab, req, R, *h, *args, *t, *b, *m,
-               _error_word(error_flag, dev), _stream())
-    _check(rc, "adjust_logits.cu", "lmsf_adjust_logits")
-
-
-_TREE_ACCEPT_ARGS = [c_void_p] * 9 + [c_int] * 3 + [c_void_p] * 3 + [c_longlong] * 4 + [c_void_p] + [c_int] * 5 + [c_void_p, c_void_p]
+    mod, address = _TREE_CALLS or _tree_calls()
+    f = _LAUNCHERS.get("adjust_logits") or _LAUNCHERS.setdefault("adjust_logits", address("adjust_logits.cu", "lmsf_adjust_logits"))
+    none3 = (None, None, None)
+    rc = mod.adjust_logits(f, out, logits, row_req, *(history or none3), *(penalties or none3), *(tree or none3), *(bias or none3),
+                           *(allowed or (None, None)), _flag_of(error_flag, logits))
+    if rc != -3:
+        _check(rc, "adjust_logits.cu", "lmsf_adjust_logits")
 
 
 def tree_accept(n_kept: torch.Tensor, path: torch.Tensor, next_token: torch.Tensor, new_len: torch.Tensor, target: torch.Tensor,
@@ -1237,36 +1114,9 @@ def tree_accept(n_kept: torch.Tensor, path: torch.Tensor, next_token: torch.Tens
     values of every layer) and cache [calls, pages, 2, kv heads, block_size, head_dim] the kept rows' keys and values are written to
     the cache, the i-th to slot slots[cu_q[s] + i], in the same launch.  A slot outside the cache is not written and is reported
     in the device's error word (or error_flag) as code 2; trees of more than 256 rows as code 5 (their first 256 count)."""
-    S, N = prefix_len.shape[0], target.shape[0]
-    if path.dim() != 2 or not 1 <= path.shape[1] <= TREE_MAX_NODES:
-        raise KernelError(f"tree_accept: the path must be int32 [requests, 1 to {TREE_MAX_NODES}]")
-    copy = [None, None, None, 0, 0, 0, 0, None, 0, 0, 0, 0, 0]
-    given = [t is not None for t in (slots, k, v, cache)]
-    if any(given):
-        if not all(given):
-            raise KernelError("tree_accept: slots, k, v and the cache belong together")
-        if cache.dim() != 6 or cache.shape[2] != 2 or not cache.is_contiguous():
-            raise KernelError("tree_accept: the cache must be contiguous [calls, pages, 2, kv heads, block_size, head_dim]")
-        calls, pages, _, kvh, block_size, hd = cache.shape
-        size = cache.element_size()
-        dtype_code(cache.dtype)
-        if slots.dtype != torch.int64 or slots.shape != (N,) or not slots.is_contiguous():
-            raise KernelError("tree_accept: slots must be contiguous int64 [rows]")
-        for t in (k, v):
-            if t.dtype != cache.dtype or t.shape != (calls, N, kvh * hd) or (N and t.stride(2) != 1):
-                raise KernelError(f"tree_accept: k and v must be [{calls}, rows, {kvh * hd}] of the cache's dtype with a contiguous last dimension")
-        if cache.numel() and N:
-            copy = [slots.data_ptr(), k.data_ptr(), v.data_ptr(), k.stride(0) * size, k.stride(1) * size, v.stride(0) * size, v.stride(1) * size,
-                    cache.data_ptr(), calls, pages, kvh, block_size, hd * size]
-    if path.shape[0] != S:
-        raise KernelError("tree_accept: the path has one row per request")
-    args = (_ints(n_kept, (S,), "n_kept"), _ints(path, path.shape, "path"), _ints(next_token, (S,), "next_token"), _ints(new_len, (S,), "new_len"),
-            _ints(target, (N,), "target"), _ints(tokens, (N,), "tokens"), _ints(parents, (N,), "parents"), _ints(cu_q, (S + 1,), "cu_q"),
-            _ints(prefix_len, (S,), "prefix_len"), S, N, path.shape[1])
-    dev = _same_device("tree_accept", n_kept, path, next_token, new_len, target, tokens, parents, cu_q, prefix_len, slots, k, v, cache, error_flag)
-    f = _func("tree.cu", "lmsf_tree_accept", _TREE_ACCEPT_ARGS)
-    with _On(dev):
-        rc = f(*args, *copy, _error_word(error_flag, dev), _stream())
+    mod, address = _TREE_CALLS or _tree_calls()
+    f = _LAUNCHERS.get("tree_accept") or _LAUNCHERS.setdefault("tree_accept", address("tree.cu", "lmsf_tree_accept"))
+    rc = mod.tree_accept(f, n_kept, path, next_token, new_len, target, tokens, parents, cu_q, prefix_len, slots, k, v, cache, _flag_of(error_flag, target))
     _check(rc, "tree.cu", "lmsf_tree")
 
 
