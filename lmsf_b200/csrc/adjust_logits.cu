@@ -11,7 +11,8 @@ namespace lmsf {
 
 constexpr int kErrOptions = 5;             // value of the error word
 constexpr int kChunk = 4096;               // values of a row that a block takes
-constexpr int kThreads = 256;
+constexpr int kThreads = 256, kPer = kChunk / kThreads;
+constexpr int kMaxNodes = 256;             // nodes of a drafted tree
 constexpr unsigned kInPrompt = 0x80000000u;
 
 struct AdjustArgs {
@@ -28,94 +29,226 @@ struct AdjustArgs {
   int* error_flag;
 };
 
-__global__ void __launch_bounds__(kThreads) adjust_logits_kernel(AdjustArgs a) {
-  __shared__ unsigned seen[kChunk];        // how often a token occurs in the output; the top bit: it occurs in the prompt
-  __shared__ float bias[kChunk];
+// A block takes kChunk values of up to `rows_block` rows in turn.  What occurs how often in them, and the biases, lie in shared memory, one word
+// per value each; they are made when a row's request is another than the row's before, so the nodes of a tree share one pass over their
+// request's history.  Every value belongs to one thread in all rows: what a node's path adds to the counts its thread adds before the row and
+// takes off behind it, without a barrier.  A row's values are requested before anything else is done for it, and not at all where a
+// grammar hides four neighbours.  Bound by memory: 8 bytes a value, 4 of them less where they are hidden.
+template <bool kWide>
+__global__ void __launch_bounds__(kThreads, 4) adjust_logits_kernel(AdjustArgs a, int rows_block) {
+  __shared__ __align__(16) unsigned seen[kChunk];        // how often a token occurs in the output; the top bit: it occurs in the prompt
+  __shared__ __align__(16) float bias[kChunk];
+  __shared__ unsigned path[kMaxNodes];     // the tree's nodes whose token is one of the chunk's: node << 16 | value
+  __shared__ int n_path;
+  __shared__ unsigned entry_at[256];       // entries of the list of biases
+  __shared__ float entry_value[256];
   pdl_launch_dependents();
   pdl_wait();
-  const int r = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
+  const int tid = threadIdx.x, lane = tid & 31;
   const int v0 = blockIdx.x * kChunk, width = min(kChunk, a.vocab - v0);
-  int req = a.row_req ? a.row_req[r] : r;
-  const bool known = req >= 0 && req < a.n_reqs;
-  if (!known && a.n_reqs > 0 && tid == 0 && blockIdx.x == 0 && a.error_flag) atomicExch(a.error_flag, kErrOptions);
-  const bool penalties = known && a.repetition, biases = known && a.bias_start;
-  if (penalties) for (int i = tid; i < kChunk; i += kThreads) seen[i] = 0u;
-  if (biases) for (int i = tid; i < kChunk; i += kThreads) bias[i] = 0.f;
-  __syncthreads();
-  auto note = [&](int token, bool prompt) {
-    const unsigned i = (unsigned)(token - v0);
-    if (i < (unsigned)width) {
-      if (prompt) atomicOr(&seen[i], kInPrompt);
-      else atomicAdd(&seen[i], 1u);
+  const int row0 = blockIdx.y * rows_block, row1 = min(row0 + rows_block, a.n_rows);
+  // this thread's k-th value; wide: four neighbours at a time
+  auto place = [&](int k) { return kWide ? 4 * (tid + kThreads * (k >> 2)) + (k & 3) : tid + kThreads * k; };
+  auto owner = [&](int i) { return kWide ? (i >> 2) % kThreads : i % kThreads; };
+  int current = -1;                        // the request that seen, bias and path are of
+  bool penalties = false, biases = false;
+  unsigned long long own = 0ull;           // this thread's entries of path
+  // Which of this thread's values mask `which` allows.
+  auto allowed = [&](int which) {
+    if (which < 0 || which >= a.n_allowed) return 0xffffu;
+    const unsigned* words = a.allowed + (size_t)which * a.allowed_words;
+    unsigned ok = 0u;
+#pragma unroll
+    for (int k = 0; k < kPer; k += kWide ? 4 : 1) {
+      const int i = place(k);
+      if (i < width) ok |= ((words[(v0 + i) >> 5] >> ((v0 + i) & 31)) & (kWide ? 15u : 1u)) << k;
     }
+    return ok;
   };
-  if (penalties) {
-    if (a.history) {
-      const int* h = a.history + req * a.history_stride;
-      const int n = min(max(a.history_len[req], 0), a.history_width), p = a.prompt_len[req];
-      for (int i = tid; i < n; i += kThreads) note(h[i], i < p);
+  auto request_of = [&](int r) { return a.row_req ? a.row_req[r] : r; };
+  auto mask_of = [&](int r) { return a.allowed ? a.allowed_row[r] : -1; };
+  int req = request_of(row0), which = mask_of(row0);
+  unsigned ok = allowed(which);
+  for (int r = row0; r < row1; ++r) {
+    const bool known = req >= 0 && req < a.n_reqs, fresh = known && req != current;
+    if (((!known && a.n_reqs > 0) || (a.allowed && which >= a.n_allowed)) && tid == 0 && blockIdx.x == 0 && a.error_flag) atomicExch(a.error_flag, kErrOptions);
+    penalties = known && a.repetition;
+    biases = known && a.bias_start;
+    int n_history = 0, n_prompt = 0, first = 0, nodes = 0, b0 = 0, b1 = 0;
+    if (fresh) {
+      if (a.history) {
+        n_history = min(max(a.history_len[req], 0), a.history_width);
+        n_prompt = a.prompt_len[req];
+      }
+      if (a.tree_tokens) {
+        first = min(max(a.cu_q[req], 0), a.n_rows);
+        nodes = min(min(a.cu_q[req + 1], a.n_rows) - first, 32 * a.words);
+      }
+      if (biases) {
+        b0 = min(max(a.bias_start[req], 0), a.n_bias);
+        b1 = min(a.bias_start[req + 1], a.n_bias);
+      }
     }
-    if (a.tree_tokens) {
-      const int first = min(max(a.cu_q[req], 0), a.n_rows), nodes = min(a.cu_q[req + 1], a.n_rows) - first;
-      for (int i = tid; i < min(nodes, 32 * a.words); i += kThreads)
-        if ((a.tree_mask[(size_t)r * a.words + (i >> 5)] >> (i & 31)) & 1u) note(a.tree_tokens[first + i], false);
+    if (fresh) {
+      if (current >= 0) __syncthreads();                         // the rows before are done with what is there
+      current = req;
+      const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (penalties) for (int i = tid; i < kChunk / 4; i += kThreads) reinterpret_cast<float4*>(seen)[i] = zero;
+      if (biases) for (int i = tid; i < kChunk / 4; i += kThreads) reinterpret_cast<float4*>(bias)[i] = zero;
+      if (tid == 0) n_path = 0;
+      __syncthreads();
     }
-  }
-  if (biases && tid < 32) {
-    // In the order of the list, so that a token that is listed twice gets the same sum in every run: one warp, 32 entries
-    // at a time, the first lane of those that name one token adds theirs up.
-    const int b0 = min(max(a.bias_start[req], 0), a.n_bias), b1 = min(a.bias_start[req + 1], a.n_bias);
-    for (int base = b0; base < b1; base += 32) {
-      const int e = base + lane;
-      const unsigned i = e < b1 ? (unsigned)(a.bias_token[e] - v0) : 0xffffffffu;
-      const float value = e < b1 ? a.bias_value[e] : 0.f;
-      const bool mine = i < (unsigned)width;
-      const unsigned same = __match_any_sync(0xffffffffu, mine ? i : 0xffffffffu);
-      if (mine && (same & ((1u << lane) - 1u)) == 0u) bias[i] += value;
-      unsigned later = mine && (same & ((1u << lane) - 1u)) == 0u ? same & ~(1u << lane) : 0u;
-      if (__any_sync(0xffffffffu, later != 0u)) {
-        for (int k = 1; k < 32; ++k) {
-          const float other = __shfl_sync(0xffffffffu, value, k);
-          if ((later >> k) & 1u) bias[i] += other;
+    const float* x_row = a.logits + r * a.stride + v0;
+    float* out_row = a.out + r * a.out_stride + v0;
+    float x[kPer];
+#pragma unroll
+    for (int k = 0; k < kPer; k += kWide ? 4 : 1) {
+      const int i = place(k);
+      if constexpr (kWide) {
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+        if ((ok >> k) & 15u) {
+          if (i + 4 <= width) {
+            y = *reinterpret_cast<const float4*>(x_row + i);
+          } else {
+            if (i < width) y.x = x_row[i];
+            if (i + 1 < width) y.y = x_row[i + 1];
+            if (i + 2 < width) y.z = x_row[i + 2];
+          }
+        }
+        x[k] = y.x; x[k + 1] = y.y; x[k + 2] = y.z; x[k + 3] = y.w;
+      } else {
+        x[k] = i < width && ((ok >> k) & 1u) ? x_row[i] : 0.f;
+      }
+    }
+    // the next row's request and mask, while these values are on their way
+    int next_req = -1, next_which = -1;
+    if (r + 1 < row1) {
+      next_req = request_of(r + 1);
+      next_which = mask_of(r + 1);
+    }
+    if (fresh) {
+      if (penalties) {
+        auto note = [&](int token, bool prompt) {
+          const unsigned i = (unsigned)(token - v0);
+          if (i < (unsigned)width) {
+            if (prompt) atomicOr(&seen[i], kInPrompt);
+            else atomicAdd(&seen[i], 1u);
+          }
+        };
+        const int* h = a.history + req * a.history_stride;
+        for (int i0 = tid; i0 < n_history; i0 += 8 * kThreads) {
+          int t[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) t[k] = i0 + k * kThreads < n_history ? h[i0 + k * kThreads] : -1;
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            if (i0 + k * kThreads < n_history) note(t[k], i0 + k * kThreads < n_prompt);
+        }
+        for (int j = tid; j < nodes; j += kThreads) {
+          const unsigned i = (unsigned)(a.tree_tokens[first + j] - v0);
+          if (i < (unsigned)width) path[atomicAdd(&n_path, 1)] = ((unsigned)j << 16) | i;
         }
       }
-      __syncwarp();
+      if (biases && tid >= kThreads - 32) {
+        // In the order of the list, so that a token that is listed twice gets the same sum in every run: one warp, 32 entries
+        // at a time (eight times as many requested at once), the first lane of those that name one token adds theirs up.
+        for (int base = b0; base < b1; base += 256) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int e = base + 32 * k + lane;
+            entry_at[32 * k + lane] = e < b1 ? (unsigned)(a.bias_token[e] - v0) : 0xffffffffu;
+            entry_value[32 * k + lane] = e < b1 ? a.bias_value[e] : 0.f;
+          }
+          __syncwarp();
+#pragma unroll 1
+          for (int k = 0; k < 8; ++k) {
+            const unsigned at = entry_at[32 * k + lane];
+            const bool mine = at < (unsigned)width;
+            if (!__any_sync(0xffffffffu, mine)) continue;
+            const unsigned same = __match_any_sync(0xffffffffu, mine ? at : 0xffffffffu);
+            if (mine && (same & ((1u << lane) - 1u)) == 0u) {
+              float sum = bias[at];
+              for (unsigned left = same; left; left &= left - 1) sum += entry_value[32 * k + __ffs((int)left) - 1];
+              bias[at] = sum;
+            }
+            __syncwarp();
+          }
+        }
+      }
+      __syncthreads();
     }
-  }
-  __syncthreads();
-  float rep = 1.f, freq = 0.f, pres = 0.f;
-  if (penalties) {
-    rep = a.repetition[req];
-    freq = a.frequency[req];
-    pres = a.presence[req];
-  }
-  const unsigned* allow = nullptr;
-  if (a.allowed) {
-    const int m = a.allowed_row ? a.allowed_row[r] : r;
-    if (m >= a.n_allowed) {
-      if (tid == 0 && blockIdx.x == 0 && a.error_flag) atomicExch(a.error_flag, kErrOptions);
-    } else if (m >= 0) {
-      allow = a.allowed + (size_t)m * a.allowed_words;
+    const unsigned next_ok = r + 1 < row1 ? allowed(next_which) : 0u;
+    const int on_path = penalties && a.tree_tokens ? n_path : 0;
+    if (fresh) {                           // the first 64 of them that are this thread's
+      own = 0ull;
+      for (int e = 0; e < min(on_path, 64); ++e)
+        if (owner((int)(path[e] & 0xffffu)) == tid) own |= 1ull << e;
     }
-  }
-  const float* x_row = a.logits + r * a.stride + v0;
-  float* out_row = a.out + r * a.out_stride + v0;
-  auto one = [&](int i, float x, bool ok) {
+    // by: 1 before the row, -1 (as an unsigned number) behind it
+    auto step = [&](int e, unsigned by) {
+      const unsigned at = path[e] & 0xffffu, node = path[e] >> 16;
+      if ((a.tree_mask[(size_t)r * a.words + (node >> 5)] >> (node & 31)) & 1u) seen[at] += by;
+    };
+    auto walk = [&](unsigned by) {
+      if (on_path == 0) return;
+      for (unsigned long long left = own; left; left &= left - 1) step(__ffsll((long long)left) - 1, by);
+      for (int e = 64; e < on_path; ++e)
+        if (owner((int)(path[e] & 0xffffu)) == tid) step(e, by);
+    };
+    walk(1u);
+    float rep = 1.f, freq = 0.f, pres = 0.f;
     if (penalties) {
-      const unsigned c = seen[i];
+      rep = a.repetition[req];
+      freq = a.frequency[req];
+      pres = a.presence[req];
+    }
+    auto adjust = [&](float y, unsigned c) {
       if (c) {
-        x = x > 0.f ? x / rep : x * rep;
+        y = y > 0.f ? y / rep : y * rep;
         const unsigned said = c & ~kInPrompt;
-        x -= freq * (float)said;
-        if (said) x -= pres;
+        y -= freq * (float)said;
+        if (said) y -= pres;
+      }
+      return y;
+    };
+#pragma unroll
+    for (int k = 0; k < kPer; k += kWide ? 4 : 1) {
+      const int i = place(k);
+      if (i >= width) continue;
+      if constexpr (kWide) {               // (seen and bias are whole, also behind the vocabulary's end)
+        if (penalties) {
+          const uint4 c = *reinterpret_cast<const uint4*>(seen + i);
+          if (c.x | c.y | c.z | c.w) {
+            x[k] = adjust(x[k], c.x);
+            x[k + 1] = adjust(x[k + 1], c.y);
+            x[k + 2] = adjust(x[k + 2], c.z);
+            x[k + 3] = adjust(x[k + 3], c.w);
+          }
+        }
+        if (biases) {
+          const float4 b = *reinterpret_cast<const float4*>(bias + i);
+          x[k] += b.x; x[k + 1] += b.y; x[k + 2] += b.z; x[k + 3] += b.w;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (!((ok >> (k + e)) & 1u)) x[k + e] = -INFINITY;
+        if (i + 4 <= width) {
+          *reinterpret_cast<float4*>(out_row + i) = make_float4(x[k], x[k + 1], x[k + 2], x[k + 3]);
+        } else {
+          out_row[i] = x[k];
+          if (i + 1 < width) out_row[i + 1] = x[k + 1];
+          if (i + 2 < width) out_row[i + 2] = x[k + 2];
+        }
+      } else {
+        if (penalties) x[k] = adjust(x[k], seen[i]);
+        if (biases) x[k] += bias[i];
+        out_row[i] = (ok >> k) & 1u ? x[k] : -INFINITY;
       }
     }
-    if (biases) x += bias[i];
-    return ok ? x : -INFINITY;
-  };
-  for (int i = tid; i < width; i += kThreads) {
-    const bool ok = !allow || ((allow[(v0 + i) >> 5] >> ((v0 + i) & 31)) & 1u);
-    out_row[i] = one(i, x_row[i], ok);
+    walk(0xffffffffu);
+    req = next_req;
+    which = next_which;
+    ok = next_ok;
   }
 }
 
@@ -132,9 +265,19 @@ LMSF_API int lmsf_adjust_logits(float* out, long long out_stride, const float* l
   using namespace lmsf;
   if (n_rows <= 0) return 0;
   if (vocab <= 0 || stride < vocab || out_stride < vocab) LMSF_REFUSE("adjust_logits: vocab=%d, strides %lld and %lld", vocab, stride, out_stride);
-  if (n_rows > 65535) LMSF_REFUSE("adjust_logits: %d rows are more than one launch takes (65535)", n_rows);
+  if (tree_tokens && (words < 1 || words > kMaxNodes / 32)) LMSF_REFUSE("adjust_logits: a tree's mask has 1 to %d words a row, not %d", kMaxNodes / 32, words);
   AdjustArgs a{out, out_stride, logits, stride, n_rows, vocab, row_req, n_reqs, history, history_stride, history_width, history_len,
                prompt_len, presence, frequency, repetition, tree_tokens, tree_mask, cu_q, words, bias_start, bias_token, bias_value, n_bias,
                allowed, allowed_row, n_allowed, allowed_words, error_flag};
-  return launch_pdl(adjust_logits_kernel, dim3(ceil_div(vocab, kChunk), n_rows), dim3(kThreads), 0, (cudaStream_t)stream, a);
+  // Rows of a block: one, where rows are few; more, where that leaves 16 blocks and more for each of 148 SMs, so that the rows of a request
+  // share its counts.
+  const int chunks = ceil_div(vocab, kChunk);
+  const long long blocks = (long long)chunks * n_rows;
+  int rows_block = 1;
+  while (rows_block < 32 && blocks / (2 * rows_block) >= 148 * 16) rows_block *= 2;
+  while (ceil_div(n_rows, rows_block) > 65535) rows_block *= 2;
+  const bool wide = ((unsigned long long)out | (unsigned long long)logits) % 16 == 0 && (n_rows == 1 || (out_stride | stride) % 4 == 0);
+  const dim3 grid(chunks, ceil_div(n_rows, rows_block));
+  if (wide) return launch_pdl(adjust_logits_kernel<true>, grid, dim3(kThreads), 0, (cudaStream_t)stream, a, rows_block);
+  return launch_pdl(adjust_logits_kernel<false>, grid, dim3(kThreads), 0, (cudaStream_t)stream, a, rows_block);
 }

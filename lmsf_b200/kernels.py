@@ -1082,7 +1082,7 @@ def adjust_logits(out: torch.Tensor, logits: torch.Tensor, row_req: Optional[tor
       A token that occurs in the prompt or the output: x / repetition if x > 0, else x * repetition; one that occurs c times in the
       output: x - frequency * c - presence.  Occurrences are counted here:
       history = (tokens int32 [R, width], length int32 [R], prompt length int32 [R]): the first `length` tokens of a row, of which the first `prompt length` are the
-      prompt, the others output; tree = (tokens int32 [rows], mask int32 [rows, words], cu_q int32 [R + 1]): rows are nodes of drafted trees,
+      prompt, the others output; tree = (tokens int32 [rows], mask int32 [rows, words <= 8], cu_q int32 [R + 1]): rows are nodes of drafted trees,
       and the nodes whose bits are set in a row's mask (bit j: row cu_q[q] + j) count as output of that row.  Ids outside the vocabulary are passed over.
     bias = (start int32 [R + 1], token int32 [B], value float32 [B]): the entries start[q] .. start[q + 1] - 1 are added to their tokens, in
       their order where a token is listed twice.
