@@ -5,9 +5,8 @@
 // one kv head of one request are its nodes x the heads of the group, node-major: row = node * group + head of the group.
 //
 // The work is cut as follows.  A unit is (request, kv head, item of up to kRows rows); it has the request's tiles of kKeys keys: its
-// cached keys first, then the nodes.  All units' tiles in a row, requests in order, are shared out evenly: of G blocks block b
-// takes the tiles [b W / G, (b + 1) W / G) of all W (G no more than W), whatever the lengths are; no plan is made on the host, so a captured launch
-// serves any lengths.  A unit that lies in one block's range is finished there.  Of a unit that is cut every block leaves a
+// cached keys first, then the nodes.  All units' tiles in a row, requests in order, are shared out evenly over the blocks, whatever the
+// lengths are; no plan is made on the host, so a captured launch serves any lengths.  A unit that lies in one block's range is finished there.  Of a unit that is cut every block leaves a
 // partial (unnormalised output, running maximum, sum; float32) in the workspace: at most two for a block (and item), one for the unit
 // that it begins with and one for the unit that it ends with.  A second kernel adds them up in the order of the blocks; both
 // depend only on lengths and G, so the result is the same in every run.
@@ -98,14 +97,22 @@ __device__ __forceinline__ void add_up_work(const Args& a, int rows, int items_p
   __syncthreads();
 }
 
-// The tiles that this block takes of `work`.  Of fewer tiles than blocks, the first blocks take one each: no block with an empty
-// share stands between the pieces of a unit.
+// Blocks that take part in `work` tiles: two tiles each at the least (a short unit that is cut costs more than its second tile), and none
+// with an empty share between the pieces of a unit.
+__device__ __forceinline__ int blocks_for(int work) { return min((int)gridDim.x, (work + 1) / 2); }
+// The tiles that this block takes of them: every block as many as every other, the first `work % blocks` one more.
 __device__ __forceinline__ void share_of_block(int work, int& begin, int& end) {
-  const int b = blockIdx.x, blocks = min((int)gridDim.x, work);
+  const int b = blockIdx.x, blocks = blocks_for(work);
   begin = end = 0;
   if (b >= blocks) return;
-  begin = (int)((long long)work * b / blocks);
-  end = (int)((long long)work * (b + 1) / blocks);
+  const int each = work / blocks, more = work - each * blocks;
+  begin = b * each + min(b, more);
+  end = begin + each + (b < more ? 1 : 0);
+}
+// The block that has tile p of all `work` tiles.
+__device__ __forceinline__ int block_of_tile(int work, int p) {
+  const int blocks = blocks_for(work), each = work / blocks, more = work - each * blocks, edge = more * (each + 1);
+  return p < edge ? p / (each + 1) : more + (p - edge) / each;
 }
 
 // The request whose tiles hold place p (0 <= p < offs[n_seqs]).
@@ -140,14 +147,6 @@ __device__ __forceinline__ Piece piece_at(const Args& a, const Lengths* all, con
 // Its note, of which = 1 alone: x = request, or -1: none; y = kv head; z = first row among the request's rows of that kv head;
 // w = rows | the last block that has a part of the unit << 8.
 __host__ __device__ __forceinline__ size_t partial_floats(int rows, int hd) { return (size_t)rows * ((hd + 3) / 4 * 4 + 2); }
-
-// The block that has tile p of all `work` tiles (share_of_block's rule).
-__device__ __forceinline__ int block_of_tile(int work, int p) {
-  const int blocks = min((int)gridDim.x, work);
-  int b = (int)((long long)p * blocks / work);
-  while ((long long)work * (b + 1) / blocks <= p) ++b;
-  return b;
-}
 
 // Adds the partials of the units that were cut: block (b, y) of the grid acts if a unit begins in b's last piece and goes on; y is
 // an item and 32 of its rows.  Lane = row, and a warp has every eighth group of four columns, so that partials are read in whole

@@ -10,7 +10,7 @@
 //   * a unit of one item: the two halves of the block take the tiles in turn with the same queries, each with an output and a maximum of
 //     its own, and add up at the end, so that one half's products run beside the other's softmax here too.
 // Warps: 0-3 and 4-7 softmax of half 0 and 1, a row per thread; 8 works out the pieces and brings queries and tiles of k by tensor-map copies (a
-// box per page, or 32 rows of the step's own k for drafted tokens); 9 brings tiles of v and goes over those that some row must not see
+// box per page, or 32 rows of the step's own k for drafted tokens); 9 brings tiles of v; 11 goes over those that some row must not see
 // all of: rows that nobody sees are cleared, and in a tile whose rows not every row sees (drafted tokens, the edge of a window)
 // values that are no numbers are set to zero and remembered, since their zero weights would make NaN of them; the rows that do
 // see them get them added at the end; 10 issues the products, the halves in turn, so that one half's products run beside the other's softmax
@@ -50,7 +50,6 @@ constexpr int kThreadsTotal = 384, kHalf = 128;
 constexpr int kRegsSoftmax = 216, kRegsOther = 72;
 constexpr int kRing = 16;                      // notes of tiles and of pieces that warps leave one another
 static_assert(kStages + 4 <= kRing, "notes are read before they are written again");
-static_assert(kStages <= 4, "warp 9 may be this far ahead of the notes");
 
 struct TcArgs {
   Args a;
@@ -97,24 +96,11 @@ __device__ __forceinline__ void tmem_st8_issue(uint32_t taddr, const float* r) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n"
                ::"r"(taddr), "f"(r[0]), "f"(r[1]), "f"(r[2]), "f"(r[3]), "f"(r[4]), "f"(r[5]), "f"(r[6]), "f"(r[7]) : "memory");
 }
-// Waits let the warp sleep until the barrier's phase is over (10 us at a time, a second or so in all).  Without the hint a wait comes back and
-// looks again after a moment, and the looks of the warps that wait take the softmax warps beside them a third of their issue slots.
-constexpr uint32_t kSleepNs = 10000;
-constexpr int kSleeps = 1 << 17;
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* failed) {
-  uint32_t done = 0;
-  for (int it = 0; it < kSleeps && !done; ++it) {
-    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\nselp.b32 %0, 1, 0, p;\n}\n"
-                 : "=r"(done) : "r"(bar), "r"(parity), "r"(kSleepNs) : "memory");
-    if (!done && *failed) return false;
-  }
-  if (!done) *failed = 1;
-  return done != 0;
-}
-// the same without the early way out: a block's own copies land before it ends
-__device__ __forceinline__ void bar_drain(uint32_t bar, uint32_t parity) {
-  int never = 0;
-  bar_wait(bar, parity, &never);
+// Waits and arrivals are the kernel's pace: a wait that finds its barrier ready takes a warp 78 cycles (110 with a hint for how long to sleep, 250
+// where one lane waits for the others), a signal from warp to warp 130.  So all lanes wait, and the one lane that arrives does so under a
+// predicate, without a branch.
+__device__ __forceinline__ void arrive_if(bool go, uint32_t bar) {
+  asm volatile("{\n.reg .pred q;\n.reg .b64 st;\nsetp.ne.b32 q, %1, 0;\n@q mbarrier.arrive.shared::cta.b64 st, [%0];\n}\n" ::"r"(bar), "r"((uint32_t)go) : "memory");
 }
 __device__ __forceinline__ void tma_load_box_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t mbar) {
   asm volatile(
@@ -141,7 +127,7 @@ __device__ __forceinline__ void rows_seen(NotePtr u, int t, int& key0, int& lo, 
   lo = nodes ? 0 : max(u->lo - key0, 0);
   hi = min((nodes ? u->nk : u->prefix) - key0, BN);
 }
-// What the warps need to know of a tile: boxes of k that are not there, which steps of 16 keys somebody sees (from, to), and whether every
+// What the warps need to know of a tile: boxes whose page is not there, which steps of 16 keys somebody sees (from, to), and whether every
 // row sees every key.
 constexpr uint32_t kAllSeen = 0x80000000u;
 __device__ __forceinline__ int from16(uint32_t note) { return (note >> 16) & 15; }
@@ -163,7 +149,7 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
   __shared__ PieceNote notes[kRing];
   __shared__ uint32_t tmem_base_mem;
   __shared__ int failed_mem, scratch[32];
-  __shared__ uint32_t tile_notes[kRing], v_holes[kRing]; // of a tile of k; boxes of a tile of v that are not there
+  __shared__ uint32_t tile_notes[2][kRing];              // of the tiles of k, and of v
   __shared__ int odd_values[kRing];                      // of a piece: values that are no numbers were set to zero
   __shared__ float2 stats[2][kHalf];                     // maximum and sum of a half's rows (a unit of one item)
   volatile int* failed = &failed_mem;
@@ -228,41 +214,45 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
   share_of_block(work, begin, end);
   // the note of the block's i-th piece
   auto note_of = [&](int i, bool& ok) -> NotePtr {
-    if (ok) ok = bar_wait(noted(i), (uint32_t)((i / kRing) & 1), failed);
+    if (ok) ok = mbar_wait_f(noted(i), (uint32_t)((i / kRing) & 1), failed);
     return &notes[i % kRing];
   };
 
   if (warp >= 8) {
     regs_dec<kRegsOther>();
+    // The tiles of k or v of one piece after the other, by a whole warp.  Lane i brings box i of a tile of cached keys (a page, or 128 keys of
+    // one), or 32 drafted tokens; the page of the tile behind is requested before this one's copies and looked at after them.
     const int n_box = BN / ta.rows_box;
-    // the page of a lane's box of tile t, whose first key is key: -2 where nobody sees the box, -1 where it is not there
-    auto page_of = [&](NotePtr u, int t) {
+    auto entry = [&](NotePtr u, int t) {                         // what the block table says of this lane's box of tile t
       const int key = (u->first + t) * BN + lane * ta.rows_box;
-      if (t >= u->t0 + u->nt || t >= u->n_pre || lane >= n_box || key >= u->prefix || key + ta.rows_box <= u->lo) return -2;
-      const int page = a.block_table[(size_t)u->s * a.max_blocks + (key >> ta.block_shift)];       // (the prefix ends inside the table)
-      return page >= 0 && page < a.pages ? page : -1;
+      return t < u->n_pre && lane < n_box && key < u->prefix ? a.block_table[(size_t)u->s * a.max_blocks + (key >> ta.block_shift)] : -1;
     };
-    // tile t of k or v into `dst`, by the whole warp
-    auto bring = [&](NotePtr u, int t, int page, bool is_v, uint32_t dst, uint32_t bar) {
-      if (t >= u->n_pre) {                                       // drafted tokens: boxes of 32 rows
-        const int j0 = (t - u->n_pre) * BN, boxes = (min(BN, u->nk - j0) + 31) / 32;
-        if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(boxes * 32 * 128 * kHB));
-        __syncwarp();
+    // The tile's note goes out with it: the barrier's arrival is behind it.
+    auto bring = [&](NotePtr u, int t, int page, bool is_v, int g) {
+      const uint32_t bar = is_v ? v_full(g % kStages) : k_full(g % kStages), dst = (is_v ? sV : sK) + (g % kStages) * kTileBytes;
+      const bool nodes = t >= u->n_pre;
+      int key0, lo, hi;
+      rows_seen(u, t, key0, lo, hi);
+      const int key = key0 + lane * ta.rows_box;
+      const bool seen = !nodes && lane < n_box && key < u->prefix && key + ta.rows_box > u->lo, there = seen && page >= 0 && page < a.pages;
+      const uint32_t here = __ballot_sync(0xffffffffu, there), missing = __ballot_sync(0xffffffffu, seen && !there);
+      const int boxes = (hi + 31) / 32;                          // of drafted tokens
+      if (lane == 0) {
+        const bool all = lo == 0 && hi == BN && !missing && !seen_by_some(a, u, t, key0);
+        *(volatile uint32_t*)&tile_notes[is_v][g % kRing] = missing | ((uint32_t)(lo / 16) << 16) | ((uint32_t)((hi + 15) / 16) << 20) | (all ? kAllSeen : 0u);
+        mbar_arrive_expect_tx(bar, (uint32_t)((nodes ? boxes * 32 : __popc(here) * ta.rows_box) * 128 * kHB));
+      }
+      __syncwarp();
+      if (nodes) {
         if (lane < boxes) {
 #pragma unroll
           for (int hb = 0; hb < kHB; ++hb)
-            tma_load_box_3d(dst + hb * (BN * 128) + lane * (32 * 128), is_v ? &v_map : &k_map, hb * 64, u->kvh, u->start + j0 + lane * 32, bar);
+            tma_load_box_3d(dst + hb * (BN * 128) + lane * (32 * 128), is_v ? &v_map : &k_map, hb * 64, u->kvh, u->start + key0 + lane * 32, bar);
         }
-      } else {
-        const uint32_t here = __ballot_sync(0xffffffffu, page >= 0);
-        if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(__popc(here) * ta.rows_box * 128 * kHB));
-        __syncwarp();
-        if (page >= 0) {
-          const int slot = ((u->first + t) * BN + lane * ta.rows_box) & (a.block_size - 1);
+      } else if (there) {
 #pragma unroll
-          for (int hb = 0; hb < kHB; ++hb)
-            tma_load_box(dst + hb * (BN * 128) + lane * ta.rows_box * 128, &cache_map, hb * 64, slot, (is_v ? a.n_kv : 0) + u->kvh, page, bar);
-        }
+        for (int hb = 0; hb < kHB; ++hb)
+          tma_load_box(dst + hb * (BN * 128) + lane * ta.rows_box * 128, &cache_map, hb * 64, key & (a.block_size - 1), (is_v ? a.n_kv : 0) + u->kvh, page, bar);
       }
     };
     if (warp == 8) {
@@ -286,25 +276,15 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
       for (int i = 0, p = begin; p < end && ok; ++i) {
         NotePtr u = &notes[i % kRing];                           // (written by this warp)
         const int t0 = u->t0, nt = u->nt;
-        // before this warp waits for a piece's scores to free the queries, the note of the piece behind is there: warp 9 runs ahead with v
-        if (i > 0) leave_note(i + 1, p + nt);
-        int page = page_of(u, t0);
+        int page = entry(u, t0);
         for (int t = t0; t < t0 + nt && ok; ++t, ++g) {
           const int s = g % kStages;
-          if (g >= kStages && !bar_wait(k_empty(s), (uint32_t)((g / kStages - 1) & 1), failed)) { ok = false; break; }
-          const int next = page_of(u, t + 1);
-          const uint32_t missing = __ballot_sync(0xffffffffu, page == -1);
-          if (lane == 0) {
-            int key0, lo, hi;
-            rows_seen(u, t, key0, lo, hi);
-            const bool all = lo == 0 && hi == BN && !missing && !seen_by_some(a, u, t, key0);
-            tile_notes[g % kRing] = missing | ((uint32_t)(lo / 16) << 16) | ((uint32_t)((hi + 15) / 16) << 20) | (all ? kAllSeen : 0u);
-          }
-          __syncwarp();
-          bring(u, t, page, false, sK + s * kTileBytes, k_full(s));
+          if (g >= kStages && !mbar_wait_f(k_empty(s), (uint32_t)((g / kStages - 1) & 1), failed)) { ok = false; break; }
+          const int next = t + 1 < t0 + nt ? entry(u, t + 1) : -1;
+          bring(u, t, page, false, g);
           page = next;
           if (t == t0) {                                         // the queries, as soon as the piece before has issued its last scores
-            if (i > 0 && !bar_wait(q_free, (uint32_t)((i - 1) & 1), failed)) { ok = false; ++g; break; }
+            if (i > 0 && !mbar_wait_f(q_free, (uint32_t)((i - 1) & 1), failed)) { ok = false; ++g; break; }
             if (lane == 0) {
               const int items = u->two ? 2 : 1;
               mbar_arrive_expect_tx(q_full, (uint32_t)(items * rows_item * 128 * kHB));
@@ -314,64 +294,57 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
                   tma_load_box_3d(sQ + x * kTileBytes + hb * (BM * 128), &q_map, hb * 64, u->kvh * a.group, u->start + (u->item + x) * ta.nodes_per_item, q_full);
             }
             __syncwarp();
-            if (i == 0) leave_note(1, p + nt);
           }
+          if (t == min(t0 + 1, t0 + nt - 1)) leave_note(i + 1, p + nt);      // (behind the first copies)
         }
         p += nt;
         if (p >= end && ok) {                                    // the last queries, and the arrival behind them
-          bar_drain(q_full, (uint32_t)(i & 1));
-          ok = bar_wait(q_free, (uint32_t)(i & 1), failed);
+          mbar_wait_drain(q_full, (uint32_t)(i & 1));
+          ok = mbar_wait_f(q_free, (uint32_t)(i & 1), failed);
         }
       }
       // no copy of this block may be in flight when it ends, nor an arrival on its barriers
-      for (int i = max(0, g - kStages); i < g; ++i) bar_drain(k_full(i % kStages), (uint32_t)((i / kStages) & 1));
-      for (int i = max(0, g - kStages); i < g && ok; ++i) ok = bar_wait(k_empty(i % kStages), (uint32_t)((i / kStages) & 1), failed);
-      if (!ok) bar_drain(q_full, 0u), bar_drain(q_full, 1u);
+      for (int i = max(0, g - kStages); i < g; ++i) mbar_wait_drain(k_full(i % kStages), (uint32_t)((i / kStages) & 1));
+      for (int i = max(0, g - kStages); i < g && ok; ++i) ok = mbar_wait_f(k_empty(i % kStages), (uint32_t)((i / kStages) & 1), failed);
+      if (!ok) mbar_wait_drain(q_full, 0u), mbar_wait_drain(q_full, 1u);
     } else if (warp == 9) {
-      // ------------------------------------------------------------------ tiles of v, and those of them that are not for everybody
-      // a tile is brought when the one whose place it takes has been multiplied, and gone over when it has landed; the two are a
-      // ring apart and lie in different pieces at times
-      int gp = 0, ip = 0, tp = 0, page = -2;                     // the next tile to bring: its number, its piece, its place in the unit
-      bool ok = true;
-      NotePtr up = nullptr;
-      const int total = end - begin;
-      auto bring_next = [&]() {
-        if (gp >= total) return;
-        const int s = gp % kStages;
-        if (gp >= kStages) ok = bar_wait(v_empty(s), (uint32_t)((gp / kStages - 1) & 1), failed);
-        if (ok && (!up || tp >= up->t0 + up->nt)) {
-          if (up) ++ip;
-          up = note_of(ip, ok);
-          if (ok) {
-            tp = up->t0;
-            page = page_of(up, tp);
-          }
-        }
-        if (!ok) return;
-        const int next = page_of(up, tp + 1);
-        const uint32_t missing = __ballot_sync(0xffffffffu, page == -1);
-        if (lane == 0) v_holes[gp % kRing] = missing;
-        bring(up, tp, page, true, sV + s * kTileBytes, v_full(s));
-        page = next;
-        ++tp;
-        ++gp;
-      };
-      for (int k = 0; k + 1 < kStages && ok; ++k) bring_next();
+      // ------------------------------------------------------------------ tiles of v
       int g = 0;
-      for (int i = 0; g < total && ok; ++i) {
+      bool ok = true;
+      for (int i = 0, p = begin; p < end && ok; ++i) {
+        NotePtr u = note_of(i, ok);
+        if (!ok) break;
+        const int t0 = u->t0, nt = u->nt;
+        int page = entry(u, t0);
+        for (int t = t0; t < t0 + nt; ++t, ++g) {
+          const int s = g % kStages;
+          if (g >= kStages && !mbar_wait_f(v_empty(s), (uint32_t)((g / kStages - 1) & 1), failed)) { ok = false; break; }
+          const int next = t + 1 < t0 + nt ? entry(u, t + 1) : -1;
+          bring(u, t, page, true, g);
+          page = next;
+        }
+        p += nt;
+      }
+      for (int i = max(0, g - kStages); i < g; ++i) mbar_wait_drain(v_full(i % kStages), (uint32_t)((i / kStages) & 1));
+      for (int i = max(0, g - kStages); i < g && ok; ++i) ok = mbar_wait_f(v_empty(i % kStages), (uint32_t)((i / kStages) & 1), failed);
+    } else if (warp == 11) {
+      // ------------------------------------------------------------------ tiles of v that are not for everybody
+      int g = 0;
+      bool ok = true;
+      for (int i = 0, p = begin; p < end && ok; ++i) {
         NotePtr u = note_of(i, ok);
         if (!ok) break;
         const int t0 = u->t0, nt = u->nt;
         if (lane == 0) odd_values[i % kRing] = 0;
         for (int t = t0; t < t0 + nt && ok; ++t, ++g) {
           const int s = g % kStages;
-          ok = bar_wait(v_full(s), (uint32_t)((g / kStages) & 1), failed);
+          ok = mbar_wait_f(v_full(s), (uint32_t)((g / kStages) & 1), failed);
           if (!ok) break;
-          int key0, lo, hi;
-          rows_seen(u, t, key0, lo, hi);
-          const bool some = seen_by_some(a, u, t, key0);
-          const uint32_t missing = v_holes[g % kRing];
-          if (some || lo > 0 || hi < BN || missing) {
+          const uint32_t note = *(volatile uint32_t*)&tile_notes[1][g % kRing], missing = note & 0xffffu;
+          if (!(note & kAllSeen)) {
+            int key0, lo, hi;
+            rows_seen(u, t, key0, lo, hi);
+            const bool some = seen_by_some(a, u, t, key0);
             // eight lanes a row, four rows at a time, and the 64-wide blocks of the head one after the other
             const uint32_t v = sV + s * kTileBytes + (lane & 7) * 16;
             const int r_lane = lane >> 3;
@@ -426,12 +399,10 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
             fence_async_smem();
           }
           __syncwarp();
-          if (lane == 0) mbar_arrive(v_fixed(s));
-          bring_next();
+          arrive_if(lane == 0, v_fixed(s));
         }
+        p += nt;
       }
-      for (int i = max(0, gp - kStages); i < gp; ++i) bar_drain(v_full(i % kStages), (uint32_t)((i / kStages) & 1));
-      for (int i = max(0, gp - kStages); i < gp && ok; ++i) ok = bar_wait(v_empty(i % kStages), (uint32_t)((i / kStages) & 1), failed);
     } else if (warp == 10) {
       // ------------------------------------------------------------------ products
       constexpr uint32_t idesc_s = instr_desc(BM, BN, 0), idesc_o = instr_desc(BM, HD, 1);
@@ -453,7 +424,7 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
             umma(leader, tmem + x * BN, dq + (off >> 4), dk + (off >> 4), idesc_s, ks > 0);
           }
           umma_commit(leader, s_full(x));
-          if (leader) mbar_arrive(s_full(x));
+          arrive_if(leader, s_full(x));
           if (!two || x == 1) {
             umma_commit(leader, k_empty(s));
             if (j == nt - 1) umma_commit(leader, q_free);        // (a tile's scores are issued in the tiles' order)
@@ -463,11 +434,11 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
         auto k_wait = [&](int j) {
           if (k_ready >= j) return;
           const int g = g0 + j;
-          ok = bar_wait(k_full(g % kStages), (uint32_t)((g / kStages) & 1), failed);
+          ok = mbar_wait_f(k_full(g % kStages), (uint32_t)((g / kStages) & 1), failed);
           tc_fence_after();
           k_ready = j;
         };
-        ok = bar_wait(q_full, (uint32_t)(i & 1), failed);
+        ok = mbar_wait_f(q_full, (uint32_t)(i & 1), failed);
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           const int j = two ? 0 : x;
@@ -476,9 +447,11 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
         }
         for (int j = 0; j < nt && ok; ++j) {
           const int g = g0 + j, s = g % kStages;
-          const uint32_t note = *(volatile uint32_t*)&tile_notes[g % kRing];
+          const uint32_t note = *(volatile uint32_t*)&tile_notes[0][g % kRing];
           const uint64_t dv = dv0 + (uint64_t)((s * kTileBytes) >> 4);
-          ok = bar_wait(v_full(s), (uint32_t)((g / kStages) & 1), failed) && bar_wait(v_fixed(s), (uint32_t)((g / kStages) & 1), failed);
+          const int jn = j + every;
+          // (v has landed and, where that was to be done, been gone over: warp 11 says so of every tile)
+          ok = mbar_wait_f(v_fixed(s), (uint32_t)((g / kStages) & 1), failed);
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
             if (!ok || (!two && x != (j & 1))) continue;
@@ -486,7 +459,7 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
             const bool first = j < every;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              if (ok) ok = bar_wait(p_full(x, h), phase, failed);
+              if (ok) ok = mbar_wait_f(p_full(x, h), phase, failed);
               if (!ok) continue;
               tc_fence_after();
 #pragma unroll
@@ -499,12 +472,12 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
             if (!ok) continue;
             ++n_p[x];
             if (!two || x == 1) umma_commit(leader, v_empty(s));
-            if (j + every < nt) {
-              k_wait(j + every);
-              if (ok) issue_s(x, j + every);
+            if (jn < nt) {
+              k_wait(jn);
+              if (ok) issue_s(x, jn);
             } else {
               umma_commit(leader, o_done(x));
-              if (leader) mbar_arrive(o_done(x));
+              arrive_if(leader, o_done(x));
             }
           }
         }
@@ -522,8 +495,8 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
     bool ok = true;
     auto meet = [&]() {
       __syncwarp();
-      if (lane == 0) mbar_arrive(met);
-      ok = bar_wait(met, (uint32_t)(n_met & 1), failed);
+      arrive_if(lane == 0, met);
+      ok = mbar_wait_f(met, (uint32_t)(n_met & 1), failed);
       ++n_met;
     };
     for (int i_piece = 0, p = begin; p < end; ++i_piece) {
@@ -548,20 +521,18 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
           for (int i = 0; i < 4; ++i) sees[i] = mine && w0 + i < n_words ? mask_word(w0 + i) : 0u;
         }
         // S of the tile is complete, and with it every product issued before it: P V of this half's tile before too
-        ok = bar_wait(s_full(x), (uint32_t)(n_s & 1), failed);
+        ok = mbar_wait_f(s_full(x), (uint32_t)(n_s & 1), failed);
         if (!ok) break;
         if (!any_mine) {                                         // a warp without rows: its P is never looked at
-          if (lane == 0) {
-            mbar_arrive(p_full(x, 0));
-            mbar_arrive(p_full(x, 1));
-          }
+          arrive_if(lane == 0, p_full(x, 0));
+          arrive_if(lane == 0, p_full(x, 1));
           continue;
         }
         tc_fence_after();
         float sc[BN];
 #pragma unroll
         for (int c = 0; c < BN; c += 32) tmem_ld32_issue(t_s + c, sc + c);
-        const uint32_t note = *(volatile uint32_t*)&tile_notes[(p - begin + j) % kRing];
+        const uint32_t note = *(volatile uint32_t*)&tile_notes[0][(p - begin + j) % kRing];
         if (note & kAllSeen) {
           tmem_wait_ld();
         } else {                                                 // what the row sees of the tile's keys, as bits
@@ -630,13 +601,13 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
           tmem_wait_st();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(p_full(x, h));
+          arrive_if(lane == 0, p_full(x, h));
         }
         float l0, l1;
         upk2(sum, l0, l1);
         l += l0 + l1;
       }
-      if (ok && have) ok = bar_wait(o_done(x), (uint32_t)(n_o & 1), failed);
+      if (ok && have) ok = mbar_wait_f(o_done(x), (uint32_t)(n_o & 1), failed);
       if (!ok) break;
       n_o += have;
       tc_fence_after();
