@@ -38,7 +38,7 @@ __global__ void __launch_bounds__(kThreads) attention_tree_kernel(Args a, bool w
   pdl_launch_dependents();
   pdl_wait();
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-  add_up_work<kKeys>(a, kRows, 1, lens, offs, scratch);
+  add_up_work<kKeys>(a, kRows, lens, offs, scratch);
   int begin, end;
   share_of_block(offs[a.n_seqs], begin, end);
   const int b = blockIdx.x;
@@ -46,7 +46,7 @@ __global__ void __launch_bounds__(kThreads) attention_tree_kernel(Args a, bool w
   __syncthreads();
   const T* q = (const T*)a.q;
   for (int p = begin; p < end;) {
-    const Piece u = piece_at<kKeys>(a, lens, offs, 1, p, end);
+    const Piece u = piece_at<kKeys, 1>(a, lens, offs, p, end);
     const int row0 = u.item * kRows, rows = min(kRows, u.r.n * a.group - row0);
     const int* table = a.block_table + (size_t)u.s * a.max_blocks;
     __syncthreads();
@@ -213,9 +213,9 @@ __global__ void __launch_bounds__(kThreads) attention_tree_kernel(Args a, bool w
           o[(size_t)quads * 4 * kRows + kRows + row] = l[i];
         }
       }
-      if (begins && tid == 0) a.notes[b] = make_int4(u.s, u.kvh, row0, rows | (block_of_tile(offs[a.n_seqs], p + u.r.tiles - 1) << 8));
+      if (begins && tid == 0) a.notes[b] = make_int4(u.s, u.kvh, row0, rows | (block_of(offs[a.n_seqs], u.last) << 8));
     }
-    p += u.t1 - u.t0;
+    p = u.next;
   }
 }
 

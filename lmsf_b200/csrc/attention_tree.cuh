@@ -6,7 +6,7 @@
 //
 // The work is cut as follows.  A unit is (request, kv head, item of up to kRows rows); it has the request's tiles of kKeys keys: its
 // cached keys first, then the nodes.  All units' tiles in a row, requests in order, are shared out evenly over the blocks, whatever the
-// lengths are; no plan is made on the host, so a captured launch serves any lengths.  A unit that lies in one block's range is finished there.  Of a unit that is cut every block leaves a
+// lengths are, a tile of a unit of two items counted twice; no plan is made on the host, so a captured launch serves any lengths.  A unit that lies in one block's range is finished there.  Of a unit that is cut every block leaves a
 // partial (unnormalised output, running maximum, sum; float32) in the workspace: at most two for a block (and item), one for the unit
 // that it begins with and one for the unit that it ends with.  A second kernel adds them up in the order of the blocks; both
 // depend only on lengths and G, so the result is the same in every run.
@@ -63,11 +63,11 @@ __device__ __forceinline__ Request request(const Args& a, const Lengths& l) {
   return r;
 }
 
-// What a block keeps of the step in shared memory: all[s], and offs[s] = tiles before request s, for 0 <= s <= n_seqs.
+// What a block keeps of the step in shared memory: all[s], and offs[s] = work before request s (a tile for an item is one), for 0 <= s <= n_seqs.
 __host__ __device__ __forceinline__ size_t work_bytes(int n_seqs) { return (size_t)n_seqs * sizeof(Lengths) + (size_t)(n_seqs + 1) * sizeof(int); }
 // By all threads of the block (a multiple of 32, at most 1024).
 template <int kKeys>
-__device__ __forceinline__ void add_up_work(const Args& a, int rows, int items_per_unit, Lengths* all, int* offs, int* scratch) {
+__device__ __forceinline__ void add_up_work(const Args& a, int rows, Lengths* all, int* offs, int* scratch) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = blockDim.x >> 5;
   const int per = (a.n_seqs + blockDim.x - 1) / blockDim.x;
   const int s0 = min(tid * per, a.n_seqs), s1 = min(s0 + per, a.n_seqs);
@@ -76,7 +76,7 @@ __device__ __forceinline__ void add_up_work(const Args& a, int rows, int items_p
     const Lengths l = lengths(a, s, rows);
     all[s] = l;
     offs[s] = sum;
-    sum += request<kKeys>(a, l).tiles * ((l.items + items_per_unit - 1) / items_per_unit) * a.n_kv;
+    sum += request<kKeys>(a, l).tiles * l.items * a.n_kv;
   }
   int x = sum;
 #pragma unroll
@@ -97,10 +97,10 @@ __device__ __forceinline__ void add_up_work(const Args& a, int rows, int items_p
   __syncthreads();
 }
 
-// Blocks that take part in `work` tiles: two tiles each at the least (a short unit that is cut costs more than its second tile), and none
-// with an empty share between the pieces of a unit.
-__device__ __forceinline__ int blocks_for(int work) { return min((int)gridDim.x, (work + 1) / 2); }
-// The tiles that this block takes of them: every block as many as every other, the first `work % blocks` one more.
+// Blocks that take part in `work`: two places each at the least (a short unit that is cut costs more than its second tile; and a share of one place
+// might have no tile), none with an empty share between the pieces of a unit.
+__device__ __forceinline__ int blocks_for(int work) { return min((int)gridDim.x, max(work / 2, 1)); }
+// What this block takes of it: every block as much as every other, the first `work % blocks` one more.
 __device__ __forceinline__ void share_of_block(int work, int& begin, int& end) {
   const int b = blockIdx.x, blocks = blocks_for(work);
   begin = end = 0;
@@ -109,13 +109,13 @@ __device__ __forceinline__ void share_of_block(int work, int& begin, int& end) {
   begin = b * each + min(b, more);
   end = begin + each + (b < more ? 1 : 0);
 }
-// The block that has tile p of all `work` tiles.
-__device__ __forceinline__ int block_of_tile(int work, int p) {
+// The block whose share place p lies in.
+__device__ __forceinline__ int block_of(int work, int p) {
   const int blocks = blocks_for(work), each = work / blocks, more = work - each * blocks, edge = more * (each + 1);
   return p < edge ? p / (each + 1) : more + (p - edge) / each;
 }
 
-// The request whose tiles hold place p (0 <= p < offs[n_seqs]).
+// The request that place p lies in (0 <= p < offs[n_seqs]).
 __device__ __forceinline__ int request_at(const int* offs, int n_seqs, int p) {
   int lo = 0, hi = n_seqs;                                       // offs[lo] <= p < offs[hi]
   while (hi - lo > 1) {
@@ -126,18 +126,25 @@ __device__ __forceinline__ int request_at(const int* offs, int n_seqs, int p) {
   return lo;
 }
 
-// A block's share of one unit: tiles [t0, t1) of the unit's.
-struct Piece { int s, kvh, item, t0, t1; Request r; };
-template <int kKeys>
-__device__ __forceinline__ Piece piece_at(const Args& a, const Lengths* all, const int* offs, int items_per_unit, int p, int end) {
+// A block's share of one unit of up to kItems items: tiles [t0, t1) of the unit's.  Tile t of a unit of two items has the places 2 t and
+// 2 t + 1 and belongs to the block that has the first of them.  next: the place behind the unit, or the block's end; last: the place that the
+// unit's last tile is found by.  A share that begins with a unit's last place has no tile of it: t0 = t1.
+struct Piece { int s, kvh, item, t0, t1, next, last; bool two; Request r; };
+template <int kKeys, int kItems>
+__device__ __forceinline__ Piece piece_at(const Args& a, const Lengths* all, const int* offs, int p, int end) {
   Piece x;
   x.s = request_at(offs, a.n_seqs, p);
   x.r = request<kKeys>(a, all[x.s]);
-  const int units = (x.r.items + items_per_unit - 1) / items_per_unit, rem = p - offs[x.s], u = rem / x.r.tiles;
-  x.t0 = rem - u * x.r.tiles;
-  x.t1 = min(x.r.tiles, x.t0 + (end - p));
-  x.kvh = u / units;
-  x.item = (u - x.kvh * units) * items_per_unit;                         // the unit's first item: its neighbours read the same keys
+  const int rem = p - offs[x.s], per_head = x.r.tiles * x.r.items;
+  x.kvh = rem / per_head;
+  const int in_head = rem - x.kvh * per_head, unit = in_head / (kItems * x.r.tiles);
+  x.item = unit * kItems;                                        // the unit's first item: its neighbours read the same keys
+  x.two = kItems == 2 && x.item + 1 < x.r.items;
+  const int off = in_head - unit * kItems * x.r.tiles, size = (x.two ? 2 : 1) * x.r.tiles, off_end = min(size, off + (end - p));
+  x.t0 = x.two ? (off + 1) / 2 : off;
+  x.t1 = x.two ? (off_end + 1) / 2 : off_end;
+  x.next = p + (off_end - off);
+  x.last = p - off + size - (x.two ? 2 : 1);
   return x;
 }
 

@@ -117,7 +117,7 @@ __device__ __forceinline__ uint32_t bits(int lo, int hi) {
 
 // What the warps of a block need to know of a piece, left in shared memory by warp 11 a piece ahead.  They read it where they need it:
 // held in registers it would not fit beside a row's scores, nor into what the other warps keep.
-struct __align__(16) PieceNote { int s, kvh, item, t0, nt, start, n, nk, prefix, lo, first, n_pre, tiles, two, last, pad; };   // last: the block that ends the unit
+struct __align__(16) PieceNote { int s, kvh, item, t0, nt, start, n, nk, prefix, lo, first, n_pre, tiles, two, last, next; };   // last: the block that ends the unit
 typedef const volatile PieceNote* NotePtr;
 // Rows [lo, hi) of a tile are seen by some row of the piece's request; none of the others is multiplied, but for those that share a step
 // of 16 with them.
@@ -203,7 +203,7 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
   }
   pdl_wait();
   const int rows_item = ta.nodes_per_item * a.group;
-  add_up_work<BN>(a, rows_item, 2, lens, offs, scratch);
+  add_up_work<BN>(a, rows_item, lens, offs, scratch);
   if (tid < 2) a.notes[2 * blockIdx.x + tid] = make_int4(-1, 0, 0, 0);
   tc_fence_before();
   __syncthreads();
@@ -261,13 +261,15 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
       bool ok = true;
       auto leave_note = [&](int i, int p) {
         if (p >= end) return;
-        const Piece u = piece_at<BN>(a, lens, offs, 2, p, end);
+        Piece u = piece_at<BN, 2>(a, lens, offs, p, end);
+        if (u.t0 == u.t1) u = piece_at<BN, 2>(a, lens, offs, u.next, end);       // (the block's first place was a unit's last)
         if (lane == 0) {
           volatile PieceNote* n = &notes[i % kRing];
           n->s = u.s; n->kvh = u.kvh; n->item = u.item; n->t0 = u.t0; n->nt = u.t1 - u.t0; n->start = u.r.start; n->n = u.r.n; n->nk = u.r.nk;
           n->prefix = u.r.prefix; n->lo = u.r.lo; n->first = u.r.first; n->n_pre = u.r.n_pre; n->tiles = u.r.tiles;
-          n->two = u.item + 1 < u.r.items;
-          n->last = u.t0 == 0 && u.t1 < u.r.tiles ? block_of_tile(work, p + u.r.tiles - 1) : 0;
+          n->two = u.two;
+          n->last = u.t0 == 0 && u.t1 < u.r.tiles ? block_of(work, u.last) : 0;
+          n->next = u.next;
           mbar_arrive(noted(i));
         }
         __syncwarp();
@@ -295,9 +297,9 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
             }
             __syncwarp();
           }
-          if (t == min(t0 + 1, t0 + nt - 1)) leave_note(i + 1, p + nt);      // (behind the first copies)
+          if (t == min(t0 + 1, t0 + nt - 1)) leave_note(i + 1, u->next);      // (behind the first copies)
         }
-        p += nt;
+        p = u->next;
         if (p >= end && ok) {                                    // the last queries, and the arrival behind them
           mbar_wait_drain(q_full, (uint32_t)(i & 1));
           ok = mbar_wait_f(q_free, (uint32_t)(i & 1), failed);
@@ -323,7 +325,7 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
           bring(u, t, page, true, g);
           page = next;
         }
-        p += nt;
+        p = u->next;
       }
       for (int i = max(0, g - kStages); i < g; ++i) mbar_wait_drain(v_full(i % kStages), (uint32_t)((i / kStages) & 1));
       for (int i = max(0, g - kStages); i < g && ok; ++i) ok = mbar_wait_f(v_empty(i % kStages), (uint32_t)((i / kStages) & 1), failed);
@@ -401,7 +403,7 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
           __syncwarp();
           arrive_if(lane == 0, v_fixed(s));
         }
-        p += nt;
+        p = u->next;
       }
     } else if (warp == 10) {
       // ------------------------------------------------------------------ products
@@ -482,7 +484,7 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
           }
         }
         g0 += nt;
-        p += nt;
+        p = u->next;
       }
     }
   } else {
@@ -491,7 +493,7 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
     const int x = warp >> 2, row = tid & 127;
     const uint32_t t_s = tmem + ((uint32_t)((warp & 3) * 32) << 16) + x * BN, t_o = t_s + kOCol;
     const float sl2 = a.scale * kLog2e;
-    int n_s = 0, n_o = 0, n_met = 0;                             // scores and outputs of this half so far, meetings of the two
+    int n_s = 0, n_o = 0, n_met = 0, g0 = 0;                             // scores and outputs of this half so far, meetings of the two; tiles of the block
     bool ok = true;
     auto meet = [&]() {
       __syncwarp();
@@ -532,7 +534,7 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
         float sc[BN];
 #pragma unroll
         for (int c = 0; c < BN; c += 32) tmem_ld32_issue(t_s + c, sc + c);
-        const uint32_t note = *(volatile uint32_t*)&tile_notes[0][(p - begin + j) % kRing];
+        const uint32_t note = *(volatile uint32_t*)&tile_notes[0][(g0 + j) % kRing];
         if (note & kAllSeen) {
           tmem_wait_ld();
         } else {                                                 // what the row sees of the tile's keys, as bits
@@ -724,7 +726,8 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
       tc_fence_before();
       if (!two) meet();
       if (!ok) break;
-      p += nt;
+      p = u->next;
+      g0 += nt;
     }
   }
   tc_fence_before();
