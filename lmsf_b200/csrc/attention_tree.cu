@@ -7,34 +7,67 @@ LMSF_DEFINE_LAST_ERROR(lmsf_attention_tree)
 namespace lmsf {
 namespace tree {
 
-constexpr int kRows = 32, kKeys = 64, kThreads = 256;
-
-// Four values of a row from column c on, zeros behind the head size.
-template <typename T>
-__device__ __forceinline__ void load4(const T* p, int c, int hd, bool wide, float (&v)[4]) {
-  if (wide && c + 4 <= hd) {
-    ld4(p + c, v);
-    return;
-  }
-#pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] = c + e < hd ? to_f32(p[c + e]) : 0.f;
+constexpr int kRows = 32, kThreads = 128;
+// Keys of a tile: two tiles of keys and two of values lie in shared memory, for head sizes up to 128 twice per SM.
+template <int HDP> constexpr int kTile = HDP <= 64 ? 64 : 32;
+template <typename T, int HDP> constexpr int kPitch = HDP + 16 / (int)sizeof(T);         // of a row in shared memory: 16 bytes more, for the banks
+template <typename T, int HDP> constexpr size_t smem_bytes(int n_seqs) {
+  return sizeof(float) * kRows * (HDP + 4) + sizeof(T) * 4 * kTile<HDP> * kPitch<T, HDP> + sizeof(float) * kRows * (kTile<HDP> + 4) + sizeof(ulonglong2) * 2 * kTile<HDP>
+         + work_bytes(n_seqs);
 }
 
-// One pass over the keys with the running maximum and sum of the softmax.  A tile of 64 keys lies in shared memory as float32
-// (keys for the scores, then values in the same place); thread (ty, tx) = (tid / 16, tid % 16) has the scores of rows 2 ty, 2 ty + 1
-// with keys tx + 16 j and the output's columns 64 c + 4 tx .. + 3.
+__device__ __forceinline__ uint64_t pk2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void upk2(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+// Four neighbouring values of shared memory as two pairs.
+__device__ __forceinline__ void pairs(const float* p, uint64_t& a, uint64_t& b) {
+  const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(p);
+  a = v.x;
+  b = v.y;
+}
+__device__ __forceinline__ void pairs(const bf16* p, uint64_t& a, uint64_t& b) {
+  float v[4];
+  ld4(p, v);
+  a = pk2(v[0], v[1]);
+  b = pk2(v[2], v[3]);
+}
+__device__ __forceinline__ void copy16(void* dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_sent() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copies_but() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ bool is_odd(float v) { return !(fabsf(v) <= 3.4028235e38f); }
+
+// One pass over the keys with the running maximum and sum of the softmax.  Thread (ty, tx) = (tid / 16, tid % 16) has the scores of rows
+// 4 ty .. 4 ty + 3 with keys tx + 16 j and of the same rows' output the columns 64 c + 4 tx .. + 3, in packed pairs of float32: the products of
+// 32 rows with 64 keys are bound by the FMA pipe then (48 shared-memory wavefronts beside 64 cycles of packed FMAs), where 8 scores a
+// thread were bound by shared memory.  The next tile's keys are on their way while this one's scores are computed, its values while
+// its weights are (cp.async, two tiles each).
 template <typename T, int HDP>
 __global__ void __launch_bounds__(kThreads) attention_tree_kernel(Args a, bool wide) {
-  constexpr int kPitch = HDP + 4;
-  extern __shared__ float smem[];
-  float* qs = smem;                                              // [kRows][kPitch]
-  float* kv = qs + kRows * kPitch;                               // [kKeys][kPitch]
-  float* ps = kv + kKeys * kPitch;                               // [kRows][kKeys + 4]
-  int* there = (int*)(ps + kRows * (kKeys + 4));                 // [kKeys] whether any row may see the key
-  Lengths* lens = (Lengths*)(there + kKeys);                     // [n_seqs]
+  constexpr int kKeys = kTile<HDP>, kJ = kKeys / 16, kC = HDP / 64, kP = kPitch<T, HDP>, kQP = HDP + 4, kPP = kKeys + 4;
+  extern __shared__ __align__(16) unsigned char smem[];
+  float* qs = (float*)smem;                                      // [kRows][kQP]
+  T* ks = (T*)(qs + kRows * kQP);                                // [2][kKeys][kP]
+  T* vs = ks + 2 * kKeys * kP;                                   // [2][kKeys][kP]
+  float* ps = (float*)(vs + 2 * kKeys * kP);                     // [kRows][kPP]
+  ulonglong2* rows_at = (ulonglong2*)(ps + kRows * kPP);         // [2][kKeys] addresses of a key's and its value's row, 0 where there is none
+  Lengths* lens = (Lengths*)(rows_at + 2 * kKeys);               // [n_seqs]
   int* offs = (int*)(lens + a.n_seqs);                           // [n_seqs + 1]
   __shared__ int scratch[32];
-  constexpr int kPP = kKeys + 4;
   pdl_launch_dependents();
   pdl_wait();
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
@@ -49,189 +82,241 @@ __global__ void __launch_bounds__(kThreads) attention_tree_kernel(Args a, bool w
     const Piece u = piece_at<kKeys, 1>(a, lens, offs, p, end);
     const int row0 = u.item * kRows, rows = min(kRows, u.r.n * a.group - row0);
     const int* table = a.block_table + (size_t)u.s * a.max_blocks;
+    // thread j < kKeys: where row j of tile t lies (asked for an iteration before its copies are, which every thread makes some of)
+    auto find_row = [&](int t) {
+      ulonglong2 at = make_ulonglong2(0ull, 0ull);
+      if (tid >= kKeys || t >= u.t1) return at;
+      if (t >= u.r.n_pre) {
+        const int key = (t - u.r.n_pre) * kKeys + tid;
+        if (key < u.r.nk) {
+          at.x = (unsigned long long)((const T*)a.k + (u.r.start + key) * a.k_stride + (size_t)u.kvh * a.hd);
+          at.y = (unsigned long long)((const T*)a.v + (u.r.start + key) * a.v_stride + (size_t)u.kvh * a.hd);
+        }
+        return at;
+      }
+      const int key = (u.r.first + t) * kKeys + tid;
+      if (key < u.r.lo || key >= u.r.prefix) return at;
+      const int block = key / a.block_size, page = table[block];
+      if (page < 0 || page >= a.pages) return at;
+      const T* row = (const T*)a.cache + page * a.page_stride + ((size_t)u.kvh * a.block_size + (key - block * a.block_size)) * a.hd;
+      at.x = (unsigned long long)row;
+      at.y = (unsigned long long)(row + a.v_off);
+      return at;
+    };
+    auto note_row = [&](int t, ulonglong2 at) {
+      if (tid < kKeys) rows_at[(t & 1) * kKeys + tid] = at;
+    };
+    constexpr int kE = 16 / (int)sizeof(T), kChunks = HDP / kE;  // values and copies of 16 bytes
+    auto request_tile = [&](int t, bool value) {
+      T* dst = (value ? vs : ks) + (t & 1) * kKeys * kP;
+#pragma unroll 4
+      for (int i = tid; i < kKeys * kChunks; i += kThreads) {
+        const int j = i / kChunks, c = (i % kChunks) * kE;
+        const ulonglong2 at = rows_at[(t & 1) * kKeys + j];
+        const T* src = (const T*)(value ? at.y : at.x);
+        if (wide) {                                              // whole rows of 16-byte words
+          copy16(dst + j * kP + c, src && c < a.hd ? (const void*)(src + c) : (const void*)a.cache, src && c < a.hd);
+        } else {
+#pragma unroll
+          for (int e = 0; e < kE; ++e) dst[j * kP + c + e] = src && c + e < a.hd ? src[c + e] : from_f32<T>(0.f);
+        }
+      }
+      copies_sent();
+    };
+    const ulonglong2 at0 = find_row(u.t0), at1 = find_row(u.t0 + 1);
     __syncthreads();
+    note_row(u.t0, at0);
+    note_row(u.t0 + 1, at1);
+    __syncthreads();
+    request_tile(u.t0, false);
+    request_tile(u.t0, true);
     for (int i = tid; i < kRows * (HDP / 4); i += kThreads) {
       const int row = i / (HDP / 4), c = (i % (HDP / 4)) * 4, r = row0 + row;
       float x[4] = {0.f, 0.f, 0.f, 0.f};
-      if (row < rows) load4(q + (u.r.start + r / a.group) * a.q_stride + (size_t)(u.kvh * a.group + r % a.group) * a.hd, c, a.hd, wide, x);
+      if (row < rows) {
+        const T* src = q + (u.r.start + r / a.group) * a.q_stride + (size_t)(u.kvh * a.group + r % a.group) * a.hd;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) qs[row * kPitch + c + e] = x[e] * (a.scale * 1.4426950408889634f);
+        for (int e = 0; e < 4; ++e)
+          if (c + e < a.hd) x[e] = to_f32(src[c + e]) * (a.scale * 1.4426950408889634f);
+      }
+      st4(qs + row * kQP + c, x);
     }
-    int node[2], after[2];                                       // of this thread's rows: node, and the cached key behind which it sees
-    float m[2], l[2], acc[2][HDP / 64][4];
+    int node[4], after[4];                                       // of this thread's rows: node, and the cached key behind which it sees
+    float m[4], l[4];
+    uint64_t acc[4][kC][2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int row = 2 * ty + i;
+    for (int i = 0; i < 4; ++i) {
+      const int row = 4 * ty + i;
       node[i] = row < rows ? (row0 + row) / a.group : -1;
       after[i] = node[i] >= 0 && a.window > 0 ? a.positions[u.r.start + node[i]] - a.window : -1;
       m[i] = -INFINITY;
       l[i] = 0.f;
 #pragma unroll
-      for (int c = 0; c < HDP / 64; ++c)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i][c][e] = 0.f;
+      for (int c = 0; c < kC; ++c) acc[i][c][0] = acc[i][c][1] = 0ull;
     }
     for (int t = u.t0; t < u.t1; ++t) {
       const bool nodes = t >= u.r.n_pre;                         // a tile of drafted keys
       const int key0 = nodes ? (t - u.r.n_pre) * kKeys : (u.r.first + t) * kKeys;
-      // the address of a key's (or value's) row, null where there is none
-      auto row_of = [&](int j, bool value) -> const T* {
-        const int key = key0 + j;
-        if (nodes) {
-          if (key >= u.r.nk) return nullptr;
-          return value ? (const T*)a.v + (u.r.start + key) * a.v_stride + (size_t)u.kvh * a.hd
-                       : (const T*)a.k + (u.r.start + key) * a.k_stride + (size_t)u.kvh * a.hd;
-        }
-        if (key < u.r.lo || key >= u.r.prefix) return nullptr;
-        const int page = table[key / a.block_size];
-        if (page < 0 || page >= a.pages) return nullptr;
-        return (const T*)a.cache + page * a.page_stride + (value ? a.v_off : 0) + ((size_t)u.kvh * a.block_size + key % a.block_size) * a.hd;
-      };
+      // sent so far: k and v up to this tile; k of it is awaited, and the next one's sent behind it
+      copies_but<1>();
       __syncthreads();
-      for (int i = tid; i < kKeys * (HDP / 4); i += kThreads) {
-        const int j = i / (HDP / 4), c = (i % (HDP / 4)) * 4;
-        const T* src = row_of(j, false);
-        float x[4] = {0.f, 0.f, 0.f, 0.f};
-        if (src) load4(src, c, a.hd, wide, x);
-        *reinterpret_cast<float4*>(kv + j * kPitch + c) = make_float4(x[0], x[1], x[2], x[3]);
-        if (c == 0) there[j] = src != nullptr;
-      }
-      __syncthreads();
-      float s[2][4] = {};
-      const float* q0 = qs + 2 * ty * kPitch;
+      if (t + 1 < u.t1) request_tile(t + 1, false);
+      else copies_sent();
+      const ulonglong2 at_next = find_row(t + 2);
+      const T* kt = ks + (t & 1) * kKeys * kP;
+      uint64_t s2[4][kJ] = {};
+      const float* q0 = qs + 4 * ty * kQP;
 #pragma unroll 4
       for (int c = 0; c < HDP; c += 4) {
-        const float4 x0 = *reinterpret_cast<const float4*>(q0 + c), x1 = *reinterpret_cast<const float4*>(q0 + kPitch + c);
+        uint64_t x[4][2];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float4 y = *reinterpret_cast<const float4*>(kv + (tx + 16 * j) * kPitch + c);
-          s[0][j] = fmaf(x0.x, y.x, s[0][j]); s[0][j] = fmaf(x0.y, y.y, s[0][j]); s[0][j] = fmaf(x0.z, y.z, s[0][j]); s[0][j] = fmaf(x0.w, y.w, s[0][j]);
-          s[1][j] = fmaf(x1.x, y.x, s[1][j]); s[1][j] = fmaf(x1.y, y.y, s[1][j]); s[1][j] = fmaf(x1.z, y.z, s[1][j]); s[1][j] = fmaf(x1.w, y.w, s[1][j]);
+        for (int i = 0; i < 4; ++i) pairs(q0 + i * kQP + c, x[i][0], x[i][1]);
+#pragma unroll
+        for (int j = 0; j < kJ; ++j) {
+          uint64_t y0, y1;
+          pairs(kt + (tx + 16 * j) * kP + c, y0, y1);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s2[i][j] = fma2(x[i][1], y1, fma2(x[i][0], y0, s2[i][j]));
         }
       }
+      const ulonglong2* here = rows_at + (t & 1) * kKeys;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        bool sees[4];
+      for (int i = 0; i < 4; ++i) {
+        float s[kJ];
+        bool sees[kJ];
         float top = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < kJ; ++j) {
           const int key = key0 + tx + 16 * j;
-          sees[j] = node[i] >= 0 && there[tx + 16 * j];
+          float lo, hi;
+          upk2(s2[i][j], lo, hi);
+          s[j] = lo + hi;
+          sees[j] = node[i] >= 0 && here[tx + 16 * j].x != 0ull;
           if (nodes) sees[j] = sees[j] && ((a.mask[(size_t)(u.r.start + node[i]) * a.words + (key >> 5)] >> (key & 31)) & 1u);
           else sees[j] = sees[j] && key > after[i];
-          if (sees[j]) top = fmaxf(top, s[i][j]);
+          if (sees[j]) top = fmaxf(top, s[j]);
         }
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         const float now = fmaxf(m[i], top), base = now == -INFINITY ? 0.f : now, keep = exp2f(m[i] - base);
         float sum = 0.f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < kJ; ++j) {
           // an unseen key's weight is -0: nothing to the sums, and told from the +0 of a seen one whose score is far below
-          const float w = sees[j] ? exp2f(s[i][j] - base) : -0.f;
+          const float w = sees[j] ? exp2f(s[j] - base) : -0.f;
           sum += w;
-          ps[(2 * ty + i) * kPP + tx + 16 * j] = w;
+          ps[(4 * ty + i) * kPP + tx + 16 * j] = w;
         }
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         l[i] = l[i] * keep + sum;
         m[i] = now;
+        const uint64_t keep2 = pk2(keep, keep);
 #pragma unroll
-        for (int c = 0; c < HDP / 64; ++c)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[i][c][e] *= keep;
+        for (int c = 0; c < kC; ++c) {
+          acc[i][c][0] = mul2(acc[i][c][0], keep2);
+          acc[i][c][1] = mul2(acc[i][c][1], keep2);
+        }
       }
-      __syncthreads();
-      bool odd = false;                                          // an infinity or NaN among the values
-      for (int i = tid; i < kKeys * (HDP / 4); i += kThreads) {
-        const int j = i / (HDP / 4), c = (i % (HDP / 4)) * 4;
-        const T* src = row_of(j, true);
-        float x[4] = {0.f, 0.f, 0.f, 0.f};
-        if (src) load4(src, c, a.hd, wide, x);
+      copies_but<1>();                                           // v of this tile
+      const T* vt = vs + (t & 1) * kKeys * kP;
+      bool odd = false;                                          // an infinity or NaN among the values (each thread looks at those that it brought)
+      for (int i = tid; i < kKeys * kChunks; i += kThreads) {
+        const T* x = vt + (i / kChunks) * kP + (i % kChunks) * kE;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) odd |= !(fabsf(x[e]) <= 3.4028235e38f);
-        *reinterpret_cast<float4*>(kv + j * kPitch + c) = make_float4(x[0], x[1], x[2], x[3]);
+        for (int e = 0; e < kE; e += 4) {
+          float y[4];
+          ld4(x + e, y);
+          odd |= is_odd(y[0]) | is_odd(y[1]) | is_odd(y[2]) | is_odd(y[3]);
+        }
       }
-      const float* p0 = ps + 2 * ty * kPP;
-      if (!__syncthreads_or(odd)) {
-#pragma unroll 4
-        for (int j = 0; j < kKeys; ++j) {
-          const float w0 = p0[j], w1 = p0[kPP + j];
+      const bool any_odd = __syncthreads_or(odd);
+      if (t + 1 < u.t1) request_tile(t + 1, true);
+      else copies_sent();
+      note_row(t + 2, at_next);                                  // (this tile's rows have been read by all)
+      const float* p0 = ps + 4 * ty * kPP;
+      if (!any_odd) {
+#pragma unroll 2
+        for (int j = 0; j < kKeys; j += 4) {
+          float w[4][4];
 #pragma unroll
-          for (int c = 0; c < HDP / 64; ++c) {
-            const float4 y = *reinterpret_cast<const float4*>(kv + j * kPitch + 64 * c + 4 * tx);
-            acc[0][c][0] = fmaf(w0, y.x, acc[0][c][0]); acc[0][c][1] = fmaf(w0, y.y, acc[0][c][1]);
-            acc[0][c][2] = fmaf(w0, y.z, acc[0][c][2]); acc[0][c][3] = fmaf(w0, y.w, acc[0][c][3]);
-            acc[1][c][0] = fmaf(w1, y.x, acc[1][c][0]); acc[1][c][1] = fmaf(w1, y.y, acc[1][c][1]);
-            acc[1][c][2] = fmaf(w1, y.z, acc[1][c][2]); acc[1][c][3] = fmaf(w1, y.w, acc[1][c][3]);
-          }
+          for (int i = 0; i < 4; ++i) ld4(p0 + i * kPP + j, w[i]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int c = 0; c < kC; ++c) {
+              uint64_t y0, y1;
+              pairs(vt + (j + e) * kP + 64 * c + 4 * tx, y0, y1);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const uint64_t w2 = pk2(w[i][e], w[i][e]);
+                acc[i][c][0] = fma2(w2, y0, acc[i][c][0]);
+                acc[i][c][1] = fma2(w2, y1, acc[i][c][1]);
+              }
+            }
         }
       } else {
         // a value that is no number must not reach the rows that do not see it (0 times infinity)
         for (int j = 0; j < kKeys; ++j)
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
+          for (int i = 0; i < 4; ++i) {
             const float w = p0[i * kPP + j];
             if (__float_as_uint(w) == 0x80000000u) continue;
 #pragma unroll
-            for (int c = 0; c < HDP / 64; ++c)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) acc[i][c][e] = fmaf(w, kv[j * kPitch + 64 * c + 4 * tx + e], acc[i][c][e]);
+            for (int c = 0; c < kC; ++c) {
+              uint64_t y0, y1;
+              pairs(vt + j * kP + 64 * c + 4 * tx, y0, y1);
+              acc[i][c][0] = fma2(pk2(w, w), y0, acc[i][c][0]);
+              acc[i][c][1] = fma2(pk2(w, w), y1, acc[i][c][1]);
+            }
           }
       }
     }
     const bool begins = u.t0 == 0, ends = u.t1 == u.r.tiles;
-    if (begins && ends) {
+    const int slot = 2 * b + (begins ? 1 : 0), quads = (a.hd + 3) / 4;
+    float* o = a.partials + slot * partial_floats(kRows, a.hd);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        if (node[i] < 0) continue;
-        const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
-        T* out = (T*)a.out + (u.r.start + node[i]) * a.out_stride + (size_t)(u.kvh * a.group + (row0 + 2 * ty + i) % a.group) * a.hd;
+    for (int i = 0; i < 4; ++i) {
+      if (node[i] < 0) continue;
+      const int row = 4 * ty + i;
+      const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
+      T* out = (T*)a.out + (u.r.start + node[i]) * a.out_stride + (size_t)(u.kvh * a.group + (row0 + row) % a.group) * a.hd;
 #pragma unroll
-        for (int c = 0; c < HDP / 64; ++c)
+      for (int c = 0; c < kC; ++c) {
+        float v[4];
+        upk2(acc[i][c][0], v[0], v[1]);
+        upk2(acc[i][c][1], v[2], v[3]);
+        const int quad = 16 * c + tx;
+        if (begins && ends) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int col = 64 * c + 4 * tx + e;
-            if (col < a.hd) out[col] = from_f32<T>(acc[i][c][e] * inv);
-          }
-      }
-    } else {
-      const int slot = 2 * b + (begins ? 1 : 0);
-      float* o = a.partials + slot * partial_floats(kRows, a.hd);
-      const int quads = (a.hd + 3) / 4;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int row = 2 * ty + i;
-        if (row >= rows) continue;
-#pragma unroll
-        for (int c = 0; c < HDP / 64; ++c) {
-          const int quad = 16 * c + tx;
-          if (quad < quads) st4(o + ((size_t)quad * kRows + row) * 4, acc[i][c]);
-        }
-        if (tx == 0) {
-          o[(size_t)quads * 4 * kRows + row] = m[i];
-          o[(size_t)quads * 4 * kRows + kRows + row] = l[i];
+          for (int e = 0; e < 4; ++e)
+            if (4 * quad + e < a.hd) out[4 * quad + e] = from_f32<T>(v[e] * inv);
+        } else if (quad < quads) {
+          st4(o + ((size_t)quad * kRows + row) * 4, v);
         }
       }
-      if (begins && tid == 0) a.notes[b] = make_int4(u.s, u.kvh, row0, rows | (block_of(offs[a.n_seqs], u.last) << 8));
+      if (!(begins && ends) && tx == 0) {
+        o[(size_t)quads * 4 * kRows + row] = m[i];
+        o[(size_t)quads * 4 * kRows + kRows + row] = l[i];
+      }
     }
+    if (begins && !ends && tid == 0) a.notes[b] = make_int4(u.s, u.kvh, row0, rows | (block_of(offs[a.n_seqs], u.last) << 8));
     p = u.next;
   }
 }
 
 template <typename T, int HDP>
 static int launch(const Args& a, int blocks, bool wide, cudaStream_t st) {
-  const size_t smem = sizeof(float) * ((size_t)(kRows + kKeys) * (HDP + 4) + kRows * (kKeys + 4) + kKeys) + work_bytes(a.n_seqs);
   static bool raised[64] = {};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return (int)e;
   if (dev < 64 && !raised[dev]) {
-    e = cudaFuncSetAttribute(attention_tree_kernel<T, HDP>, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+    e = cudaFuncSetAttribute(attention_tree_kernel<T, HDP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes<T, HDP>(kMaxSeqs));
     if (e != cudaSuccess) return (int)e;
     raised[dev] = true;
   }
-  int rc = launch_pdl(attention_tree_kernel<T, HDP>, dim3(blocks), dim3(kThreads), smem, st, a, wide);
+  int rc = launch_pdl(attention_tree_kernel<T, HDP>, dim3(blocks), dim3(kThreads), smem_bytes<T, HDP>(a.n_seqs), st, a, wide);
   if (rc) return rc;
   const bool wide_out = ((unsigned long long)a.out | (unsigned long long)(a.out_stride * sizeof(T)) | (unsigned long long)(a.hd * sizeof(T))) % 16 == 0;
   return launch_pdl(join_kernel<T, kRows, 1, HDP>, dim3(blocks, 1), dim3(256), 0, st, a, wide_out);
@@ -241,9 +326,9 @@ static int launch(const Args& a, int blocks, bool wide, cudaStream_t st) {
 }  // namespace lmsf
 
 // Blocks of a launch, and the bytes of workspace that go with them.
-LMSF_API int lmsf_attention_tree_blocks(int sms) { return 2 * sms; }
+LMSF_API int lmsf_attention_tree_blocks(int sms, int hd) { return hd <= 128 ? 2 * sms : sms; }
 LMSF_API long long lmsf_attention_tree_workspace(int sms, int hd) {
-  const long long blocks = lmsf_attention_tree_blocks(sms);
+  const long long blocks = lmsf_attention_tree_blocks(sms, hd);
   return blocks * (2 * (long long)lmsf::tree::partial_floats(lmsf::tree::kRows, hd) * 4 + 16);
 }
 
@@ -264,18 +349,19 @@ LMSF_API int lmsf_attention_tree(const void* q, long long q_stride, const void* 
   if (window > 0 && !positions) LMSF_REFUSE("attention_tree: a window needs the nodes' positions");
   if (dtype != LMSF_F32 && dtype != LMSF_BF16) LMSF_REFUSE("attention_tree: unknown dtype code %d", dtype);
   const long long group = n_q_heads / n_kv_heads;
-  const long long tiles = ((long long)max_blocks * block_size + kKeys - 1) / kKeys + (32ll * words + kKeys - 1) / kKeys + 1;
+  const int keys = hd <= 64 ? kTile<64> : kTile<128>;
+  const long long tiles = ((long long)max_blocks * block_size + keys - 1) / keys + (32ll * words + keys - 1) / keys + 1;
   if (((n_rows * group + kRows - 1) / kRows + n_seqs) * n_kv_heads * tiles > 0x7fffffffll)
     LMSF_REFUSE("attention_tree: %d rows of %d heads over %d pages are too much work for one launch", n_rows, n_q_heads, max_blocks);
   Args a{q, q_stride, k, k_stride, v, v_stride, out, out_stride, cache, page_stride, v_off, pages, block_table, max_blocks, block_size,
          cu_q, prefix_len, mask, words, positions, window, scale, n_seqs, n_rows, n_q_heads, n_kv_heads, (int)group, hd, nullptr, nullptr};
-  const int blocks = lmsf_attention_tree_blocks(sms);
+  const int blocks = lmsf_attention_tree_blocks(sms, hd);
   a.notes = (int4*)workspace;
   a.partials = (float*)(a.notes + blocks);
   const int size = dtype == LMSF_F32 ? 4 : 2;
   const unsigned long long bits = (unsigned long long)q | (unsigned long long)k | (unsigned long long)v | (unsigned long long)cache |
                                   (unsigned long long)(size * (q_stride | k_stride | v_stride | page_stride | v_off | hd));
-  const bool wide = bits % (4 * size) == 0;
+  const bool wide = bits % 16 == 0;             // rows of 16-byte words
   cudaStream_t st = (cudaStream_t)stream;
   if (dtype == LMSF_F32) {
     if (hd <= 64) return launch<float, 64>(a, blocks, wide, st);
