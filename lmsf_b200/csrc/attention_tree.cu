@@ -130,16 +130,30 @@ __global__ void __launch_bounds__(kThreads) attention_tree_kernel(Args a, bool w
     __syncthreads();
     request_tile(u.t0, false);
     request_tile(u.t0, true);
-    for (int i = tid; i < kRows * (HDP / 4); i += kThreads) {
-      const int row = i / (HDP / 4), c = (i % (HDP / 4)) * 4, r = row0 + row;
-      float x[4] = {0.f, 0.f, 0.f, 0.f};
-      if (row < rows) {
-        const T* src = q + (u.r.start + r / a.group) * a.q_stride + (size_t)(u.kvh * a.group + r % a.group) * a.hd;
+    {
+      constexpr int kQuads = HDP / 4, kEach = kRows * kQuads / kThreads;     // groups of four values: of a row, of a thread
+      float x[kEach < 8 ? kEach : 8][4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (c + e < a.hd) x[e] = to_f32(src[c + e]) * (a.scale * 1.4426950408889634f);
+      for (int k0 = 0; k0 < kEach; k0 += 8) {
+#pragma unroll
+        for (int k = 0; k < 8 && k0 + k < kEach; ++k) {          // all requested before the first is stored
+          const int i = tid + (k0 + k) * kThreads, row = i / kQuads, c = (i % kQuads) * 4, r = row0 + row, n = r / a.group;
+          const T* src = q + (u.r.start + n) * a.q_stride + (size_t)(u.kvh * a.group + (r - n * a.group)) * a.hd + c;
+          if (wide && row < rows && c < a.hd) {
+            ld4(src, x[k]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[k][e] = row < rows && c + e < a.hd ? to_f32(src[e]) : 0.f;
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 8 && k0 + k < kEach; ++k) {
+          const int i = tid + (k0 + k) * kThreads;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[k][e] *= a.scale * 1.4426950408889634f;
+          st4(qs + (i / kQuads) * kQP + (i % kQuads) * 4, x[k]);
+        }
       }
-      st4(qs + row * kQP + c, x);
     }
     int node[4], after[4];                                       // of this thread's rows: node, and the cached key behind which it sees
     float m[4], l[4];
@@ -163,61 +177,87 @@ __global__ void __launch_bounds__(kThreads) attention_tree_kernel(Args a, bool w
       if (t + 1 < u.t1) request_tile(t + 1, false);
       else copies_sent();
       const ulonglong2 at_next = find_row(t + 2);
+      uint32_t words[4][kKeys / 32];                             // what the rows see of drafted tokens
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int w = 0; w < kKeys / 32; ++w)
+          words[i][w] = nodes && node[i] >= 0 && key0 / 32 + w < a.words ? a.mask[(size_t)(u.r.start + node[i]) * a.words + key0 / 32 + w] : 0xffffffffu;
       const T* kt = ks + (t & 1) * kKeys * kP;
       uint64_t s2[4][kJ] = {};
       const float* q0 = qs + 4 * ty * kQP;
-#pragma unroll 4
-      for (int c = 0; c < HDP; c += 4) {
-        uint64_t x[4][2];
+      // (the next four columns are asked for before these are multiplied: a scheduler has one or two warps of this kernel)
+      uint64_t x[2][4][2], y[2][kJ][2];
+      auto columns = [&](int g, int c) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) pairs(q0 + i * kQP + c, x[i][0], x[i][1]);
+        for (int i = 0; i < 4; ++i) pairs(q0 + i * kQP + c, x[g][i][0], x[g][i][1]);
 #pragma unroll
-        for (int j = 0; j < kJ; ++j) {
-          uint64_t y0, y1;
-          pairs(kt + (tx + 16 * j) * kP + c, y0, y1);
+        for (int j = 0; j < kJ; ++j) pairs(kt + (tx + 16 * j) * kP + c, y[g][j][0], y[g][j][1]);
+      };
+      columns(0, 0);
+#pragma unroll 2
+      for (int c = 0; c < HDP; c += 8) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s2[i][j] = fma2(x[i][1], y1, fma2(x[i][0], y0, s2[i][j]));
+        for (int g = 0; g < 2; ++g) {
+          if (g == 0) columns(1, c + 4);
+          else columns(0, c + 8 < HDP ? c + 8 : 0);
+#pragma unroll
+          for (int j = 0; j < kJ; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s2[i][j] = fma2(x[g][i][0], y[g][j][0], s2[i][j]);
+#pragma unroll
+          for (int j = 0; j < kJ; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s2[i][j] = fma2(x[g][i][1], y[g][j][1], s2[i][j]);
         }
       }
       const ulonglong2* here = rows_at + (t & 1) * kKeys;
+      // the four rows side by side: their sixteen threads' maxima and sums pass through the warp in four steps
+      float s[4][kJ], top[4], sum[4], keep[4];
+      bool sees[4][kJ];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        float s[kJ];
-        bool sees[kJ];
-        float top = -INFINITY;
+        top[i] = -INFINITY;
 #pragma unroll
         for (int j = 0; j < kJ; ++j) {
-          const int key = key0 + tx + 16 * j;
+          const int at = tx + 16 * j;
           float lo, hi;
           upk2(s2[i][j], lo, hi);
-          s[j] = lo + hi;
-          sees[j] = node[i] >= 0 && here[tx + 16 * j].x != 0ull;
-          if (nodes) sees[j] = sees[j] && ((a.mask[(size_t)(u.r.start + node[i]) * a.words + (key >> 5)] >> (key & 31)) & 1u);
-          else sees[j] = sees[j] && key > after[i];
-          if (sees[j]) top = fmaxf(top, s[j]);
+          s[i][j] = lo + hi;
+          sees[i][j] = node[i] >= 0 && here[at].x != 0ull && ((words[i][j / 2] >> (at & 31)) & 1u) && (nodes || key0 + at > after[i]);
+          if (sees[i][j]) top[i] = fmaxf(top[i], s[i][j]);
         }
+      }
 #pragma unroll
-        for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const float now = fmaxf(m[i], top), base = now == -INFINITY ? 0.f : now, keep = exp2f(m[i] - base);
-        float sum = 0.f;
+      for (int o = 8; o > 0; o >>= 1)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float now = fmaxf(m[i], top[i]), base = now == -INFINITY ? 0.f : now;
+        keep[i] = exp2f(m[i] - base);
+        m[i] = now;
+        sum[i] = 0.f;
 #pragma unroll
         for (int j = 0; j < kJ; ++j) {
           // an unseen key's weight is -0: nothing to the sums, and told from the +0 of a seen one whose score is far below
-          const float w = sees[j] ? exp2f(s[j] - base) : -0.f;
-          sum += w;
+          const float w = sees[i][j] ? exp2f(s[i][j] - base) : -0.f;
+          sum[i] += w;
           ps[(4 * ty + i) * kPP + tx + 16 * j] = w;
         }
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        l[i] = l[i] * keep + sum;
-        m[i] = now;
-        const uint64_t keep2 = pk2(keep, keep);
+        const uint64_t keep2 = pk2(keep[i], keep[i]);
 #pragma unroll
         for (int c = 0; c < kC; ++c) {
           acc[i][c][0] = mul2(acc[i][c][0], keep2);
           acc[i][c][1] = mul2(acc[i][c][1], keep2);
         }
       }
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], o);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) l[i] = l[i] * keep[i] + sum[i];
       copies_but<1>();                                           // v of this tile
       const T* vt = vs + (t & 1) * kKeys * kP;
       bool odd = false;                                          // an infinity or NaN among the values (each thread looks at those that it brought)
@@ -236,24 +276,38 @@ __global__ void __launch_bounds__(kThreads) attention_tree_kernel(Args a, bool w
       note_row(t + 2, at_next);                                  // (this tile's rows have been read by all)
       const float* p0 = ps + 4 * ty * kPP;
       if (!any_odd) {
+        float w[2][4][2];
+        uint64_t y[2][2][kC][2];
+        auto two_keys = [&](int g, int j) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 f = *reinterpret_cast<const float2*>(p0 + i * kPP + j);
+            w[g][i][0] = f.x;
+            w[g][i][1] = f.y;
+          }
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int c = 0; c < kC; ++c) pairs(vt + (j + e) * kP + 64 * c + 4 * tx, y[g][e][c][0], y[g][e][c][1]);
+        };
+        two_keys(0, 0);
 #pragma unroll 2
         for (int j = 0; j < kKeys; j += 4) {
-          float w[4][4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) ld4(p0 + i * kPP + j, w[i]);
+          for (int g = 0; g < 2; ++g) {
+            if (g == 0) two_keys(1, j + 2);
+            else two_keys(0, j + 4 < kKeys ? j + 4 : 0);
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
+            for (int e = 0; e < 2; ++e)
 #pragma unroll
-            for (int c = 0; c < kC; ++c) {
-              uint64_t y0, y1;
-              pairs(vt + (j + e) * kP + 64 * c + 4 * tx, y0, y1);
+              for (int c = 0; c < kC; ++c)
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const uint64_t w2 = pk2(w[i][e], w[i][e]);
-                acc[i][c][0] = fma2(w2, y0, acc[i][c][0]);
-                acc[i][c][1] = fma2(w2, y1, acc[i][c][1]);
-              }
-            }
+                for (int i = 0; i < 4; ++i) {
+                  const uint64_t w2 = pk2(w[g][i][e], w[g][i][e]);
+                  acc[i][c][0] = fma2(w2, y[g][e][c][0], acc[i][c][0]);
+                  acc[i][c][1] = fma2(w2, y[g][e][c][1], acc[i][c][1]);
+                }
+          }
         }
       } else {
         // a value that is no number must not reach the rows that do not see it (0 times infinity)

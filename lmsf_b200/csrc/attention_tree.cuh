@@ -69,6 +69,29 @@ __host__ __device__ __forceinline__ size_t work_bytes(int n_seqs) { return (size
 template <int kKeys>
 __device__ __forceinline__ void add_up_work(const Args& a, int rows, Lengths* all, int* offs, int* scratch) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = blockDim.x >> 5;
+  if (a.n_seqs <= 32) {                          // one warp's work: no second pass through shared memory
+    if (warp == 0) {
+      Lengths l = {};
+      int w = 0;
+      if (lane < a.n_seqs) {
+        l = lengths(a, lane, rows);
+        w = request<kKeys>(a, l).tiles * l.items * a.n_kv;
+      }
+      int x = w;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      if (lane < a.n_seqs) {
+        all[lane] = l;
+        offs[lane] = x - w;
+      }
+      if (lane == 31) offs[a.n_seqs] = x;
+    }
+    __syncthreads();
+    return;
+  }
   const int per = (a.n_seqs + blockDim.x - 1) / blockDim.x;
   const int s0 = min(tid * per, a.n_seqs), s1 = min(s0 + per, a.n_seqs);
   int sum = 0;
