@@ -8,6 +8,7 @@ namespace lmsf {
 namespace tree {
 
 constexpr int kRows = 32, kThreads = 128;
+constexpr int kExtra = 0;                      // places of a unit beside its tiles (1: 56 us where 0 takes 50, as the shares no longer end with units)
 // Keys of a tile: two tiles of keys and two of values lie in shared memory, for head sizes up to 128 twice per SM.
 template <int HDP> constexpr int kTile = HDP <= 64 ? 64 : 32;
 template <typename T, int HDP> constexpr int kPitch = HDP + 16 / (int)sizeof(T);         // of a row in shared memory: 16 bytes more, for the banks
@@ -71,15 +72,15 @@ __global__ void __launch_bounds__(kThreads) attention_tree_kernel(Args a, bool w
   pdl_launch_dependents();
   pdl_wait();
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-  add_up_work<kKeys>(a, kRows, lens, offs, scratch);
+  add_up_work<kKeys, 1, kExtra>(a, kRows, lens, offs, scratch);
   int begin, end;
-  share_of_block(offs[a.n_seqs], begin, end);
+  share_of_block<kExtra>(offs[a.n_seqs], begin, end);
   const int b = blockIdx.x;
   if (tid == 0) a.notes[b] = make_int4(-1, 0, 0, 0);
   __syncthreads();
   const T* q = (const T*)a.q;
   for (int p = begin; p < end;) {
-    const Piece u = piece_at<kKeys, 1>(a, lens, offs, p, end);
+    const Piece u = piece_at<kKeys, 1, kExtra>(a, lens, offs, p, end);
     const int row0 = u.item * kRows, rows = min(kRows, u.r.n * a.group - row0);
     const int* table = a.block_table + (size_t)u.s * a.max_blocks;
     // thread j < kKeys: where row j of tile t lies (asked for an iteration before its copies are, which every thread makes some of)
@@ -354,7 +355,7 @@ __global__ void __launch_bounds__(kThreads) attention_tree_kernel(Args a, bool w
         o[(size_t)quads * 4 * kRows + kRows + row] = l[i];
       }
     }
-    if (begins && !ends && tid == 0) a.notes[b] = make_int4(u.s, u.kvh, row0, rows | (block_of(offs[a.n_seqs], u.last) << 8));
+    if (begins && !ends && tid == 0) a.notes[b] = make_int4(u.s, u.kvh, row0, rows | (block_of<kExtra>(offs[a.n_seqs], u.last) << 8));
     p = u.next;
   }
 }
@@ -404,7 +405,7 @@ LMSF_API int lmsf_attention_tree(const void* q, long long q_stride, const void* 
   if (dtype != LMSF_F32 && dtype != LMSF_BF16) LMSF_REFUSE("attention_tree: unknown dtype code %d", dtype);
   const long long group = n_q_heads / n_kv_heads;
   const int keys = hd <= 64 ? kTile<64> : kTile<128>;
-  const long long tiles = ((long long)max_blocks * block_size + keys - 1) / keys + (32ll * words + keys - 1) / keys + 1;
+  const long long tiles = ((long long)max_blocks * block_size + keys - 1) / keys + (32ll * words + keys - 1) / keys + 1 + kExtra;
   if (((n_rows * group + kRows - 1) / kRows + n_seqs) * n_kv_heads * tiles > 0x7fffffffll)
     LMSF_REFUSE("attention_tree: %d rows of %d heads over %d pages are too much work for one launch", n_rows, n_q_heads, max_blocks);
   Args a{q, q_stride, k, k_stride, v, v_stride, out, out_stride, cache, page_stride, v_off, pages, block_table, max_blocks, block_size,

@@ -6,8 +6,8 @@
 //
 // The work is cut as follows.  A unit is (request, kv head, item of up to kRows rows); it has the request's tiles of kKeys keys: its
 // cached keys first, then the nodes.  All units' tiles in a row, requests in order, are shared out evenly over the blocks, whatever the
-// lengths are, a tile of a unit of two items counted twice; no plan is made on the host, so a captured launch serves any lengths.  A unit that lies in one block's range is finished there.  Of a unit that is cut every block leaves a
-// partial (unnormalised output, running maximum, sum; float32) in the workspace: at most two for a block (and item), one for the unit
+// lengths are, a tile of a unit of two items counted twice and every unit as kExtra tiles more, for what it costs beside them; no
+// plan is made on the host, so a captured launch serves any lengths.  A unit that lies in one block's range is finished there.  Of a unit that is cut every block leaves a partial (unnormalised output, running maximum, sum; float32) in the workspace: at most two for a block (and item), one for the unit
 // that it begins with and one for the unit that it ends with.  A second kernel adds them up in the order of the blocks; both
 // depend only on lengths and G, so the result is the same in every run.
 #pragma once
@@ -63,10 +63,14 @@ __device__ __forceinline__ Request request(const Args& a, const Lengths& l) {
   return r;
 }
 
-// What a block keeps of the step in shared memory: all[s], and offs[s] = work before request s (a tile for an item is one), for 0 <= s <= n_seqs.
+// What a block keeps of the step in shared memory: all[s], and offs[s] = work before request s, in places, for 0 <= s <= n_seqs.
 __host__ __device__ __forceinline__ size_t work_bytes(int n_seqs) { return (size_t)n_seqs * sizeof(Lengths) + (size_t)(n_seqs + 1) * sizeof(int); }
+template <int kKeys, int kItems, int kExtra>
+__device__ __forceinline__ int work_of(const Request& r, int n_kv) {
+  return n_kv * (r.tiles * r.items + kExtra * ((r.items + kItems - 1) / kItems));
+}
 // By all threads of the block (a multiple of 32, at most 1024).
-template <int kKeys>
+template <int kKeys, int kItems, int kExtra>
 __device__ __forceinline__ void add_up_work(const Args& a, int rows, Lengths* all, int* offs, int* scratch) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = blockDim.x >> 5;
   if (a.n_seqs <= 32) {                          // one warp's work: no second pass through shared memory
@@ -75,7 +79,7 @@ __device__ __forceinline__ void add_up_work(const Args& a, int rows, Lengths* al
       int w = 0;
       if (lane < a.n_seqs) {
         l = lengths(a, lane, rows);
-        w = request<kKeys>(a, l).tiles * l.items * a.n_kv;
+        w = work_of<kKeys, kItems, kExtra>(request<kKeys>(a, l), a.n_kv);
       }
       int x = w;
 #pragma unroll
@@ -99,7 +103,7 @@ __device__ __forceinline__ void add_up_work(const Args& a, int rows, Lengths* al
     const Lengths l = lengths(a, s, rows);
     all[s] = l;
     offs[s] = sum;
-    sum += request<kKeys>(a, l).tiles * l.items * a.n_kv;
+    sum += work_of<kKeys, kItems, kExtra>(request<kKeys>(a, l), a.n_kv);
   }
   int x = sum;
 #pragma unroll
@@ -120,12 +124,15 @@ __device__ __forceinline__ void add_up_work(const Args& a, int rows, Lengths* al
   __syncthreads();
 }
 
-// Blocks that take part in `work`: two places each at the least (a short unit that is cut costs more than its second tile; and a share of one place
-// might have no tile), none with an empty share between the pieces of a unit.
-__device__ __forceinline__ int blocks_for(int work) { return min((int)gridDim.x, max(work / 2, 1)); }
+// Blocks that take part in `work`: kExtra + 2 places each at the least, so that every share has a tile (it may begin with the last place of
+// a unit of two items, whose tile belongs to the block before, and go on with the kExtra places of the next unit), and no share that lies
+// inside a unit is without one.
+template <int kExtra>
+__device__ __forceinline__ int blocks_for(int work) { return min((int)gridDim.x, max(work / (kExtra + 2), 1)); }
 // What this block takes of it: every block as much as every other, the first `work % blocks` one more.
+template <int kExtra>
 __device__ __forceinline__ void share_of_block(int work, int& begin, int& end) {
-  const int b = blockIdx.x, blocks = blocks_for(work);
+  const int b = blockIdx.x, blocks = blocks_for<kExtra>(work);
   begin = end = 0;
   if (b >= blocks) return;
   const int each = work / blocks, more = work - each * blocks;
@@ -133,8 +140,9 @@ __device__ __forceinline__ void share_of_block(int work, int& begin, int& end) {
   end = begin + each + (b < more ? 1 : 0);
 }
 // The block whose share place p lies in.
+template <int kExtra>
 __device__ __forceinline__ int block_of(int work, int p) {
-  const int blocks = blocks_for(work), each = work / blocks, more = work - each * blocks, edge = more * (each + 1);
+  const int blocks = blocks_for<kExtra>(work), each = work / blocks, more = work - each * blocks, edge = more * (each + 1);
   return p < edge ? p / (each + 1) : more + (p - edge) / each;
 }
 
@@ -149,24 +157,28 @@ __device__ __forceinline__ int request_at(const int* offs, int n_seqs, int p) {
   return lo;
 }
 
-// A block's share of one unit of up to kItems items: tiles [t0, t1) of the unit's.  Tile t of a unit of two items has the places 2 t and
-// 2 t + 1 and belongs to the block that has the first of them.  next: the place behind the unit, or the block's end; last: the place that the
-// unit's last tile is found by.  A share that begins with a unit's last place has no tile of it: t0 = t1.
+// A block's share of one unit of up to kItems items: tiles [t0, t1) of the unit's.  The unit has kExtra places and then those of its tiles: tile t of
+// a unit of two items has two and belongs to the block that has the first of them.  next: the place behind the unit, or the block's
+// end, also where the share ends before the first tile of the unit behind; last: the place that the unit's last tile is found by.  A share
+// that begins with a unit's last place has no tile of it: t0 = t1.
 struct Piece { int s, kvh, item, t0, t1, next, last; bool two; Request r; };
-template <int kKeys, int kItems>
+template <int kKeys, int kItems, int kExtra>
 __device__ __forceinline__ Piece piece_at(const Args& a, const Lengths* all, const int* offs, int p, int end) {
   Piece x;
   x.s = request_at(offs, a.n_seqs, p);
   x.r = request<kKeys>(a, all[x.s]);
-  const int rem = p - offs[x.s], per_head = x.r.tiles * x.r.items;
+  const int rem = p - offs[x.s], whole = kItems * x.r.tiles + kExtra, units = (x.r.items + kItems - 1) / kItems;
+  const int per_head = x.r.tiles * x.r.items + kExtra * units;
   x.kvh = rem / per_head;
-  const int in_head = rem - x.kvh * per_head, unit = in_head / (kItems * x.r.tiles);
+  const int in_head = rem - x.kvh * per_head, unit = in_head / whole;
   x.item = unit * kItems;                                        // the unit's first item: its neighbours read the same keys
   x.two = kItems == 2 && x.item + 1 < x.r.items;
-  const int off = in_head - unit * kItems * x.r.tiles, size = (x.two ? 2 : 1) * x.r.tiles, off_end = min(size, off + (end - p));
-  x.t0 = x.two ? (off + 1) / 2 : off;
-  x.t1 = x.two ? (off_end + 1) / 2 : off_end;
+  const int off = in_head - unit * whole, size = (x.two ? 2 : 1) * x.r.tiles + kExtra, off_end = min(size, off + (end - p));
+  const int from = max(off - kExtra, 0), to = max(off_end - kExtra, 0);
+  x.t0 = x.two ? (from + 1) / 2 : from;
+  x.t1 = x.two ? (to + 1) / 2 : to;
   x.next = p + (off_end - off);
+  if (end - x.next <= kExtra) x.next = end;                      // no tile of the unit behind
   x.last = p - off + size - (x.two ? 2 : 1);
   return x;
 }

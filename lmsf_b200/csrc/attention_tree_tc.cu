@@ -46,6 +46,9 @@ constexpr int kOffK = 2 * kTileBytes, kOffV = kOffK + kStages * kTileBytes, kOff
 constexpr uint32_t kTmemCols = 512, kOCol = 256;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescale = 8.0f;               // the output is rescaled when the maximum grew by more than this (log2 units)
+// What a unit costs beside its tiles, in places of the sharing: the first tile's way from memory, the queries, the end.  27 requests of 1..64 nodes behind
+// 130..2,300 keys take 52 us with 0, 46 with 1, 43 with 2, 42 with 3 and 4; a request of 8 behind 1,000 18.5 with 2, 21 with 3, 23 with 4.
+constexpr int kExtra = 2;
 constexpr int kThreadsTotal = 384, kHalf = 128;
 constexpr int kRegsSoftmax = 216, kRegsOther = 72;
 constexpr int kRing = 16;                      // notes of tiles and of pieces that warps leave one another
@@ -203,7 +206,7 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
   }
   pdl_wait();
   const int rows_item = ta.nodes_per_item * a.group;
-  add_up_work<BN>(a, rows_item, lens, offs, scratch);
+  add_up_work<BN, 2, kExtra>(a, rows_item, lens, offs, scratch);
   if (tid < 2) a.notes[2 * blockIdx.x + tid] = make_int4(-1, 0, 0, 0);
   tc_fence_before();
   __syncthreads();
@@ -211,7 +214,7 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
   const uint32_t tmem = tmem_base_mem;
   int begin, end;
   const int work = offs[a.n_seqs];
-  share_of_block(work, begin, end);
+  share_of_block<kExtra>(work, begin, end);
   // the note of the block's i-th piece
   auto note_of = [&](int i, bool& ok) -> NotePtr {
     if (ok) ok = mbar_wait_f(noted(i), (uint32_t)((i / kRing) & 1), failed);
@@ -261,14 +264,14 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
       bool ok = true;
       auto leave_note = [&](int i, int p) {
         if (p >= end) return;
-        Piece u = piece_at<BN, 2>(a, lens, offs, p, end);
-        if (u.t0 == u.t1) u = piece_at<BN, 2>(a, lens, offs, u.next, end);       // (the block's first place was a unit's last)
+        Piece u = piece_at<BN, 2, kExtra>(a, lens, offs, p, end);
+        if (u.t0 == u.t1) u = piece_at<BN, 2, kExtra>(a, lens, offs, u.next, end);       // (the block's first place was a unit's last)
         if (lane == 0) {
           volatile PieceNote* n = &notes[i % kRing];
           n->s = u.s; n->kvh = u.kvh; n->item = u.item; n->t0 = u.t0; n->nt = u.t1 - u.t0; n->start = u.r.start; n->n = u.r.n; n->nk = u.r.nk;
           n->prefix = u.r.prefix; n->lo = u.r.lo; n->first = u.r.first; n->n_pre = u.r.n_pre; n->tiles = u.r.tiles;
           n->two = u.two;
-          n->last = u.t0 == 0 && u.t1 < u.r.tiles ? block_of(work, u.last) : 0;
+          n->last = u.t0 == 0 && u.t1 < u.r.tiles ? block_of<kExtra>(work, u.last) : 0;
           n->next = u.next;
           mbar_arrive(noted(i));
         }
@@ -771,7 +774,7 @@ LMSF_API int lmsf_attention_tree_tc(const void* q, long long q_stride, const voi
   if (((unsigned long long)q | (unsigned long long)k | (unsigned long long)v | (unsigned long long)cache) % 16 ||
       (q_stride | k_stride | v_stride | page_stride) % 8)
     LMSF_REFUSE("attention_tree: q, k, v and the cache need 16-byte aligned rows");
-  const long long tiles = ((long long)max_blocks * block_size + BN - 1) / BN + (32ll * words + BN - 1) / BN + 1;
+  const long long tiles = ((long long)max_blocks * block_size + BN - 1) / BN + (32ll * words + BN - 1) / BN + 1 + kExtra;
   TcArgs ta;
   ta.nodes_per_item = BM / group;
   const int rows_item = ta.nodes_per_item * group;
