@@ -124,11 +124,12 @@ struct __align__(16) PieceNote { int s, kvh, item, t0, nt, start, n, nk, prefix,
 typedef const volatile PieceNote* NotePtr;
 // Rows [lo, hi) of a tile are seen by some row of the piece's request; none of the others is multiplied, but for those that share a step
 // of 16 with them.
-__device__ __forceinline__ void rows_seen(NotePtr u, int t, int& key0, int& lo, int& hi) {
-  const bool nodes = t >= u->n_pre;
-  key0 = nodes ? (t - u->n_pre) * BN : (u->first + t) * BN;
-  lo = nodes ? 0 : max(u->lo - key0, 0);
-  hi = min((nodes ? u->nk : u->prefix) - key0, BN);
+template <typename Note>
+__device__ __forceinline__ void rows_seen(const Note& u, int t, int& key0, int& lo, int& hi) {
+  const bool nodes = t >= u.n_pre;
+  key0 = nodes ? (t - u.n_pre) * BN : (u.first + t) * BN;
+  lo = nodes ? 0 : max(u.lo - key0, 0);
+  hi = min((nodes ? u.nk : u.prefix) - key0, BN);
 }
 // What the warps need to know of a tile: boxes whose page is not there, which steps of 16 keys somebody sees (from, to), and whether every
 // row sees every key.
@@ -136,8 +137,9 @@ constexpr uint32_t kAllSeen = 0x80000000u;
 __device__ __forceinline__ int from16(uint32_t note) { return (note >> 16) & 15; }
 __device__ __forceinline__ int to16(uint32_t note) { return (note >> 20) & 15; }
 // Seen by some row, but perhaps not by every one: drafted tokens, and cached ones at the edge of a window.
-__device__ __forceinline__ bool seen_by_some(const Args& a, NotePtr u, int t, int key0) {
-  return t >= u->n_pre || (a.window > 0 && key0 <= u->prefix + u->n - 1 - a.window);
+template <typename Note>
+__device__ __forceinline__ bool seen_by_some(const Args& a, const Note& u, int t, int key0) {
+  return t >= u.n_pre || (a.window > 0 && key0 <= u.prefix + u.n - 1 - a.window);
 }
 
 __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(const TcArgs ta, const __grid_constant__ CUtensorMap q_map,
@@ -215,10 +217,14 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
   int begin, end;
   const int work = offs[a.n_seqs];
   share_of_block<kExtra>(work, begin, end);
-  // the note of the block's i-th piece
+  // the note of the block's i-th piece; for the warps that bring tiles a copy of it
   auto note_of = [&](int i, bool& ok) -> NotePtr {
     if (ok) ok = mbar_wait_f(noted(i), (uint32_t)((i / kRing) & 1), failed);
     return &notes[i % kRing];
+  };
+  auto copy_of = [&](int i, bool& ok) {
+    if (ok) ok = mbar_wait_f(noted(i), (uint32_t)((i / kRing) & 1), failed);
+    return notes[i % kRing];
   };
 
   if (warp >= 8) {
@@ -226,18 +232,18 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
     // The tiles of k or v of one piece after the other, by a whole warp.  Lane i brings box i of a tile of cached keys (a page, or 128 keys of
     // one), or 32 drafted tokens; the page of the tile behind is requested before this one's copies and looked at after them.
     const int n_box = BN / ta.rows_box;
-    auto entry = [&](NotePtr u, int t) {                         // what the block table says of this lane's box of tile t
-      const int key = (u->first + t) * BN + lane * ta.rows_box;
-      return t < u->n_pre && lane < n_box && key < u->prefix ? a.block_table[(size_t)u->s * a.max_blocks + (key >> ta.block_shift)] : -1;
+    auto entry = [&](const auto& u, int t) {                         // what the block table says of this lane's box of tile t
+      const int key = (u.first + t) * BN + lane * ta.rows_box;
+      return t < u.n_pre && lane < n_box && key < u.prefix ? a.block_table[(size_t)u.s * a.max_blocks + (key >> ta.block_shift)] : -1;
     };
     // The tile's note goes out with it: the barrier's arrival is behind it.
-    auto bring = [&](NotePtr u, int t, int page, bool is_v, int g) {
+    auto bring = [&](const PieceNote& u, int t, int page, bool is_v, int g) {
       const uint32_t bar = is_v ? v_full(g % kStages) : k_full(g % kStages), dst = (is_v ? sV : sK) + (g % kStages) * kTileBytes;
-      const bool nodes = t >= u->n_pre;
+      const bool nodes = t >= u.n_pre;
       int key0, lo, hi;
       rows_seen(u, t, key0, lo, hi);
       const int key = key0 + lane * ta.rows_box;
-      const bool seen = !nodes && lane < n_box && key < u->prefix && key + ta.rows_box > u->lo, there = seen && page >= 0 && page < a.pages;
+      const bool seen = !nodes && lane < n_box && key < u.prefix && key + ta.rows_box > u.lo, there = seen && page >= 0 && page < a.pages;
       const uint32_t here = __ballot_sync(0xffffffffu, there), missing = __ballot_sync(0xffffffffu, seen && !there);
       const int boxes = (hi + 31) / 32;                          // of drafted tokens
       if (lane == 0) {
@@ -250,59 +256,69 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
         if (lane < boxes) {
 #pragma unroll
           for (int hb = 0; hb < kHB; ++hb)
-            tma_load_box_3d(dst + hb * (BN * 128) + lane * (32 * 128), is_v ? &v_map : &k_map, hb * 64, u->kvh, u->start + key0 + lane * 32, bar);
+            tma_load_box_3d(dst + hb * (BN * 128) + lane * (32 * 128), is_v ? &v_map : &k_map, hb * 64, u.kvh, u.start + key0 + lane * 32, bar);
         }
       } else if (there) {
 #pragma unroll
         for (int hb = 0; hb < kHB; ++hb)
-          tma_load_box(dst + hb * (BN * 128) + lane * ta.rows_box * 128, &cache_map, hb * 64, key & (a.block_size - 1), (is_v ? a.n_kv : 0) + u->kvh, page, bar);
+          tma_load_box(dst + hb * (BN * 128) + lane * ta.rows_box * 128, &cache_map, hb * 64, key & (a.block_size - 1), (is_v ? a.n_kv : 0) + u.kvh, page, bar);
       }
     };
     if (warp == 8) {
       // ------------------------------------------------------------------ notes, queries, tiles of k
       int g = 0;                                                 // tiles of the block so far
       bool ok = true;
-      auto leave_note = [&](int i, int p) {
-        if (p >= end) return;
+      auto note_at = [&](int p) {                                // (last: a place yet)
         Piece u = piece_at<BN, 2, kExtra>(a, lens, offs, p, end);
         if (u.t0 == u.t1) u = piece_at<BN, 2, kExtra>(a, lens, offs, u.next, end);       // (the block's first place was a unit's last)
+        return PieceNote{u.s, u.kvh, u.item, u.t0, u.t1 - u.t0, u.r.start, u.r.n, u.r.nk, u.r.prefix, u.r.lo, u.r.first, u.r.n_pre, u.r.tiles, u.two, u.last, u.next};
+      };
+      auto leave_note = [&](int i, PieceNote& u) {
+        u.last = u.t0 == 0 && u.nt < u.tiles ? block_of<kExtra>(work, u.last) : 0;
         if (lane == 0) {
-          volatile PieceNote* n = &notes[i % kRing];
-          n->s = u.s; n->kvh = u.kvh; n->item = u.item; n->t0 = u.t0; n->nt = u.t1 - u.t0; n->start = u.r.start; n->n = u.r.n; n->nk = u.r.nk;
-          n->prefix = u.r.prefix; n->lo = u.r.lo; n->first = u.r.first; n->n_pre = u.r.n_pre; n->tiles = u.r.tiles;
-          n->two = u.two;
-          n->last = u.t0 == 0 && u.t1 < u.r.tiles ? block_of<kExtra>(work, u.last) : 0;
-          n->next = u.next;
+          notes[i % kRing] = u;
           mbar_arrive(noted(i));
         }
         __syncwarp();
       };
-      leave_note(0, begin);
-      for (int i = 0, p = begin; p < end && ok; ++i) {
-        NotePtr u = &notes[i % kRing];                           // (written by this warp)
-        const int t0 = u->t0, nt = u->nt;
-        int page = entry(u, t0);
+      auto bring_q = [&](const PieceNote& u) {
+        if (lane == 0) {
+          const int items = u.two ? 2 : 1;
+          mbar_arrive_expect_tx(q_full, (uint32_t)(items * rows_item * 128 * kHB));
+          for (int x = 0; x < items; ++x)
+#pragma unroll
+            for (int hb = 0; hb < kHB; ++hb)
+              tma_load_box_3d(sQ + x * kTileBytes + hb * (BM * 128), &q_map, hb * 64, u.kvh * a.group, u.start + (u.item + x) * ta.nodes_per_item, q_full);
+        }
+        __syncwarp();
+      };
+      PieceNote u = {}, behind = {};
+      int page = -1;
+      if (begin < end) {                                         // the way to the first keys is the block's start: nothing waits on it that can go beside it
+        u = note_at(begin);
+        page = entry(u, u.t0);
+        leave_note(0, u);
+        bring_q(u);
+      }
+      for (int i = 0, p = begin; p < end && ok; ++i, u = behind) {
+        const int t0 = u.t0, nt = u.nt;
+        if (i > 0) page = entry(u, t0);
         for (int t = t0; t < t0 + nt && ok; ++t, ++g) {
           const int s = g % kStages;
           if (g >= kStages && !mbar_wait_f(k_empty(s), (uint32_t)((g / kStages - 1) & 1), failed)) { ok = false; break; }
           const int next = t + 1 < t0 + nt ? entry(u, t + 1) : -1;
           bring(u, t, page, false, g);
           page = next;
-          if (t == t0) {                                         // the queries, as soon as the piece before has issued its last scores
-            if (i > 0 && !mbar_wait_f(q_free, (uint32_t)((i - 1) & 1), failed)) { ok = false; ++g; break; }
-            if (lane == 0) {
-              const int items = u->two ? 2 : 1;
-              mbar_arrive_expect_tx(q_full, (uint32_t)(items * rows_item * 128 * kHB));
-              for (int x = 0; x < items; ++x)
-#pragma unroll
-                for (int hb = 0; hb < kHB; ++hb)
-                  tma_load_box_3d(sQ + x * kTileBytes + hb * (BM * 128), &q_map, hb * 64, u->kvh * a.group, u->start + (u->item + x) * ta.nodes_per_item, q_full);
-            }
-            __syncwarp();
+          if (t == t0 && i > 0) {                                // the queries, as soon as the piece before has issued its last scores
+            if (!mbar_wait_f(q_free, (uint32_t)((i - 1) & 1), failed)) { ok = false; ++g; break; }
+            bring_q(u);
           }
-          if (t == min(t0 + 1, t0 + nt - 1)) leave_note(i + 1, u->next);      // (behind the first copies)
+          if (t == min(t0 + 1, t0 + nt - 1) && u.next < end) {   // (behind the first copies)
+            behind = note_at(u.next);
+            leave_note(i + 1, behind);
+          }
         }
-        p = u->next;
+        p = u.next;
         if (p >= end && ok) {                                    // the last queries, and the arrival behind them
           mbar_wait_drain(q_full, (uint32_t)(i & 1));
           ok = mbar_wait_f(q_free, (uint32_t)(i & 1), failed);
@@ -317,9 +333,9 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
       int g = 0;
       bool ok = true;
       for (int i = 0, p = begin; p < end && ok; ++i) {
-        NotePtr u = note_of(i, ok);
+        const PieceNote u = copy_of(i, ok);
         if (!ok) break;
-        const int t0 = u->t0, nt = u->nt;
+        const int t0 = u.t0, nt = u.nt;
         int page = entry(u, t0);
         for (int t = t0; t < t0 + nt; ++t, ++g) {
           const int s = g % kStages;
@@ -328,7 +344,7 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
           bring(u, t, page, true, g);
           page = next;
         }
-        p = u->next;
+        p = u.next;
       }
       for (int i = max(0, g - kStages); i < g; ++i) mbar_wait_drain(v_full(i % kStages), (uint32_t)((i / kStages) & 1));
       for (int i = max(0, g - kStages); i < g && ok; ++i) ok = mbar_wait_f(v_empty(i % kStages), (uint32_t)((i / kStages) & 1), failed);
@@ -337,9 +353,9 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
       int g = 0;
       bool ok = true;
       for (int i = 0, p = begin; p < end && ok; ++i) {
-        NotePtr u = note_of(i, ok);
+        const PieceNote u = copy_of(i, ok);
         if (!ok) break;
-        const int t0 = u->t0, nt = u->nt;
+        const int t0 = u.t0, nt = u.nt;
         if (lane == 0) odd_values[i % kRing] = 0;
         for (int t = t0; t < t0 + nt && ok; ++t, ++g) {
           const int s = g % kStages;
@@ -406,7 +422,7 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
           __syncwarp();
           arrive_if(lane == 0, v_fixed(s));
         }
-        p = u->next;
+        p = u.next;
       }
     } else if (warp == 10) {
       // ------------------------------------------------------------------ products
@@ -542,7 +558,7 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
           tmem_wait_ld();
         } else {                                                 // what the row sees of the tile's keys, as bits
           int key0, lo, hi;
-          rows_seen(u, t, key0, lo, hi);
+          rows_seen(*u, t, key0, lo, hi);
           lo = max(lo, after + 1 - key0);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -642,8 +658,8 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
 #pragma unroll 1
           for (int t = u->t0; t < u->t0 + nt; ++t) {
             int key0, lo, hi;
-            rows_seen(u, t, key0, lo, hi);
-            if (!seen_by_some(a, u, t, key0)) continue;
+            rows_seen(*u, t, key0, lo, hi);
+            if (!seen_by_some(a, *u, t, key0)) continue;
             const bool nodes = t >= u->n_pre;
 #pragma unroll 1
             for (int k = key0 + lo; k < key0 + hi; ++k) {
@@ -690,7 +706,7 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
         }
       };
       if (any_mine && two) {
-        constexpr int kN = HD % 32 == 0 ? 32 : 16;
+        constexpr int kN = HD / 2;
 #pragma unroll 1
         for (int c0 = 0; c0 < HD; c0 += kN) {
           float o[kN];
@@ -700,10 +716,10 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
           put(c0, o);
         }
       } else if (any_mine) {
-        constexpr int kN = HD % 32 == 0 ? 16 : 8;
+        constexpr int kN = HD / 2;
         const bool other_has = (x ^ 1) < nt;
-#pragma unroll 1
-        for (int c0 = x * (HD / 2); c0 < (x + 1) * (HD / 2); c0 += kN) {
+        const int c0 = x * kN;
+        {
           float o[kN], r[kN];
 #pragma unroll
           for (int c = 0; c < kN; c += 8) {
