@@ -13,6 +13,7 @@ constexpr int kErrOptions = 5;             // value of the error word
 constexpr int kChunk = 4096;               // values of a row that a block takes
 constexpr int kThreads = 256, kPer = kChunk / kThreads;
 constexpr int kMaxNodes = 256;             // nodes of a drafted tree
+constexpr int kEntries = 2 * kThreads;     // biases that are looked at at once, two a thread
 constexpr unsigned kInPrompt = 0x80000000u;
 
 struct AdjustArgs {
@@ -40,11 +41,12 @@ __global__ void __launch_bounds__(kThreads, 4) adjust_logits_kernel(AdjustArgs a
   __shared__ __align__(16) float bias[kChunk];
   __shared__ unsigned path[kMaxNodes];     // the tree's nodes whose token is one of the chunk's: node << 16 | value
   __shared__ int n_path;
-  __shared__ unsigned entry_at[256];       // entries of the list of biases
-  __shared__ float entry_value[256];
+  __shared__ unsigned entry_at[kEntries];  // of so many entries of the list of biases those of the chunk's tokens, in the list's order
+  __shared__ float entry_value[kEntries];
+  __shared__ int entries_of[kThreads / 32];
   pdl_launch_dependents();
   pdl_wait();
-  const int tid = threadIdx.x, lane = tid & 31;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int v0 = blockIdx.x * kChunk, width = min(kChunk, a.vocab - v0);
   const int row0 = blockIdx.y * rows_block, row1 = min(row0 + rows_block, a.n_rows);
   // this thread's k-th value; wide: four neighbours at a time
@@ -52,6 +54,7 @@ __global__ void __launch_bounds__(kThreads, 4) adjust_logits_kernel(AdjustArgs a
   auto owner = [&](int i) { return kWide ? (i >> 2) % kThreads : i % kThreads; };
   int current = -1;                        // the request that seen, bias and path are of
   bool penalties = false, biases = false;
+  float rep = 1.f, freq = 0.f, pres = 0.f;
   unsigned long long own = 0ull;           // this thread's entries of path
   // Which of this thread's values mask `which` allows.
   auto allowed = [&](int which) {
@@ -79,6 +82,11 @@ __global__ void __launch_bounds__(kThreads, 4) adjust_logits_kernel(AdjustArgs a
       if (a.history) {
         n_history = min(max(a.history_len[req], 0), a.history_width);
         n_prompt = a.prompt_len[req];
+      }
+      if (penalties) {
+        rep = a.repetition[req];
+        freq = a.frequency[req];
+        pres = a.presence[req];
       }
       if (a.tree_tokens) {
         first = min(max(a.cu_q[req], 0), a.n_rows);
@@ -127,6 +135,17 @@ __global__ void __launch_bounds__(kThreads, 4) adjust_logits_kernel(AdjustArgs a
       next_which = mask_of(r + 1);
     }
     if (fresh) {
+      unsigned at[2];
+      float value[2];
+      auto entries = [&](int base) {                             // this thread's two of them
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int e = base + 2 * tid + k;
+          at[k] = e < b1 ? (unsigned)(a.bias_token[e] - v0) : 0xffffffffu;
+          value[k] = e < b1 ? a.bias_value[e] : 0.f;
+        }
+      };
+      entries(b0);
       if (penalties) {
         auto note = [&](int token, bool prompt) {
           const unsigned i = (unsigned)(token - v0);
@@ -149,30 +168,39 @@ __global__ void __launch_bounds__(kThreads, 4) adjust_logits_kernel(AdjustArgs a
           if (i < (unsigned)width) path[atomicAdd(&n_path, 1)] = ((unsigned)j << 16) | i;
         }
       }
-      if (biases && tid >= kThreads - 32) {
-        // In the order of the list, so that a token that is listed twice gets the same sum in every run: one warp, 32 entries
-        // at a time (eight times as many requested at once), the first lane of those that name one token adds theirs up.
-        for (int base = b0; base < b1; base += 256) {
+      // In the order of the list, so that a token that is listed twice gets the same sum in every run: the first entry of those that name
+      // one token adds theirs up.
+      for (int base = b0; base < b1; base += kEntries) {
+        const bool mine0 = at[0] < (unsigned)width, mine1 = at[1] < (unsigned)width;
+        const unsigned has0 = __ballot_sync(0xffffffffu, mine0), has1 = __ballot_sync(0xffffffffu, mine1), below = (1u << lane) - 1u;
+        if (lane == 0) entries_of[warp] = __popc(has0) + __popc(has1);
+        __syncthreads();
+        int n = 0, to = 0;
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const int e = base + 32 * k + lane;
-            entry_at[32 * k + lane] = e < b1 ? (unsigned)(a.bias_token[e] - v0) : 0xffffffffu;
-            entry_value[32 * k + lane] = e < b1 ? a.bias_value[e] : 0.f;
-          }
-          __syncwarp();
-#pragma unroll 1
-          for (int k = 0; k < 8; ++k) {
-            const unsigned at = entry_at[32 * k + lane];
-            const bool mine = at < (unsigned)width;
-            if (!__any_sync(0xffffffffu, mine)) continue;
-            const unsigned same = __match_any_sync(0xffffffffu, mine ? at : 0xffffffffu);
-            if (mine && (same & ((1u << lane) - 1u)) == 0u) {
-              float sum = bias[at];
-              for (unsigned left = same; left; left &= left - 1) sum += entry_value[32 * k + __ffs((int)left) - 1];
-              bias[at] = sum;
-            }
-            __syncwarp();
-          }
+        for (int w = 0; w < kThreads / 32; ++w) {
+          if (w == warp) to = n;
+          n += entries_of[w];
+        }
+        to += __popc(has0 & below) + __popc(has1 & below);
+        if (mine0) {
+          entry_at[to] = at[0];
+          entry_value[to] = value[0];
+        }
+        if (mine1) {
+          entry_at[to + mine0] = at[1];
+          entry_value[to + mine0] = value[1];
+        }
+        if (base + kEntries < b1) entries(base + kEntries);
+        __syncthreads();
+        for (int e = tid; e < n; e += kThreads) {
+          const unsigned i = entry_at[e];
+          bool is_first = true;
+          for (int o = 0; o < e; ++o) is_first &= entry_at[o] != i;
+          if (!is_first) continue;
+          float sum = bias[i];
+          for (int o = e; o < n; ++o)
+            if (entry_at[o] == i) sum += entry_value[o];
+          bias[i] = sum;
         }
       }
       __syncthreads();
@@ -196,12 +224,6 @@ __global__ void __launch_bounds__(kThreads, 4) adjust_logits_kernel(AdjustArgs a
         if (owner((int)(path[e] & 0xffffu)) == tid) step(e, by);
     };
     walk(1u);
-    float rep = 1.f, freq = 0.f, pres = 0.f;
-    if (penalties) {
-      rep = a.repetition[req];
-      freq = a.frequency[req];
-      pres = a.presence[req];
-    }
     auto adjust = [&](float y, unsigned c) {
       if (c) {
         y = y > 0.f ? y / rep : y * rep;
