@@ -174,7 +174,6 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
   auto noted = [&](int i) { return bar0 + 8u * (5 * kStages + 11 + i % kRing); };
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-  pdl_launch_dependents();
   if (tid == 0) {
     // s_full and o_done take the products' completion and an arrival of the thread that issued them: what that thread had seen before (a
     // tile's note, odd values) is then seen by those who wait there.  p_full takes an arrival of every warp of the half.
@@ -202,11 +201,13 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
     const CUtensorMap* m = lane == 0 ? &q_map : lane == 1 ? &k_map : lane == 2 ? &v_map : &cache_map;
     asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
   }
-  if (warp == 0) {
+  pdl_wait();
+  // Tensor memory is claimed behind everything that ran before, and what comes behind is let in once all blocks have theirs: a block that waited for
+  // a kernel while it held columns which that kernel's blocks still wait for would wait for good.
+  if (warp == 11) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_base_mem)), "r"(kTmemCols));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
-  pdl_wait();
   const int rows_item = ta.nodes_per_item * a.group;
   add_up_work<BN, 2, kExtra>(a, rows_item, lens, offs, scratch);
   if (tid < 2) a.notes[2 * blockIdx.x + tid] = make_int4(-1, 0, 0, 0);
@@ -214,6 +215,7 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_base_mem;
+  pdl_launch_dependents();
   int begin, end;
   const int work = offs[a.n_seqs];
   share_of_block<kExtra>(work, begin, end);
@@ -752,7 +754,7 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
   tc_fence_before();
   __syncthreads();
   if (*failed && tid == 0 && ta.error_flag) atomicExch(ta.error_flag, 3);
-  if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
+  if (warp == 11) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
 }
 
 // A map of [outer][middle][HD] bfloat16 with boxes of 64 x box_middle x box_outer.
