@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(kThreads) attention_tree_kernel(Args a, bool w
         const ulonglong2 at = rows_at[(t & 1) * kKeys + j];
         const T* src = (const T*)(value ? at.y : at.x);
         if (wide) {                                              // whole rows of 16-byte words
-          copy16(dst + j * kP + c, src && c < a.hd ? (const void*)(src + c) : (const void*)a.cache, src && c < a.hd);
+          copy16(dst + j * kP + c, src && c < a.hd ? (const void*)(src + c) : a.k, src && c < a.hd);
         } else {
 #pragma unroll
           for (int e = 0; e < kE; ++e) dst[j * kP + c + e] = src && c + e < a.hd ? src[c + e] : from_f32<T>(0.f);

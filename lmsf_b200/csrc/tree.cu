@@ -60,7 +60,7 @@ __global__ void __launch_bounds__(kMaxNodes) tree_layout_kernel(LayoutArgs a) {
   for (int w = 0; w < 8; ++w) before += sums[w];
   const int start = (int)min(before, (long long)a.n_rows);
   const int want = nodes_of(a, s), n = min(want, a.n_rows - start);
-  const int prefix = max(a.prefix_len[s], 0);
+  const int prefix = min(max(a.prefix_len[s], 0), 0x7fffffff - n);     // (no place or position of the request passes 32 bits)
   if (tid == 0) {
     if (s == 0) a.cu_q[0] = 0;
     a.cu_q[s + 1] = start + n;

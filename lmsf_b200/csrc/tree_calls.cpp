@@ -93,8 +93,28 @@ void must_be_ints(const at::Tensor* t, std::initializer_list<int64_t> shape, con
 // The size of dimension d, -1 where there is none.
 int64_t size_of(const at::Tensor* t, int64_t d) { return t && d < t->dim() ? t->size(d) : -1; }
 
+// Tensors of one option: all of them or none.
+void together(std::initializer_list<const at::Tensor*> ts, const char* names) {
+  size_t given = 0;
+  for (const at::Tensor* t : ts) given += t != nullptr;
+  if (given && given != ts.size()) refuse(std::string(names) + " belong together");
+}
+// Whether rows of x and of y (2-dimensional, contiguous in the last dimension) share memory; columns of one buffer do not.
+bool overlap(const at::Tensor& x, const at::Tensor& y) {
+  if (!x.numel() || !y.numel()) return false;
+  const int64_t nx = x.size(0), ny = y.size(0), wx = x.size(1) * x.element_size(), wy = y.size(1) * y.element_size();
+  const int64_t px = (int64_t)x.data_ptr(), py = (int64_t)y.data_ptr(), sx = nx > 1 ? x.stride(0) * x.element_size() : wx, sy = ny > 1 ? y.stride(0) * y.element_size() : wy;
+  if (px + (nx - 1) * sx + wx <= py || py + (ny - 1) * sy + wy <= px) return false;
+  if (sx != sy || sx <= 0) return true;
+  const int64_t d = ((py - px) % sx + sx) % sx;
+  return d < wx || d + wy > sx;
+}
+// The distance of rows that a kernel is given; of a single row it says nothing.
+int64_t row_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+constexpr int64_t kMost = 1ll << 30;             // of sizes that kernels count in 32 bits, with room for what they add
+
 int fits(int64_t v, const char* what) {
-  if (v > 2147483647ll) refuse(std::string(what) + ": a size of " + std::to_string(v));
+  if (v > kMost) refuse(std::string(what) + ": a size of " + std::to_string(v));
   return (int)v;
 }
 int dtype_code(const at::Tensor& t) {
@@ -131,6 +151,8 @@ PyObject* tree_layout(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const int block_size = r.small("block_size"), window = r.small("window");
     const at::Tensor* flag = r.tensor("error_flag", true);
     const int64_t S = size_of(tree_len, 0), N = size_of(token_seq, 0);
+    fits(S, what);
+    fits(N, what);
     must_be_ints(tree_len, {S}, "tree_len");
     must_be_ints(prefix_len, {S}, "prefix_len");
     must_be_ints(cu_q, {S + 1}, "cu_q");
@@ -198,21 +220,27 @@ PyObject* attention_tree(PyObject*, PyObject* const* args, Py_ssize_t n) {
     must_be_ints(mask, {N, mask->size(1)}, "mask");
     must_be_ints(positions, {N}, "positions");
     if (window < 0 || (window && !positions)) refuse("attention_tree: a window is positive and needs positions");
-    if (!std::isfinite(scale)) refuse("attention_tree: the scale must be finite");
+    if (!std::isfinite((float)scale)) refuse("attention_tree: the scale must be a finite float32");
+    if (mask->size(1) > kMost / 32 || block_size < 1 || block_size > kMost || table->size(1) > kMost / block_size || N > kMost)
+      refuse("attention_tree: " + std::to_string(table->size(1)) + " pages of " + std::to_string(block_size) + " positions, " + std::to_string(mask->size(1)) + " mask words, " +
+             std::to_string(N) + " rows are more than 32 bits count");
+    for (const at::Tensor* t : {q, k, v})
+      if (overlap(*out, *t)) refuse("attention_tree: out shares memory with q, k or v");
     must_be_ints(flag, {1}, "error_flag");
     const c10::cuda::CUDAGuard guard(r.device());
     if (N == 0 || S == 0) return kNothing;
+    const int64_t qs = row_stride(*q), ks = row_stride(*k), vs = row_stride(*v), os = row_stride(*out);
     const auto addresses = (uintptr_t)q->data_ptr() | (uintptr_t)k->data_ptr() | (uintptr_t)v->data_ptr() | (uintptr_t)cache->data_ptr();
-    const bool on_tc = tc && code == 1 && heads / kvh <= 128 && block_size >= 8 && (block_size & (block_size - 1)) == 0 && cache->size(0) > 0 && scale > 0.0 &&
-                       (q->stride(0) | k->stride(0) | v->stride(0)) % 8 == 0 && addresses % 16 == 0;
+    const bool on_tc = tc && code == 1 && heads / kvh <= 128 && block_size >= 8 && (block_size & (block_size - 1)) == 0 && cache->size(0) > 0 && (float)scale > 0.f &&
+                       (qs | ks | vs) % 8 == 0 && std::min(qs, std::min(ks, vs)) > 0 && addresses % 16 == 0;
     const at::Tensor space = at::empty({on_tc ? tc_bytes : plain_bytes}, q->options().dtype(at::kByte));
     void* stream = c10::cuda::getCurrentCUDAStream().stream();
     const int pages = fits(cache->size(0), what), blocks = fits(table->size(1), what), words = fits(mask->size(1), what), bs = fits(block_size, what);
     if (on_tc)
-      return tc(q->data_ptr(), q->stride(0), k->data_ptr(), k->stride(0), v->data_ptr(), v->stride(0), out->data_ptr(), out->stride(0), cache->data_ptr(), cache->stride(0),
+      return tc(q->data_ptr(), qs, k->data_ptr(), ks, v->data_ptr(), vs, out->data_ptr(), os, cache->data_ptr(), cache->stride(0),
                 cache->stride(1), pages, data(table), blocks, bs, data(cu_q), data(prefix), data(mask), words, data(positions), window, (float)scale, fits(S, what),
                 fits(N, what), (int)heads, (int)kvh, (int)hd, space.data_ptr(), sms, data(flag), stream);
-    const int rc = plain(q->data_ptr(), q->stride(0), k->data_ptr(), k->stride(0), v->data_ptr(), v->stride(0), out->data_ptr(), out->stride(0), cache->data_ptr(),
+    const int rc = plain(q->data_ptr(), qs, k->data_ptr(), ks, v->data_ptr(), vs, out->data_ptr(), os, cache->data_ptr(),
                          cache->stride(0), cache->stride(1), pages, data(table), blocks, bs, data(cu_q), data(prefix), data(mask), words, data(positions), window, (float)scale,
                          fits(S, what), fits(N, what), (int)heads, (int)kvh, (int)hd, code, space.data_ptr(), sms, stream);
     return rc < 0 ? kRefusedByPlain : rc;
@@ -239,8 +267,13 @@ PyObject* adjust_logits(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const bool some = rows && vocab;
     if (some && (logits->stride(1) != 1 || out->stride(1) != 1 || (rows > 1 && (logits->stride(0) < vocab || out->stride(0) < vocab))))
       refuse("adjust_logits: logits and out need a contiguous last dimension and rows apart");
-    if (some && rows > 1 && out->data_ptr() == logits->data_ptr() && out->stride(0) != logits->stride(0))
+    if (some && (out->data_ptr() != logits->data_ptr() || row_stride(*out) != row_stride(*logits)) && overlap(*out, *logits))
       refuse("adjust_logits: out is logits itself or lies apart from it");
+    together({history, length, prompt}, "adjust_logits: a history's tokens, lengths and prompt lengths");
+    together({presence, frequency, repetition}, "adjust_logits: the three penalties");
+    together({tokens, mask, cu_q}, "adjust_logits: a tree's tokens, mask and cu_q");
+    together({b_start, b_token, b_value}, "adjust_logits: a bias's starts, tokens and values");
+    together({bits, which}, "adjust_logits: masks and which of them a row takes");
     if ((history || tokens) && !presence) refuse("adjust_logits: occurrences are counted for penalties");
     const int64_t R = presence ? size_of(presence, 0) : b_start ? size_of(b_start, 0) - 1 : 0;
     must_be(presence, at::kFloat, {R}, "adjust_logits: presence");

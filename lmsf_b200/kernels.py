@@ -1011,8 +1011,8 @@ def tree_layout(cu_q: torch.Tensor, token_seq: torch.Tensor, positions: torch.Te
     cached tokens and its ancestors before it.  slots int64 [N]: the slot of the request's place prefix_len + i for its i-th row, page *
     block_size + offset by block_table (int32 [S, blocks]), -1 where there is no page.  mask int32 [N, words]: bit j of a row is
     set for its ancestors and itself, of which with window > 0 the nearest `window` only; None: not made.  Rows behind the last request's are left as they
-    were.  A tree has at most 32 * words and at most 256 nodes; a longer one, a parent that is not before its node, and rows beyond N are cut off
-    and reported in the device's error word (or error_flag) as code 5."""
+    were.  A tree has at most 32 * words and at most 256 nodes; a longer one, a parent that is not before its node, positions beyond 32 bits, and rows beyond N are
+    cut off and reported in the device's error word (or error_flag) as code 5."""
     mod, address = _TREE_CALLS or _tree_calls()
     f = _LAUNCHERS.get("tree_layout") or _LAUNCHERS.setdefault("tree_layout", address("tree.cu", "lmsf_tree_layout"))
     rc = mod.tree_layout(f, cu_q, token_seq, positions, slots, mask, parents, tree_len, prefix_len, block_table, block_size, window,
@@ -1051,7 +1051,8 @@ def attention_tree(out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch
                    n_kv_heads: int, head_dim: int, positions: Optional[torch.Tensor] = None, window: int = 0, error_flag: Optional[torch.Tensor] = None):
     """Attention of drafted trees: row t of request s sees the request's prefix_len[s] cached keys, read from the pages of `cache`
     [pages, 2, n_kv_heads, block_size, head_dim], and those of the request's own rows whose bits are set in mask[t] (int32 [N,
-    words]: bit j is the request's j-th row; `tree_layout` makes it), whose keys and values are in k and v.  Nothing is written to the cache: `tree_accept` moves there what is kept.
+    words]: bit j is the request's j-th row; `tree_layout` makes it), whose keys and values are in k and v.  Nothing is written to the cache: `tree_accept` moves there what is kept.  At
+    most 1,024 requests a call; out lies apart from q, k, v and the cache.
     q, out: [N, n_q_heads * head_dim]; k, v: [N, n_kv_heads * head_dim]; views whose last dimension is contiguous, float32 or
     bfloat16 like the cache (k rotated already).  cu_q int32 [S + 1], prefix_len int32 [S], block_table int32 [S, blocks].  A cached
     key in a page that the cache does not have (-1, say), or behind the table's last block, is seen by nobody; a row that sees nothing gets zeros.  window > 0: a row at
@@ -1093,6 +1094,9 @@ def adjust_logits(out: torch.Tensor, logits: torch.Tensor, row_req: Optional[tor
     mod, address = _TREE_CALLS or _tree_calls()
     f = _LAUNCHERS.get("adjust_logits") or _LAUNCHERS.setdefault("adjust_logits", address("adjust_logits.cu", "lmsf_adjust_logits"))
     none3 = (None, None, None)
+    for name, option, parts in (("history", history, 3), ("penalties", penalties, 3), ("tree", tree, 3), ("bias", bias, 3), ("allowed", allowed, 2)):
+        if option is not None and len(option) != parts:
+            raise KernelError(f"adjust_logits: {name} are {parts} tensors")
     rc = mod.adjust_logits(f, out, logits, row_req, *(history or none3), *(penalties or none3), *(tree or none3), *(bias or none3),
                            *(allowed or (None, None)), _flag_of(error_flag, logits))
     if rc != -3:

@@ -596,3 +596,70 @@ def test_a_step_of_trees_is_what_single_steps_give(dtype):
             kernels.attention_generic(one, q1, single[0], bt[s:s + 1], bs, zero, at, hd ** -0.5, 0, heads, kvh, hd)
             assert ((one.cpu().double() - out[row:row + 1].cpu().double()).abs() <= 2 * bound[row:row + 1]).all()
     assert single.equal(cache)
+
+
+# ----------------------------------------------------------------------------- calls at the edge of what is allowed
+
+@pytest.mark.parametrize("shape", ["tree", "chain"])
+@pytest.mark.parametrize("prefix", [2 ** 31 - 1, 2 ** 31 - 4])
+def test_layout_behind_the_last_position(shape, prefix):
+    """Positions that 32 bits do not hold: the request is laid out where its last one still is, has no slots and is reported."""
+    from lmsf_b200 import kernels
+    n, f = 7, flag()
+    o = [torch.empty(2, dtype=torch.int32, device=D), ints([0] * n), ints([0] * n), torch.zeros(n, dtype=torch.int64, device=D), torch.zeros((n, 1), dtype=torch.int32, device=D)]
+    parents = None if shape == "chain" else ints([-1, 0, 0, 1, 2, 3, 3])
+    kernels.tree_layout(*o, parents, ints([n]), ints([prefix]), ints([[0, 1, 2]]), 16, error_flag=f)
+    first = 2 ** 31 - 1 - n
+    depth = list(range(n)) if shape == "chain" else [0, 1, 1, 2, 2, 3, 3]
+    assert o[0].tolist() == [0, n] and o[2].tolist() == [first + d for d in depth]
+    assert o[3].tolist() == [-1] * n and f.item() == 5
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_of_a_row_without_a_stride(dtype, hd):
+    """One row: what its tensors say of the distance to the next means nothing."""
+    c = attention_case(6, [1], [70], 4, 2, hd, 16, dtype)
+    want = call_attention(c)
+    check_attention(c, want)
+    for name in ("q", "k", "v"):
+        t = c[name].clone()
+        for stride in (0, 1, 8):
+            assert call_attention({**c, name: t.as_strided(t.shape, (stride, 1))}).equal(want)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_of_nodes_that_share_keys(dtype, hd):
+    """Rows of k and v that are one row in memory."""
+    c = attention_case(7, [19], [70], 4, 2, hd, 16, dtype)
+    c["k"], c["v"] = c["k"][3:4].expand(19, -1), c["v"][5:6].expand(19, -1)
+    check_attention(c, call_attention(c))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_attention_without_a_cache(dtype):
+    """No page at all: a node sees its ancestors only."""
+    c = attention_case(9, [40, 3], [0, 0], 4, 2, 64, 16, dtype)
+    want = call_attention(c)
+    check_attention(c, want)
+    bare = {**c, "cache": c["cache"][:0], "prefix": [100, 5]}         # pages of the table that are none: nobody sees their keys
+    out = call_attention(bare)
+    check_attention(bare, out)
+
+
+def test_adjust_of_many_biases():
+    """More entries than are looked at at once, tokens listed many times far apart: every one counts once, in float32 and the list's order."""
+    from lmsf_b200 import kernels
+    rng = random.Random(3)
+    vocab, rows, n = 5000, 2, [1700, 513]
+    token = [rng.choice([7, 4095, 4096, rng.randrange(vocab)]) for _ in range(sum(n))]
+    value = [rng.uniform(-2, 2) for _ in token]
+    logits = torch.randn((rows, vocab), device=D)
+    v32 = torch.tensor(value, dtype=torch.float32)
+    out = torch.empty_like(logits)
+    kernels.adjust_logits(out, logits, bias=(ints([0, n[0], sum(n)]), ints(token), v32.to(D)))
+    add = torch.zeros((rows, vocab), dtype=torch.float32)
+    for i, t in enumerate(token):
+        add[0 if i < n[0] else 1, t] += v32[i]
+    assert (out.cpu() == logits.cpu() + add).all()

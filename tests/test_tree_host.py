@@ -98,3 +98,58 @@ def test_plain_tree_and_a_chain():
     tokens = [rng.randrange(50) for _ in range(20)]
     assert P.accept(tokens[1:] + [99], tokens, list(range(-1, 19)), [0, 20], 32) == ([list(range(20))], [99])
     assert P.accept(tokens[1:] + [99], tokens, list(range(-1, 19)), [0, 20], 6) == ([list(range(6))], [tokens[6]])
+
+
+# ----------------------------------------------------------------------------- calls that would read what is not there
+
+@pytest.mark.parametrize("kw", [dict(history=(I(2, 7), None, I(2))), dict(history=(I(2, 7), I(2), None)), dict(history=(None, I(2), I(2))), dict(penalties=(F(2), None, F(2))),
+                                dict(penalties=(F(2), F(2), None)), dict(tree=(I(6), I(6, 1), None)), dict(tree=(I(6), None, I(3))), dict(tree=(None, I(6, 1), I(3))),
+                                dict(bias=(I(3), None, F(5))), dict(bias=(I(3), I(5), None)), dict(bias=(None, I(5), F(5))), dict(allowed=(I(3, 2), None)),
+                                dict(allowed=(None, I(6)))])
+def test_adjust_refuses_half_an_option(kw):
+    with pytest.raises(KernelError, match="belong together"):
+        kernels.adjust_logits(**adjust_args(**kw))
+
+
+@pytest.mark.parametrize("kw", [dict(history=(I(2, 7), I(2))), dict(penalties=(F(2),)), dict(tree=(I(6), I(6, 1), I(3), I(3))), dict(bias=()), dict(allowed=(I(3, 2), I(6), I(6)))])
+def test_adjust_refuses_an_option_of_other_parts(kw):
+    with pytest.raises(KernelError, match="tensors"):
+        kernels.adjust_logits(**adjust_args(**kw))
+
+
+def test_adjust_apart_or_itself():
+    both, line = F(6, 96), F(6 * 40 + 20)
+    bad = [(line[:240].view(6, 40), line[20:].view(6, 40)), (both[:, :40], both[:, 30:70]), (both[:, 40:80], both[:, :48][:, 8:])]
+    for out, logits in bad:
+        with pytest.raises(KernelError, match="apart"):
+            kernels.adjust_logits(out, logits)
+    for out, logits in [(both[:, :40], both[:, 40:80]), (both[:, 56:], both[:, :40]), (both, both), (line[:40].view(1, 40), line[40:80].view(1, 40))]:
+        with pytest.raises(KernelError, match="CUDA tensors"):       # nothing else is wrong with them
+            kernels.adjust_logits(out, logits)
+
+
+def test_attention_refuses_an_output_over_its_inputs():
+    rows = F(9, 64 + 2 * 32)
+    q, k, v = rows[:, :64], rows[:, 64:96], rows[:, 96:]
+    for out in (q, rows[:, 32:96], rows[:, 64:]):
+        with pytest.raises(KernelError, match="shares memory"):
+            kernels.attention_tree(**attention_args(out=out, q=q, k=k, v=v))
+    wide = F(9, 2 * 64 + 2 * 32)
+    with pytest.raises(KernelError, match="CUDA tensors"):            # columns of one buffer
+        kernels.attention_tree(**attention_args(out=wide[:, 64:128], q=wide[:, :64], k=wide[:, 128:160], v=wide[:, 160:]))
+
+
+@pytest.mark.parametrize("kw", [dict(scale=1e300), dict(scale=-1e39), dict(scale=math.inf)])
+def test_attention_refuses_a_scale_beyond_float32(kw):
+    with pytest.raises(KernelError, match="scale"):
+        kernels.attention_tree(**attention_args(**kw))
+
+
+def test_attention_refuses_what_32_bits_do_not_count():
+    none = dict(out=F(0, 64), q=F(0, 64), k=F(0, 32), v=F(0, 32), cu_q=I(1), prefix_len=I(0))
+    with pytest.raises(KernelError, match="32 bits"):
+        kernels.attention_tree(**attention_args(**none, mask=I(0, 2 ** 25 + 1), block_table=I(0, 4)))
+    with pytest.raises(KernelError, match="32 bits"):
+        kernels.attention_tree(**attention_args(**none, mask=I(0, 1), block_table=I(0, 2 ** 26 + 1)))
+    with pytest.raises(KernelError, match="CUDA tensors"):
+        kernels.attention_tree(**attention_args(**none, mask=I(0, 2 ** 25), block_table=I(0, 2 ** 26)))
