@@ -1,5 +1,8 @@
 // Attention of drafted trees on the CUDA cores: float32 throughout for float32 (no TF32), and bfloat16 where the tensor-core
 // kernel does not take the shape.  Any head size up to 256, any group, any page size, any stride.
+// Measured: 3 requests of 13..48 nodes behind 515..1,500 keys, a window of 1,024, 32 heads of 64 over 8, float32: 50 to 54 us, 15 TFLOP/s of some 70.  Bound by
+// instructions and their latency: issue slots are 40 % used, a third of that by FMAs, with two warps a scheduler (a block has 89 KB of shared memory).  Tiles of 32 keys with three or
+// four blocks an SM took 62 to 72 us, 64 rows and 256 threads a block 55.
 #include "attention_tree.cuh"
 
 LMSF_DEFINE_LAST_ERROR(lmsf_attention_tree)

@@ -2,7 +2,12 @@
 // power of two of at least 8 keys.  The mathematics is attention_tree.cuh's: one pass over the keys with the running maximum and sum of the softmax.
 //
 // What bounds it: a request's keys and values are read once for all its nodes and all heads of a group, so up to some 150 rows a
-// kv head (nodes x heads of the group) the kernel is bound by their bytes, above by the tensor cores and the exponentials.
+// kv head (nodes x heads of the group) the kernel is bound by their bytes, above by the tensor cores and the exponentials.  What holds it
+// from both is the way of one tile: scores, their maximum, weights, the product with v and the next scores follow one another, some 3,100 cycles for a tile of two
+// items where their products take 2,048, and the first tile of a block has its way from memory before it.
+// Measured (captured in a graph, other inputs in every launch): 64 requests of 33..64 nodes behind 2,048..4,096 keys, 32 heads of 128 over 8: 226 us, 685 TFLOP/s
+// (of 1,628 that a library product reaches); 2 of 48 behind 24,000..32,000: 80 us, 600 TFLOP/s and 3.1 TB/s; 8 of 32 behind 2,047: 27.5 us, 2.6 TB/s (of 6.55); 27 of 1..64 behind
+// 130..2,300, 32 heads of 64 over 8: 40.5 us; one of 8 behind 97: 10.7 us.
 //
 // An item is up to 128 rows: 128 / group nodes x the heads of the group, which one copy brings into shared memory node-major.  A
 // block works on pieces of units (a request, a kv head, two items; see attention_tree.cuh) with 128 keys a tile:
@@ -17,7 +22,9 @@
 // (a warp for each half let both halves do the same at the same time).
 // Tensor memory: S of half x (128 columns, P over the first 64 of them as bfloat16 pairs) at 128 x, its output at 256 + 128 x.  (Steps of
 // 64 keys, whose scores would have two places to be in, were slower: a product of 64 columns takes the tensor cores as long as one
-// of 128, whose left operand has as many rows to be read.)
+// of 128, whose left operand has as many rows to be read.  For heads of 64, P in columns of its own and the next scores issued as soon as the last ones
+// are read was slower too, 45 us where this takes 41: one warp issues all products in one order, and a wait more a tile costs as much as the scores' time;
+// so was a strict turn of the two halves at their exponentials, 44 us: they do not contend for the exponentials' unit, which is 44 % busy.)
 // Weights are rounded to bfloat16 for P V (2^-8 relative, the operand type of the product); sums, maxima, outputs are float32.
 // Every wait is bounded (the two halves meet at an mbarrier too); when one runs out the block raises the error word (code 3) and ends.
 #include <cstring>
@@ -652,11 +659,53 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
       const int slot = (2 * (int)blockIdx.x + (u->t0 == 0 ? 1 : 0)) * 2 + (two ? x : 0);
       float* part = a.partials + slot * partial_floats(BM, HD) + row * 4;
       bf16* out = (bf16*)a.out + (u->start + node) * a.out_stride + (size_t)(u->kvh * a.group + row % a.group) * HD;
-      // columns [c0, c0 + kN) of the row's output, summed over this block's keys
-      auto put = [&](int c0, auto& o) {
-        constexpr int kN = sizeof(o) / 4;
+      // half a row's columns at a time, summed over this block's keys
+      constexpr int kN = HD / 2;
+      const bool other_has = !two && (x ^ 1) < nt;
+      const int c_from = two ? 0 : x * kN, c_to = two ? HD : c_from + kN;
+      if (any_mine) {
+#pragma unroll 1
+        for (int c0 = c_from; c0 < c_to; c0 += kN) {
+          float o[kN];
+#pragma unroll
+          for (int c = 0; c < kN; c += 8) tmem_ld8_issue(t_o + c0 + c, o + c);
+          if (two) {
+            tmem_wait_ld();
+          } else {
+            float r[kN];
+#pragma unroll
+            for (int c = 0; c < kN; c += 8) tmem_ld8_issue((t_o ^ 128u) + c0 + c, r + c);
+            tmem_wait_ld();
+#pragma unroll
+            for (int c = 0; c < kN; ++c) o[c] = (have ? o[c] * w_own : 0.f) + (other_has ? r[c] * w_other : 0.f);
+          }
+          if (!mine) continue;
+          if (whole) {
+#pragma unroll
+            for (int c = 0; c < kN; ++c) o[c] *= inv;
+            if (ta.wide_out) {
+#pragma unroll
+              for (int c = 0; c < kN; c += 8) {
+                uint4 w;
+                w.x = pack_bf16(o[c], o[c + 1]);
+                w.y = pack_bf16(o[c + 2], o[c + 3]);
+                w.z = pack_bf16(o[c + 4], o[c + 5]);
+                w.w = pack_bf16(o[c + 6], o[c + 7]);
+                *reinterpret_cast<uint4*>(out + c0 + c) = w;
+              }
+            } else {
+#pragma unroll
+              for (int c = 0; c < kN; ++c) out[c0 + c] = __float2bfloat16_rn(o[c]);
+            }
+          } else {
+#pragma unroll
+            for (int c = 0; c < kN; c += 4)
+              *reinterpret_cast<float4*>(part + (size_t)(c0 + c) * BM) = make_float4(o[c], o[c + 1], o[c + 2], o[c + 3]);
+          }
+        }
         if (odd_values[i_piece % kRing] && mine) {
-          // values that were set to zero, for the rows that see them (rare: nothing here is made to be fast)
+          // Values that were set to zero, for the rows that see them: infinities and NaN only, so that it does not matter that what they are added to has been
+          // divided and rounded already.  (Rare: nothing here is made to be fast.)
 #pragma unroll 1
           for (int t = u->t0; t < u->t0 + nt; ++t) {
             int key0, lo, hi;
@@ -675,63 +724,15 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
                 if (page < 0 || page >= a.pages) continue;
                 src = (const bf16*)a.cache + page * a.page_stride + a.v_off + ((size_t)u->kvh * a.block_size + (k & (a.block_size - 1))) * HD;
               }
-#pragma unroll
-              for (int c = 0; c < kN; ++c) {
-                const float v = __bfloat162float(src[c0 + c]);
-                if (!(fabsf(v) <= 3.4e38f)) o[c] += v;
+#pragma unroll 1
+              for (int c = c_from; c < c_to; ++c) {
+                const float v = __bfloat162float(src[c]);
+                if (fabsf(v) <= 3.4e38f) continue;
+                if (whole) out[c] = __float2bfloat16_rn(__bfloat162float(out[c]) + v);
+                else part[(size_t)(c & ~3) * BM + (c & 3)] += v;
               }
             }
           }
-        }
-        if (!mine) return;
-        if (whole) {
-#pragma unroll
-          for (int c = 0; c < kN; ++c) o[c] *= inv;
-          if (ta.wide_out) {
-#pragma unroll
-            for (int c = 0; c < kN; c += 8) {
-              uint4 w;
-              w.x = pack_bf16(o[c], o[c + 1]);
-              w.y = pack_bf16(o[c + 2], o[c + 3]);
-              w.z = pack_bf16(o[c + 4], o[c + 5]);
-              w.w = pack_bf16(o[c + 6], o[c + 7]);
-              *reinterpret_cast<uint4*>(out + c0 + c) = w;
-            }
-          } else {
-#pragma unroll
-            for (int c = 0; c < kN; ++c) out[c0 + c] = __float2bfloat16_rn(o[c]);
-          }
-        } else {
-#pragma unroll
-          for (int c = 0; c < kN; c += 4)
-            *reinterpret_cast<float4*>(part + (size_t)(c0 + c) * BM) = make_float4(o[c], o[c + 1], o[c + 2], o[c + 3]);
-        }
-      };
-      if (any_mine && two) {
-        constexpr int kN = HD / 2;
-#pragma unroll 1
-        for (int c0 = 0; c0 < HD; c0 += kN) {
-          float o[kN];
-#pragma unroll
-          for (int c = 0; c < kN; c += 8) tmem_ld8_issue(t_o + c0 + c, o + c);
-          tmem_wait_ld();
-          put(c0, o);
-        }
-      } else if (any_mine) {
-        constexpr int kN = HD / 2;
-        const bool other_has = (x ^ 1) < nt;
-        const int c0 = x * kN;
-        {
-          float o[kN], r[kN];
-#pragma unroll
-          for (int c = 0; c < kN; c += 8) {
-            tmem_ld8_issue(t_o + c0 + c, o + c);
-            tmem_ld8_issue((t_o ^ 128u) + c0 + c, r + c);
-          }
-          tmem_wait_ld();
-#pragma unroll
-          for (int c = 0; c < kN; ++c) o[c] = (have ? o[c] * w_own : 0.f) + (other_has ? r[c] * w_other : 0.f);
-          put(c0, o);
         }
       }
       if (!whole && mine && (two || x == 0)) {
