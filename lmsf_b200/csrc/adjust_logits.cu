@@ -34,22 +34,22 @@ struct AdjustArgs {
 };
 
 // A block takes kChunk values of up to `rows_block` rows in turn.  Few of a row's values have anything to do with its request: those that occur in the
-// history, in the tree or in the list of biases are put on a list when a row's request is another than the row's before, so the nodes of a tree share
+// history, in the tree or in the list of biases; they are marked when a row's request is another than the row's before, so the nodes of a tree share
 // one pass over their request's history.  A row's values come into shared memory by copies of their own (cp.async, the next row's while this one
-// is worked on; not at all where a grammar hides four neighbours); the listed ones are changed there, a thread each; then all leave, with -inf for those
-// that are not allowed.  Bound by memory: 8 bytes a value, 4 of them less where they are hidden.  (With the counts of every value looked at in every row,
-// more than half of the issue slots went to some 34 instructions a value, most of them
-// for divisions that one lane of a warp had asked for.)  Measured: 16 requests with 17 to 32 nodes, 128,256 values, a mask each, 85 us: 397 MB at 4.7 TB/s; 8
-// single rows 7.4 us, of which the launch and the chain of lengths, history, values and stores are nearly all.
+// is worked on; not at all where a grammar hides four neighbours); every thread changes the marked ones among those that it brought, without a barrier, and
+// all leave, with -inf for those that are not allowed.  Bound by memory: 8 bytes a value, 4 of them less where they are hidden.
+// (With the counts of every value looked at in every row, more than half of the issue slots went to some 34 instructions a value, most of them for divisions
+// that one lane of a warp had asked for: 89 us; with the marked ones on a list of the block's, between two barriers, 85.)  Measured: 16 requests with 17 to 32 nodes, 128,256 values, a mask each
+// row: 81 us, 397 MB at 4.9 TB/s; 8 single rows 7.1 us, of which the launch and the chain of lengths, history, values and stores are nearly all.  Chunks of 1,024
+// values took 116 us, of 4,096 (three blocks an SM) 84.
 template <bool kWide>
-__global__ void __launch_bounds__(kThreads) adjust_logits_kernel(AdjustArgs a, int rows_block) {
+__global__ void __launch_bounds__(kThreads, 5) adjust_logits_kernel(AdjustArgs a, int rows_block) {
   __shared__ __align__(16) float xs[2][kChunk];
   __shared__ __align__(16) unsigned seen[kChunk];
   __shared__ float bias[kChunk];           // where kHasBias says so
-  __shared__ unsigned short listed[kChunk];
   __shared__ unsigned path[kMaxNodes];     // the tree's nodes whose token is one of the chunk's: node << 16 | value
-  __shared__ bool on_row[kMaxNodes];       // which of them are on the row's path
-  __shared__ int n_path, n_listed;
+  __shared__ unsigned on_row[kThreads / 32][kMaxNodes / 32];      // a row's mask of the tree, a copy for every warp
+  __shared__ int n_path;
   __shared__ unsigned entry_at[kEntries];  // of so many entries of the list of biases those of the chunk's tokens, in the list's order
   __shared__ float entry_value[kEntries];
   __shared__ int entries_of[kThreads / 32];
@@ -60,16 +60,16 @@ __global__ void __launch_bounds__(kThreads) adjust_logits_kernel(AdjustArgs a, i
   const int row0 = blockIdx.y * rows_block, row1 = min(row0 + rows_block, a.n_rows);
   // this thread's k-th value; wide: four neighbours at a time
   auto place = [&](int k) { return kWide ? 4 * (tid + kThreads * (k >> 2)) + (k & 3) : tid + kThreads * k; };
+  const bool whole = width == kChunk;      // no place of the chunk is behind the vocabulary's end: nothing to look at in the loops over a row
   // Which of this thread's values mask `which` allows.
   auto allowed = [&](int which) {
     if (which < 0 || which >= a.n_allowed) return 0xffffu;
-    const unsigned* words = a.allowed + (size_t)which * a.allowed_words;
+    const unsigned* words = a.allowed + (size_t)which * a.allowed_words + (v0 + place(0)) / 32;
+    const int shift = place(0) & 31;       // (v0 and the distances between a thread's places are multiples of 32)
     unsigned ok = 0u;
 #pragma unroll
-    for (int k = 0; k < kPer; k += kWide ? 4 : 1) {
-      const int i = place(k);
-      if (i < width) ok |= ((words[(v0 + i) >> 5] >> ((v0 + i) & 31)) & (kWide ? 15u : 1u)) << k;
-    }
+    for (int k = 0; k < kPer; k += kWide ? 4 : 1)
+      if (whole || place(k) < width) ok |= ((words[(place(k) - place(0)) / 32] >> shift) & (kWide ? 15u : 1u)) << k;
     return ok;
   };
   auto copy = [&](float* dst, const float* src, auto bytes) {
@@ -86,14 +86,14 @@ __global__ void __launch_bounds__(kThreads) adjust_logits_kernel(AdjustArgs a, i
 #pragma unroll
     for (int k = 0; k < kPer; k += kWide ? 4 : 1) {
       const int i = place(k);
+      if (!((ok >> k) & (kWide ? 15u : 1u))) continue;
       if constexpr (kWide) {
-        if (!((ok >> k) & 15u)) continue;
-        if (i + 4 <= width) {
+        if (whole || i + 4 <= width) {
           copy(x + i, x_row + i, Sixteen{});
         } else {
           for (int e = i; e < width; ++e) copy(x + e, x_row + e, Four{});
         }
-      } else if (i < width && ((ok >> k) & 1u)) {
+      } else if (whole || i < width) {
         copy(x + i, x_row + i, Four{});
       }
     }
@@ -101,7 +101,8 @@ __global__ void __launch_bounds__(kThreads) adjust_logits_kernel(AdjustArgs a, i
   auto sent = [&]() { asm volatile("cp.async.commit_group;" ::: "memory"); };
   auto request_of = [&](int r) { return a.row_req ? a.row_req[r] : r; };
   auto mask_of = [&](int r) { return a.allowed ? a.allowed_row[r] : -1; };
-  int current = -1;                        // the request that the list is of
+  int current = -1;                        // the request that seen, bias and path are of
+  unsigned touched = 0u;                   // which of this thread's values it has anything to do with
   float rep = 1.f, freq = 0.f, pres = 0.f;
   int req = request_of(row0), which = mask_of(row0);
   unsigned ok = allowed(which);
@@ -117,7 +118,8 @@ __global__ void __launch_bounds__(kThreads) adjust_logits_kernel(AdjustArgs a, i
       next_req = request_of(r + 1);
       next_which = mask_of(r + 1);
     }
-    if (fresh) {                           // (everybody is done with the row before's list: the barrier before its values left)
+    if (fresh) {
+      if (current >= 0) __syncthreads();                         // the rows before are done with what is there
       int n_history = 0, n_prompt = 0, first = 0, nodes = 0, b0 = 0, b1 = 0;
       if (a.history) {
         n_history = min(max(a.history_len[req], 0), a.history_width);
@@ -138,11 +140,8 @@ __global__ void __launch_bounds__(kThreads) adjust_logits_kernel(AdjustArgs a, i
       }
       current = req;
       for (int i = tid; i < kChunk / 4; i += kThreads) reinterpret_cast<uint4*>(seen)[i] = make_uint4(0u, 0u, 0u, 0u);
-      if (tid == 0) n_path = n_listed = 0;
+      if (tid == 0) n_path = 0;
       __syncthreads();
-      auto list = [&](unsigned i, unsigned before) {             // before: the value's word as it was
-        if (before == 0u) listed[atomicAdd(&n_listed, 1)] = (unsigned short)i;
-      };
       unsigned at[2];
       float value[2];
       auto entries = [&](int base) {                             // this thread's two of them
@@ -163,15 +162,17 @@ __global__ void __launch_bounds__(kThreads) adjust_logits_kernel(AdjustArgs a, i
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
             const unsigned i = (unsigned)(t[k] - v0);
-            if (i0 + k * kThreads < n_history && i < (unsigned)width)
-              list(i, i0 + k * kThreads < n_prompt ? atomicOr(&seen[i], kInPrompt) : atomicAdd(&seen[i], 1u));
+            if (i0 + k * kThreads < n_history && i < (unsigned)width) {
+              if (i0 + k * kThreads < n_prompt) atomicOr(&seen[i], kInPrompt);
+              else atomicAdd(&seen[i], 1u);
+            }
           }
         }
         for (int j = tid; j < nodes; j += kThreads) {
           const unsigned i = (unsigned)(a.tree_tokens[first + j] - v0);
           if (i < (unsigned)width) {
             path[atomicAdd(&n_path, 1)] = ((unsigned)j << 16) | i;
-            list(i, atomicOr(&seen[i], kOnTree));
+            atomicOr(&seen[i], kOnTree);
           }
         }
       }
@@ -209,29 +210,34 @@ __global__ void __launch_bounds__(kThreads) adjust_logits_kernel(AdjustArgs a, i
           for (int o = e; o < n; ++o)
             if (entry_at[o] == i) sum += entry_value[o];
           bias[i] = sum;
-          list(i, before);
         }
       }
       __syncthreads();
+      touched = 0u;
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) touched |= (place(k) < width && seen[place(k)] ? 1u : 0u) << k;
     }
     const unsigned next_ok = r + 1 < row1 ? allowed(next_which) : 0u;
     if (r + 1 < row1) request(r + 1, next_ok, xs[(r + 1 - row0) & 1]);
     sent();
     const int on_path = penalties && a.tree_tokens ? n_path : 0;
-    for (int e = tid; e < on_path; e += kThreads) {
-      const unsigned node = path[e] >> 16;
-      on_row[e] = (a.tree_mask[(size_t)r * a.words + (node >> 5)] >> (node & 31)) & 1u;
+    if (on_path > 0) {
+      if (lane < a.words) on_row[warp][lane] = a.tree_mask[(size_t)r * a.words + lane];
+      __syncwarp();
     }
-    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    asm volatile("cp.async.wait_group 1;" ::: "memory");         // (a thread works on values that it brought itself)
     if (penalties || biases) {
-      __syncthreads();
-      for (int l = tid; l < n_listed; l += kThreads) {
-        const unsigned i = listed[l], word = seen[i];
+      for (unsigned left = touched & ok; left; left &= left - 1) {
+        const int i = place(__ffs((int)left) - 1);
+        const unsigned word = seen[i];
         unsigned said = word & kCount;
         if (word & kOnTree)
-          for (int e = 0; e < on_path; ++e) said += (path[e] & 0xffffu) == i && on_row[e];
+          for (int e = 0; e < on_path; ++e) {
+            const unsigned node = path[e] >> 16;
+            if ((path[e] & 0xffffu) == i) said += (on_row[warp][node >> 5] >> (node & 31)) & 1u;
+          }
         float y = x[i];
-        if (said | (word & kInPrompt)) {
+        if (penalties && (said | (word & kInPrompt))) {
           y = y > 0.f ? y / rep : y * rep;
           y -= freq * (float)said;
           if (said) y -= pres;
@@ -239,20 +245,20 @@ __global__ void __launch_bounds__(kThreads) adjust_logits_kernel(AdjustArgs a, i
         if (word & kHasBias) y += bias[i];
         x[i] = y;
       }
-      __syncthreads();
+      __syncwarp();
     }
     float* out_row = a.out + r * a.out_stride + v0;
 #pragma unroll
     for (int k = 0; k < kPer; k += kWide ? 4 : 1) {
       const int i = place(k);
-      if (i >= width) continue;
+      if (!whole && i >= width) continue;
       if constexpr (kWide) {               // (x is whole, also behind the vocabulary's end)
         const float4 f = *reinterpret_cast<const float4*>(x + i);
         float y[4] = {f.x, f.y, f.z, f.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           if (!((ok >> (k + e)) & 1u)) y[e] = -INFINITY;
-        if (i + 4 <= width) {
+        if (whole || i + 4 <= width) {
           *reinterpret_cast<float4*>(out_row + i) = make_float4(y[0], y[1], y[2], y[3]);
         } else {
 #pragma unroll
@@ -288,7 +294,7 @@ LMSF_API int lmsf_adjust_logits(float* out, long long out_stride, const float* l
                prompt_len, presence, frequency, repetition, tree_tokens, tree_mask, cu_q, words, bias_start, bias_token, bias_value, n_bias,
                allowed, allowed_row, n_allowed, allowed_words, error_flag};
   // Rows of a block: one, where rows are few; more, where that leaves 16 blocks and more for each of 148 SMs, so that the rows of a request
-  // share its list.  (16 requests with 17 to 32 nodes over 128,256 values: 100 us with 4 blocks and more, 90 with 8, 85 with 16, 89 with 32.)
+  // share its list.  (16 requests with 17 to 32 nodes over 128,256 values: 102 us with 4 blocks and more, 87 with 8, 81 with 16, 86 with 32.)
   const int chunks = ceil_div(vocab, kChunk);
   const long long blocks = (long long)chunks * n_rows;
   int rows_block = 1;
