@@ -663,3 +663,61 @@ def test_adjust_of_many_biases():
     for i, t in enumerate(token):
         add[0 if i < n[0] else 1, t] += v32[i]
     assert (out.cpu() == logits.cpu() + add).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_attention_of_as_many_requests_as_a_launch_takes(dtype):
+    from lmsf_b200 import kernels
+    rng = random.Random(12)
+    lens, prefix = [rng.choice([0, 1, 1, 2, 5]) for _ in range(1024)], [rng.choice([0, 1, 17, 40, 130]) for _ in range(1024)]
+    c = attention_case(12, lens, prefix, 4, 2, 64, 16, dtype, spare_rows=3)
+    check_attention(c, call_attention(c))
+    more = {**c, "prefix": prefix + [0], "cu": c["cu"] + [c["cu"][-1]], "table": c["table"] + [[-1] * len(c["table"][0])]}
+    with pytest.raises(kernels.KernelError, match="1024"):
+        call_attention(more)
+
+
+@pytest.mark.parametrize("rows,vocab", [(70000, 3), (66000, 64)])
+def test_adjust_of_very_many_rows(rows, vocab):
+    """More rows than a grid has in one dimension."""
+    from lmsf_b200 import kernels
+    g = torch.Generator(device=D).manual_seed(2)
+    logits = torch.randn((rows, vocab), generator=g, device=D)
+    req = torch.randint(0, 2, (rows,), generator=g, device=D, dtype=torch.int32)
+    which = torch.randint(-1, 2, (rows,), generator=g, device=D, dtype=torch.int32)
+    bits = ints([[0b101] + [0] * ((vocab + 31) // 32 - 1), [0b010] + [-1] * ((vocab + 31) // 32 - 1)])
+    f = flag()
+    out = torch.empty_like(logits)
+    kernels.adjust_logits(out, logits, row_req=req, bias=(ints([0, 1, 2]), ints([0, 1]), torch.tensor([0.5, -2.0], device=D)), allowed=(bits, which), error_flag=f)
+    want = logits.clone()
+    want[:, 0] += torch.where(req == 0, 0.5, 0.0)
+    want[:, 1] += torch.where(req == 1, -2.0, 0.0)
+    for m in range(2):
+        hidden = [v for v in range(vocab) if not ((bits[m, v // 32].item() >> (v % 32)) & 1)]
+        rows_of = (which == m).nonzero().flatten()
+        want[rows_of[:, None], torch.tensor(hidden, device=D)] = -math.inf
+    assert out.equal(want) and f.item() == 0
+
+
+def test_two_streams_at_once():
+    """Calls side by side keep workspaces of their own: the same bits as one after the other."""
+    cases = [attention_case(20 + i, lens, prefix, 8, 2, 128, 16, "bf16") for i, (lens, prefix) in enumerate([([33, 64, 1], [700, 300, 2000]), ([48], [5000])])]
+    args = []
+    for c in cases:
+        S = len(c["prefix"])
+        args.append((c["q"], c["k"], c["v"], c["cache"], ints(c["table"]).reshape(S, -1), c["bs"], ints(c["cu"]), ints(c["prefix"]), c["mask"].to(D), c["scale"], 8, 2, 128))
+    from lmsf_b200 import kernels
+    want = [torch.empty_like(c["q"].contiguous()) for c in cases]
+    for w, a in zip(want, args):
+        kernels.attention_tree(w, *a)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[torch.empty_like(w) for _ in range(10)] for w in want]
+    torch.cuda.synchronize()
+    for i in range(10):
+        for st, outs, a in zip(streams, got, args):
+            with torch.cuda.stream(st):
+                kernels.attention_tree(outs[i], *a)
+    torch.cuda.synchronize()
+    for w, outs in zip(want, got):
+        assert all(o.equal(w) for o in outs)
