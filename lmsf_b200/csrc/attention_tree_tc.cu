@@ -125,7 +125,7 @@ __device__ __forceinline__ uint32_t bits(int lo, int hi) {
   return upto & ~below;
 }
 
-// What the warps of a block need to know of a piece, left in shared memory by warp 11 a piece ahead.  They read it where they need it:
+// What the warps of a block need to know of a piece, left in shared memory by warp 8 a piece ahead.  They read it where they need it:
 // held in registers it would not fit beside a row's scores, nor into what the other warps keep.
 struct __align__(16) PieceNote { int s, kvh, item, t0, nt, start, n, nk, prefix, lo, first, n_pre, tiles, two, last, next; };   // last: the block that ends the unit
 typedef const volatile PieceNote* NotePtr;

@@ -721,3 +721,70 @@ def test_two_streams_at_once():
     torch.cuda.synchronize()
     for w, outs in zip(want, got):
         assert all(o.equal(w) for o in outs)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_a_captured_step_of_all_four(dtype):
+    """Layout, attention, logits and acceptance captured as one graph: replayed on other lengths, trees and tokens it gives the bits of eager calls."""
+    from lmsf_b200 import kernels
+    dt, S, N, H, KV, hd, bs, pages, vocab, calls = DTYPES[dtype], 3, 24, 8, 2, 64, 16, 80, 700, 2
+    g = torch.Generator(device=D).manual_seed(5)
+    rnd = lambda *shape: torch.randn(shape, generator=g, device=D).to(dt)  # noqa: E731
+    tokens, parents = torch.zeros(N, dtype=torch.int32, device=D), torch.zeros(N, dtype=torch.int32, device=D)
+    lens, prefix = torch.zeros(S, dtype=torch.int32, device=D), torch.zeros(S, dtype=torch.int32, device=D)
+    table = torch.randperm(pages, generator=g, device=D)[:S * 26].view(S, 26).to(torch.int32)
+    q, k, v = rnd(N, H * hd), rnd(calls, N, KV * hd), rnd(calls, N, KV * hd)
+    w = torch.randn((H * hd, vocab), generator=g, device=D) * 0.05
+    history = torch.randint(0, vocab, (S, 400), generator=g, device=D, dtype=torch.int32)
+    penalties = tuple(torch.rand(S, generator=g, device=D) + 0.5 for _ in range(3))
+    bits = torch.randint(-2 ** 31, 2 ** 31, (2, (vocab + 31) // 32), generator=g, device=D).to(torch.int32)
+    which = torch.randint(-1, 2, (N,), generator=g, device=D, dtype=torch.int32)
+    cache0 = rnd(calls, pages, 2, KV, bs, hd)
+    kernels.error_word(torch.device(D)).zero_()
+
+    def buffers():
+        i = lambda *shape: torch.full(shape, -9, dtype=torch.int32, device=D)  # noqa: E731
+        return dict(cu=i(S + 1), seq=torch.zeros(N, dtype=torch.int32, device=D), pos=i(N), slots=torch.full((N,), -9, dtype=torch.int64, device=D), mask=torch.zeros((N, 1), dtype=torch.int32, device=D),
+                    out=torch.zeros((N, H * hd), dtype=dt, device=D), logits=torch.zeros((N, vocab), device=D), kept=i(S), path=i(S, 8), nxt=i(S), new=i(S), cache=cache0.clone())
+
+    def step(b):
+        kernels.tree_layout(b["cu"], b["seq"], b["pos"], b["slots"], b["mask"], parents, lens, prefix, table, bs)
+        kernels.attention_tree(b["out"], q, k[0], v[0], b["cache"][0], table, bs, b["cu"], prefix, b["mask"], hd ** -0.5, H, KV, hd)
+        torch.mm(b["out"].float(), w, out=b["logits"])
+        kernels.adjust_logits(b["logits"], b["logits"], row_req=b["seq"], history=(history, prefix, prefix), penalties=penalties, tree=(tokens, b["mask"], b["cu"]), allowed=(bits, which))
+        target = b["logits"].argmax(1).to(torch.int32)
+        kernels.tree_accept(b["kept"], b["path"], b["nxt"], b["new"], target, tokens, parents, b["cu"], prefix, b["slots"], k, v, b["cache"])
+
+    def inputs(seed):
+        rng = random.Random(seed)
+        n = [rng.randrange(0, 9) for _ in range(S)]
+        trees = [P.random_parents(rng, m) for m in n]
+        flat = [p for t in trees for p in t]
+        parents.copy_(ints(flat + [0] * (N - len(flat))))
+        tokens.copy_(torch.randint(0, vocab, (N,), generator=torch.Generator().manual_seed(seed), dtype=torch.int32))
+        lens.copy_(ints(n))
+        prefix.copy_(ints([rng.randrange(0, 390) for _ in range(S)]))
+
+    captured = buffers()
+    inputs(0)
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        step(captured)                                               # (libraries are loaded and workspaces made before the capture)
+        graph = torch.cuda.CUDAGraph()
+        stream.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            step(captured)
+    torch.cuda.synchronize()
+    for seed in range(1, 7):
+        inputs(seed)
+        eager = buffers()
+        for name, t in buffers().items():
+            captured[name].copy_(t)
+        torch.cuda.synchronize()
+        step(eager)
+        graph.replay()
+        torch.cuda.synchronize()
+        for name in eager:
+            assert captured[name].equal(eager[name]), (seed, name)
+    assert kernels.error_word(torch.device(D)).item() == 0
+    del graph
