@@ -645,8 +645,10 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
       float w_own = 1.f, w_other = 0.f;
       if (!two) {
         stats[x][row] = make_float2(m, l);
+        tc_fence_before();
         meet();
         if (!ok) break;
+        tc_fence_after();                                        // the other half's output is read below, and o_done of this half says nothing of it
         const float2 o = stats[x ^ 1][row];
         const float m_all = fmaxf(m, o.x), base = m_all == -INFINITY ? 0.f : m_all;
         w_own = ex2_approx(m - base);

@@ -788,3 +788,17 @@ def test_a_captured_step_of_all_four(dtype):
             assert captured[name].equal(eager[name]), (seed, name)
     assert kernels.error_word(torch.device(D)).item() == 0
     del graph
+
+
+# ----------------------------------------------------------------------------- what one thread leaves for another
+
+@pytest.mark.parametrize("hd", [64, 80, 128])
+@pytest.mark.parametrize("prefix", [0, 100, 128, 300])
+def test_attention_whose_halves_add_up(hd, prefix):
+    """Units of one item, whose tiles the two halves of a block take in turn and whose outputs they read from each other: one tile (a half without any), two,
+    three and four; the same bits in every run."""
+    c = attention_case(hd + prefix, [3, 1, 9] * 30, [prefix] * 90, 4, 2, hd, 16, "bf16")
+    out = call_attention(c)
+    check_attention(c, out)
+    for _ in range(10):
+        assert call_attention(c).equal(out)
