@@ -681,8 +681,7 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
 #pragma unroll
             for (int c = 0; c < kN; ++c) o[c] = (have ? o[c] * w_own : 0.f) + (other_has ? r[c] * w_other : 0.f);
           }
-          if (!mine) continue;
-          if (whole) {
+          if (mine && whole) {
 #pragma unroll
             for (int c = 0; c < kN; ++c) o[c] *= inv;
             if (ta.wide_out) {
@@ -699,11 +698,12 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
 #pragma unroll
               for (int c = 0; c < kN; ++c) out[c0 + c] = __float2bfloat16_rn(o[c]);
             }
-          } else {
+          } else if (mine) {
 #pragma unroll
             for (int c = 0; c < kN; c += 4)
               *reinterpret_cast<float4*>(part + (size_t)(c0 + c) * BM) = make_float4(o[c], o[c + 1], o[c + 2], o[c + 3]);
           }
+          __syncwarp();                                          // (the next columns are read by the whole warp at once, with or without a row of its own)
         }
         if (odd_values[i_piece % kRing] && mine) {
           // Values that were set to zero, for the rows that see them: infinities and NaN only, so that it does not matter that what they are added to has been

@@ -802,3 +802,17 @@ def test_attention_whose_halves_add_up(hd, prefix):
     check_attention(c, out)
     for _ in range(10):
         assert call_attention(c).equal(out)
+
+
+@pytest.mark.parametrize("hd", [64, 96, 128])
+@pytest.mark.parametrize("heads,kvh", [(8, 2), (3, 1), (7, 1)])
+@pytest.mark.parametrize("prefix", [[0, 0, 0], [700, 0, 300]])
+def test_attention_of_warps_with_a_few_rows(hd, heads, kvh, prefix):
+    """Units of two items of which the second ends inside a warp: each finished by one block (one tile, as many blocks as units), and cut."""
+    per = 128 // (heads // kvh)
+    lens = [per + 1, 2 * per - 1, per + per // 2]
+    c = attention_case(hd + heads, lens, prefix, heads, kvh, hd, 16, "bf16", spare_rows=2)
+    out = call_attention(c)
+    check_attention(c, out)
+    for _ in range(3):
+        assert call_attention(c).equal(out)
