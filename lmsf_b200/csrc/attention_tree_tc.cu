@@ -127,14 +127,18 @@ __device__ __forceinline__ uint32_t bits(int lo, int hi) {
 
 // What the warps of a block need to know of a piece, left in shared memory by warp 8 a piece ahead.  They read it where they need it:
 // held in registers it would not fit beside a row's scores, nor into what the other warps keep.
-struct __align__(16) PieceNote { int s, kvh, item, t0, nt, start, n, nk, prefix, lo, first, n_pre, tiles, two, last, next; };   // last: the block that ends the unit
+// last: the block that ends the unit; edge: the cached key up to which some row of the piece does not see all (its window lies behind), -1: none
+struct __align__(16) PieceNote { int s, kvh, item, t0, nt, start, n, nk, prefix, lo, edge, n_pre, tiles, two, last, next; };
 typedef const volatile PieceNote* NotePtr;
+// The unit's first tile begins with cached key `lo`, rounded down.
+template <typename Note>
+__device__ __forceinline__ int cached_key(const Note& u, int t) { return (u.lo / BN + t) * BN; }
 // Rows [lo, hi) of a tile are seen by some row of the piece's request; none of the others is multiplied, but for those that share a step
 // of 16 with them.
 template <typename Note>
 __device__ __forceinline__ void rows_seen(const Note& u, int t, int& key0, int& lo, int& hi) {
   const bool nodes = t >= u.n_pre;
-  key0 = nodes ? (t - u.n_pre) * BN : (u.first + t) * BN;
+  key0 = nodes ? (t - u.n_pre) * BN : cached_key(u, t);
   lo = nodes ? 0 : max(u.lo - key0, 0);
   hi = min((nodes ? u.nk : u.prefix) - key0, BN);
 }
@@ -143,11 +147,9 @@ __device__ __forceinline__ void rows_seen(const Note& u, int t, int& key0, int& 
 constexpr uint32_t kAllSeen = 0x80000000u;
 __device__ __forceinline__ int from16(uint32_t note) { return (note >> 16) & 15; }
 __device__ __forceinline__ int to16(uint32_t note) { return (note >> 20) & 15; }
-// Seen by some row, but perhaps not by every one: drafted tokens, and cached ones at the edge of a window.
+// Seen by some row, but perhaps not by every one: drafted tokens, and cached ones at the edge of a window or before it.
 template <typename Note>
-__device__ __forceinline__ bool seen_by_some(const Args& a, const Note& u, int t, int key0) {
-  return t >= u.n_pre || (a.window > 0 && key0 <= u.prefix + u.n - 1 - a.window);
-}
+__device__ __forceinline__ bool seen_by_some(const Note& u, int t, int key0) { return t >= u.n_pre || key0 <= u.edge; }
 
 __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(const TcArgs ta, const __grid_constant__ CUtensorMap q_map,
                                                                              const __grid_constant__ CUtensorMap k_map,
@@ -242,7 +244,7 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
     // one), or 32 drafted tokens; the page of the tile behind is requested before this one's copies and looked at after them.
     const int n_box = BN / ta.rows_box;
     auto entry = [&](const auto& u, int t) {                         // what the block table says of this lane's box of tile t
-      const int key = (u.first + t) * BN + lane * ta.rows_box;
+      const int key = cached_key(u, t) + lane * ta.rows_box;
       return t < u.n_pre && lane < n_box && key < u.prefix ? a.block_table[(size_t)u.s * a.max_blocks + (key >> ta.block_shift)] : -1;
     };
     // The tile's note goes out with it: the barrier's arrival is behind it.
@@ -256,7 +258,7 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
       const uint32_t here = __ballot_sync(0xffffffffu, there), missing = __ballot_sync(0xffffffffu, seen && !there);
       const int boxes = (hi + 31) / 32;                          // of drafted tokens
       if (lane == 0) {
-        const bool all = lo == 0 && hi == BN && !missing && !seen_by_some(a, u, t, key0);
+        const bool all = lo == 0 && hi == BN && !missing && !seen_by_some(u, t, key0);
         *(volatile uint32_t*)&tile_notes[is_v][g % kRing] = missing | ((uint32_t)(lo / 16) << 16) | ((uint32_t)((hi + 15) / 16) << 20) | (all ? kAllSeen : 0u);
         mbar_arrive_expect_tx(bar, (uint32_t)((nodes ? boxes * 32 : __popc(here) * ta.rows_box) * 128 * kHB));
       }
@@ -277,13 +279,19 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
       // ------------------------------------------------------------------ notes, queries, tiles of k
       int g = 0;                                                 // tiles of the block so far
       bool ok = true;
-      auto note_at = [&](int p) {                                // (last: a place yet)
+      auto note_at = [&](int p) {                                // (last: a place yet; edge: none yet)
         Piece u = piece_at<BN, 2, kExtra>(a, lens, offs, p, end);
         if (u.t0 == u.t1) u = piece_at<BN, 2, kExtra>(a, lens, offs, u.next, end);       // (the block's first place was a unit's last)
-        return PieceNote{u.s, u.kvh, u.item, u.t0, u.t1 - u.t0, u.r.start, u.r.n, u.r.nk, u.r.prefix, u.r.lo, u.r.first, u.r.n_pre, u.r.tiles, u.two, u.last, u.next};
+        return PieceNote{u.s, u.kvh, u.item, u.t0, u.t1 - u.t0, u.r.start, u.r.n, u.r.nk, u.r.prefix, u.r.lo, -1, u.r.n_pre, u.r.tiles, u.two, u.last, u.next};
       };
       auto leave_note = [&](int i, PieceNote& u) {
         u.last = u.t0 == 0 && u.nt < u.tiles ? block_of<kExtra>(work, u.last) : 0;
+        if (a.window > 0) {                                      // by the rows' own positions: a caller's may lie anywhere behind the cached tokens
+          const int from = u.item * ta.nodes_per_item, to = min(u.n, from + (u.two ? 2 : 1) * ta.nodes_per_item);
+          int top = 0;
+          for (int i = from + lane; i < to; i += 32) top = max(top, a.positions[u.start + i]);
+          u.edge = __reduce_max_sync(0xffffffffu, top) - a.window;
+        }
         if (lane == 0) {
           notes[i % kRing] = u;
           mbar_arrive(noted(i));
@@ -374,7 +382,7 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
           if (!(note & kAllSeen)) {
             int key0, lo, hi;
             rows_seen(u, t, key0, lo, hi);
-            const bool some = seen_by_some(a, u, t, key0);
+            const bool some = seen_by_some(u, t, key0);
             // eight lanes a row, four rows at a time, and the 64-wide blocks of the head one after the other
             const uint32_t v = sV + s * kTileBytes + (lane & 7) * 16;
             const int r_lane = lane >> 3;
@@ -712,7 +720,7 @@ __global__ void __launch_bounds__(kThreadsTotal, 1) attention_tree_tc_kernel(con
           for (int t = u->t0; t < u->t0 + nt; ++t) {
             int key0, lo, hi;
             rows_seen(*u, t, key0, lo, hi);
-            if (!seen_by_some(a, *u, t, key0)) continue;
+            if (!seen_by_some(*u, t, key0)) continue;
             const bool nodes = t >= u->n_pre;
 #pragma unroll 1
             for (int k = key0 + lo; k < key0 + hi; ++k) {

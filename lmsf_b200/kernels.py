@@ -1056,7 +1056,7 @@ def attention_tree(out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch
     q, out: [N, n_q_heads * head_dim]; k, v: [N, n_kv_heads * head_dim]; views whose last dimension is contiguous, float32 or
     bfloat16 like the cache (k rotated already).  cu_q int32 [S + 1], prefix_len int32 [S], block_table int32 [S, blocks].  A cached
     key in a page that the cache does not have (-1, say), or behind the table's last block, is seen by nobody; a row that sees nothing gets zeros.  window > 0: a row at
-    positions[t] (int32 [N], no less than prefix_len) sees only cached keys behind positions[t] - window; its own
+    positions[t] (int32 [N], no less than prefix_len, however far behind it) sees only cached keys behind positions[t] - window; its own
     request's rows are the mask's matter.  The lengths are read on the device alone: a captured call serves any lengths
     that fit its tensors.  Scores, softmax and sums are float32; in bfloat16 the weights are rounded to bfloat16 for their product with v."""
     mod, _ = _TREE_CALLS or _tree_calls()

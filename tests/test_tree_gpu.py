@@ -816,3 +816,58 @@ def test_attention_of_warps_with_a_few_rows(hd, heads, kvh, prefix):
     check_attention(c, out)
     for _ in range(3):
         assert call_attention(c).equal(out)
+
+
+# ----------------------------------------------------------------------------- windows of rows that lie anywhere behind the cached tokens
+
+def on_cores(monkeypatch, dtype):
+    """"bf16 on the CUDA cores" -> "bf16", with the tensor cores left out."""
+    from lmsf_b200 import kernels
+    if dtype.startswith("bf16 "):
+        monkeypatch.setattr(kernels, "USE_TC_TREE", False)
+        return "bf16"
+    return dtype
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "bf16 on the CUDA cores"])
+@pytest.mark.parametrize("hd,bs", [(64, 16), (128, 16), (96, 128)])
+@pytest.mark.parametrize("far", [0, 1, 130, 276, 599, 5000])
+def test_attention_of_positions_far_behind_the_cache(dtype, hd, bs, far, monkeypatch):
+    """A row's window follows its position wherever that lies: `far` and more behind the last cached token and the tree.  Every other request's cached
+    keys that no row sees are NaN, and so are their values."""
+    dtype, window = on_cores(monkeypatch, dtype), 600
+    prefix, lens = [1024, 1000, 385, 700], [1, 7, 40, 2]
+    c = attention_case(far + hd, lens, prefix, 4, 2, hd, bs, dtype, window)
+    rng = random.Random(far)
+    for s in range(4):
+        for t in range(c["cu"][s], c["cu"][s + 1]):
+            c["positions"][t] = prefix[s] + far + (rng.randrange(0, 2 * window) if t % 3 else 0)
+        least = min(c["positions"][c["cu"][s]:c["cu"][s + 1]])
+        for i in range(min(prefix[s], least - window + 1) if s % 2 == 0 else 0):
+            c["cache"][c["table"][s][i // bs], :, :, i % bs] = math.nan
+    check_attention(c, call_attention(c))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "bf16 on the CUDA cores"])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_with_a_window_over_a_table_that_ends(dtype, hd, monkeypatch):
+    """Cached tokens behind the table's last block are seen by nobody, and move nobody's window."""
+    c = attention_case(hd, [5, 1, 30], [1000, 900, 650], 4, 2, hd, 16, on_cores(monkeypatch, dtype), window=600)
+    c["table"] = [row[:40] for row in c["table"]]
+    check_attention(c, call_attention(c))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_attention_hides_infinities_behind_a_far_window(dtype):
+    """A value of infinity in a cached place reaches the rows whose window holds it, and no other."""
+    prefix, window = 512, 300
+    c = attention_case(3, [6], [prefix], 4, 2, 64, 16, dtype, window=window)
+    c["positions"] = [512, 640, 700, 730, 900, 513]
+    place, col = 390, 9                                           # seen by positions up to 689
+    c["cache"][c["table"][0][place // 16], 1, :, place % 16, col] = math.inf
+    out = call_attention(c)
+    for t, p in enumerate(c["positions"]):
+        inf = torch.isinf(out[t]).nonzero().flatten().tolist()
+        assert inf == ([col + 64 * h for h in range(4)] if p - window < place else []) and not torch.isnan(out[t]).any()
+    c["cache"][c["table"][0][place // 16], 1, :, place % 16, col] = 0.25
+    check_attention(c, call_attention(c))
