@@ -226,6 +226,7 @@ PyObject* attention_tree(PyObject*, PyObject* const* args, Py_ssize_t n) {
              std::to_string(N) + " rows are more than 32 bits count");
     for (const at::Tensor* t : {q, k, v})
       if (overlap(*out, *t)) refuse("attention_tree: out shares memory with q, k or v");
+    if (out->numel() && row_stride(*out) < out->size(1)) refuse("attention_tree: rows of out share memory");
     must_be_ints(flag, {1}, "error_flag");
     const c10::cuda::CUDAGuard guard(r.device());
     if (N == 0 || S == 0) return kNothing;

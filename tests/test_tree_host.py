@@ -153,3 +153,16 @@ def test_attention_refuses_what_32_bits_do_not_count():
         kernels.attention_tree(**attention_args(**none, mask=I(0, 1), block_table=I(0, 2 ** 26 + 1)))
     with pytest.raises(KernelError, match="CUDA tensors"):
         kernels.attention_tree(**attention_args(**none, mask=I(0, 2 ** 25), block_table=I(0, 2 ** 26)))
+
+
+# ----------------------------------------------------------------------------- memory that is written to and read or written again in one call
+
+def test_attention_refuses_rows_of_out_over_one_another():
+    for out in (F(1, 64).expand(9, 64), F(9 * 64).as_strided((9, 64), (63, 1)), F(9 * 64).as_strided((9, 64), (8, 1))):
+        with pytest.raises(KernelError, match="rows of out"):
+            kernels.attention_tree(**attention_args(out=out))
+    one = dict(out=F(1, 64).as_strided((1, 64), (0, 1)), q=F(1, 64), k=F(1, 32), v=F(1, 32), mask=I(1, 1))
+    with pytest.raises(KernelError, match="CUDA tensors"):            # a single row's stride says nothing
+        kernels.attention_tree(**attention_args(**one))
+    with pytest.raises(KernelError, match="CUDA tensors"):
+        kernels.attention_tree(**attention_args(out=F(9, 80)[:, 3:67]))
