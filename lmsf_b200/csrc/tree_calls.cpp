@@ -109,6 +109,14 @@ bool overlap(const at::Tensor& x, const at::Tensor& y) {
   const int64_t d = ((py - px) % sx + sx) % sx;
   return d < wx || d + wy > sx;
 }
+// Whether one of n rows of `width` bytes, `stride` apart from `rows` on, lies in the bytes of y, which is contiguous.
+bool rows_in(int64_t rows, int64_t n, int64_t width, int64_t stride, const at::Tensor& y) {
+  const int64_t from = (int64_t)y.data_ptr(), to = from + y.numel() * y.element_size();
+  if (n < 1 || width < 1 || from == to) return false;
+  const int64_t before = from - rows - width;      // the first row that ends behind y's first byte
+  const int64_t i = before < 0 ? 0 : stride > 0 ? before / stride + 1 : n;
+  return i < n && rows + i * stride < to;
+}
 // The distance of rows that a kernel is given; of a single row it says nothing.
 int64_t row_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
 constexpr int64_t kMost = 1ll << 30;             // of sizes that kernels count in 32 bits, with room for what they add
@@ -226,6 +234,8 @@ PyObject* attention_tree(PyObject*, PyObject* const* args, Py_ssize_t n) {
              std::to_string(N) + " rows are more than 32 bits count");
     for (const at::Tensor* t : {q, k, v})
       if (overlap(*out, *t)) refuse("attention_tree: out shares memory with q, k or v");
+    if (out->numel() && rows_in((int64_t)out->data_ptr(), N, out->size(1) * out->element_size(), row_stride(*out) * out->element_size(), *cache))
+      refuse("attention_tree: out shares memory with the cache");
     if (out->numel() && row_stride(*out) < out->size(1)) refuse("attention_tree: rows of out share memory");
     must_be_ints(flag, {1}, "error_flag");
     const c10::cuda::CUDAGuard guard(r.device());

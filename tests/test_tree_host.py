@@ -166,3 +166,23 @@ def test_attention_refuses_rows_of_out_over_one_another():
         kernels.attention_tree(**attention_args(**one))
     with pytest.raises(KernelError, match="CUDA tensors"):
         kernels.attention_tree(**attention_args(out=F(9, 80)[:, 3:67]))
+
+
+def test_attention_refuses_an_output_in_the_cache():
+    size = 5 * 2 * 2 * 16 * 16                                        # of the cache; 9 rows of 64 are 576
+    line = F(size + 2000)
+    cache = line[1000:1000 + size].view(5, 2, 2, 16, 16)
+    spread = F(9 * 3000)                                              # rows 3,000 apart, the cache after the first, its last value on the second or not
+    for out in (line[1000:1576].view(9, 64), line[425:1001].view(9, 64), line[1000 + size - 1:][:576].view(9, 64), line[500:].as_strided((9, 64), (600, 1))):
+        with pytest.raises(KernelError, match="the cache"):
+            kernels.attention_tree(**attention_args(out=out, cache=cache))
+    for out in (line[424:1000].view(9, 64), line[1000 + size:][:576].view(9, 64)):
+        with pytest.raises(KernelError, match="CUDA tensors"):        # right before and behind it
+            kernels.attention_tree(**attention_args(out=out, cache=cache))
+    small = dict(cache=spread[64:64 + 2560].view(1, 2, 2, 40, 16), block_size=40)
+    with pytest.raises(KernelError, match="CUDA tensors"):            # between two rows
+        kernels.attention_tree(**attention_args(out=spread.as_strided((9, 64), (2624, 1)), **small))
+    with pytest.raises(KernelError, match="the cache"):
+        kernels.attention_tree(**attention_args(out=spread.as_strided((9, 64), (2623, 1)), **small))
+    with pytest.raises(KernelError, match="CUDA tensors"):            # a cache of no pages
+        kernels.attention_tree(**attention_args(cache=F(0, 2, 2, 16, 16)))
