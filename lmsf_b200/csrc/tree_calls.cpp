@@ -362,6 +362,10 @@ PyObject* tree_accept(PyObject*, PyObject* const* args, Py_ssize_t n) {
           refuse("tree_accept: k and v must be [calls, rows, kv heads * head_dim] of the cache's dtype with a contiguous last dimension");
       copy = cache->numel() && N;
       if (copy) {
+        for (const at::Tensor* t : {k, v})
+          for (int64_t c = 0; c < t->size(0); ++c)
+            if (rows_in((int64_t)t->data_ptr() + c * t->stride(0) * size, N, width * size, t->stride(1) * size, *cache))
+              refuse("tree_accept: k and v lie apart from the cache");
         strides[0] = k->stride(0) * size; strides[1] = k->stride(1) * size; strides[2] = v->stride(0) * size; strides[3] = v->stride(1) * size;
         sizes[0] = fits(cache->size(0), what); sizes[1] = fits(cache->size(1), what); sizes[2] = fits(cache->size(3), what);
         sizes[3] = fits(cache->size(4), what); sizes[4] = fits(cache->size(5) * size, what);

@@ -1115,7 +1115,7 @@ def tree_accept(n_kept: torch.Tensor, path: torch.Tensor, next_token: torch.Tens
     them.  next_token int32 [S]: the model's choice behind the last of them (-1 without rows).  new_len int32 [S]: prefix_len + n_kept.
 
     With slots (int64 [N], of `tree_layout`), k, v ([calls, N, kv heads * head_dim] views with a contiguous last dimension: the step's keys and
-    values of every layer) and cache [calls, pages, 2, kv heads, block_size, head_dim] the kept rows' keys and values are written to
+    values of every layer, apart from the cache) and cache [calls, pages, 2, kv heads, block_size, head_dim] the kept rows' keys and values are written to
     the cache, the i-th to slot slots[cu_q[s] + i], in the same launch.  A slot outside the cache is not written and is reported
     in the device's error word (or error_flag) as code 2; trees of more than 256 rows as code 5 (their first 256 count)."""
     mod, address = _TREE_CALLS or _tree_calls()

@@ -186,3 +186,21 @@ def test_attention_refuses_an_output_in_the_cache():
         kernels.attention_tree(**attention_args(out=spread.as_strided((9, 64), (2623, 1)), **small))
     with pytest.raises(KernelError, match="CUDA tensors"):            # a cache of no pages
         kernels.attention_tree(**attention_args(cache=F(0, 2, 2, 16, 16)))
+
+
+def test_accept_refuses_keys_in_the_cache():
+    """Rows are copied in no order: one that lies in the cache may have been written over before it is read."""
+    size = 3 * 5 * 2 * 2 * 16 * 16
+    line = F(size + 4000)
+    cache = line[2000:2000 + size].view(3, 5, 2, 2, 16, 16)
+    inside, first, last = (line[at:at + 864].view(3, 9, 32) for at in (5000, 2000 - 863, 2000 + size - 1))
+    third = line[1000:].as_strided((3, 9, 32), (600, 40, 1))          # the third layer's rows alone
+    for t in (inside, first, last, third):
+        for name in ("k", "v"):
+            with pytest.raises(KernelError, match="apart from the cache"):
+                kernels.tree_accept(**accept_args(cache=cache, **{name: t}))
+    for t in (line[2000 - 864:2000].view(3, 9, 32), line[2000 + size:][:864].view(3, 9, 32), F(1, 1, 32).expand(3, 9, 32)):
+        with pytest.raises(KernelError, match="CUDA tensors"):        # right before and behind it, and one row for all
+            kernels.tree_accept(**accept_args(cache=cache, k=t, v=t))
+    with pytest.raises(KernelError, match="CUDA tensors"):            # nothing is written to a cache of no pages
+        kernels.tree_accept(**accept_args(cache=cache[:, :0]))
