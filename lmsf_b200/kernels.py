@@ -965,10 +965,6 @@ def attention_prefill_tc(out: torch.Tensor, q: torch.Tensor, cache: torch.Tensor
 
 # ----------------------------------------------------------------------------- trees of drafted tokens
 
-TREE_MAX_NODES = 256           # nodes of one tree (tree.cu)
-TREE_MAX_SEQS = 1024           # requests of one launch of attention_tree (attention_tree.cuh)
-
-
 _TREE_CALLS = None
 
 
