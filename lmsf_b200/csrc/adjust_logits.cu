@@ -23,7 +23,7 @@ struct AdjustArgs {
   float* out; long long out_stride;
   const float* logits; long long stride;
   int n_rows, vocab;
-  const int* row_req; int n_reqs;                                // null: row r is request r
+  const int* row_req; int n_reqs;                                // null: row r is request r; -1: no option is a request's
   const int* history; long long history_stride; int history_width;   // [n_reqs, width]
   const int* history_len; const int* prompt_len;
   const float* presence; const float* frequency; const float* repetition;
@@ -100,7 +100,7 @@ __global__ void __launch_bounds__(kThreads, 5) adjust_logits_kernel(AdjustArgs a
   };
   auto sent = [&]() { asm volatile("cp.async.commit_group;" ::: "memory"); };
   auto request_of = [&](int r) { return a.row_req ? a.row_req[r] : r; };
-  auto mask_of = [&](int r) { return a.allowed ? a.allowed_row[r] : -1; };
+  auto mask_of = [&](int r) { return a.allowed_row ? a.allowed_row[r] : -1; };
   int current = -1;                        // the request that seen, bias and path are of
   unsigned touched = 0u;                   // which of this thread's values it has anything to do with
   float rep = 1.f, freq = 0.f, pres = 0.f;
@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(kThreads, 5) adjust_logits_kernel(AdjustArgs a
   for (int r = row0; r < row1; ++r) {
     float* x = xs[(r - row0) & 1];
     const bool known = req >= 0 && req < a.n_reqs, fresh = known && req != current;
-    if (((!known && a.n_reqs > 0) || (a.allowed && which >= a.n_allowed)) && tid == 0 && blockIdx.x == 0 && a.error_flag) atomicExch(a.error_flag, kErrOptions);
+    if (((!known && a.n_reqs >= 0) || (a.allowed_row && which >= a.n_allowed)) && tid == 0 && blockIdx.x == 0 && a.error_flag) atomicExch(a.error_flag, kErrOptions);
     const bool penalties = known && a.repetition, biases = known && a.bias_start;
     int next_req = -1, next_which = -1;
     if (r + 1 < row1) {
@@ -277,7 +277,7 @@ __global__ void __launch_bounds__(kThreads, 5) adjust_logits_kernel(AdjustArgs a
 
 }  // namespace lmsf
 
-// logits, out: float32 [n_rows, vocab] (the same memory, or apart).  Every option may be null.
+// logits, out: float32 [n_rows, vocab] (the same memory, or apart).  Every option may be null; n_reqs -1: there are neither penalties nor biases.
 LMSF_API int lmsf_adjust_logits(float* out, long long out_stride, const float* logits, long long stride, int n_rows, int vocab,
                                 const int* row_req, int n_reqs, const int* history, long long history_stride, int history_width,
                                 const int* history_len, const int* prompt_len, const float* presence, const float* frequency,

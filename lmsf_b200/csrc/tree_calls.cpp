@@ -317,7 +317,7 @@ PyObject* adjust_logits(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const c10::cuda::CUDAGuard guard(r.device());
     if (!some) return kNothing;
     return launch(out->data_ptr(), std::max(out->stride(0), vocab), logits->data_ptr(), std::max(logits->stride(0), vocab), fits(rows, what), fits(vocab, what), data(row_req),
-                  fits(R, what), data(history), history ? history->stride(0) : 0, history ? fits(history->size(1), what) : 0, data(length), data(prompt), data(presence),
+                  presence || b_start ? fits(R, what) : -1, data(history), history ? history->stride(0) : 0, history ? fits(history->size(1), what) : 0, data(length), data(prompt), data(presence),
                   data(frequency), data(repetition), data(tokens), data(mask), data(cu_q), mask ? fits(mask->size(1), what) : 0, data(b_start), data(b_token), data(b_value),
                   b_token ? fits(b_token->size(0), what) : 0, data(bits), data(which), bits ? fits(bits->size(0), what) : 0, bits ? fits(words, what) : 0, data(flag),
                   c10::cuda::getCurrentCUDAStream().stream());

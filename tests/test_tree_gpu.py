@@ -871,3 +871,20 @@ def test_attention_hides_infinities_behind_a_far_window(dtype):
         assert inf == ([col + 64 * h for h in range(4)] if p - window < place else []) and not torch.isnan(out[t]).any()
     c["cache"][c["table"][0][place // 16], 1, :, place % 16, col] = 0.25
     check_attention(c, call_attention(c))
+
+
+# ----------------------------------------------------------------------------- options that are there for nobody
+
+@pytest.mark.parametrize("option", ["penalties", "bias", "masks"])
+def test_adjust_reports_options_of_no_request(option):
+    """Penalties or biases of no request, masks of which there is none: a row that asks for one is reported and passes, one that asks for no mask is not."""
+    from lmsf_b200 import kernels
+    none = torch.zeros(0, device=D)
+    kw = dict(penalties=dict(penalties=(none, none, none)), bias=dict(bias=(ints([0]), ints([]), none)), masks=dict(allowed=(ints([]).reshape(0, 4), ints([-1, 0, -1]))))[option]
+    x, f = torch.randn((3, 100), device=D), flag()
+    out = torch.empty_like(x)
+    kernels.adjust_logits(out, x, row_req=ints([0, 0, 0]), error_flag=f, **kw)
+    assert f.item() == 5 and out.equal(x)
+    f.zero_()
+    kernels.adjust_logits(out, x, row_req=ints([5, -1, 0]), allowed=(ints([]).reshape(0, 4), ints([-1, -1, -1])), error_flag=f)
+    assert f.item() == 0 and out.equal(x)
