@@ -888,3 +888,80 @@ def test_adjust_reports_options_of_no_request(option):
     f.zero_()
     kernels.adjust_logits(out, x, row_req=ints([5, -1, 0]), allowed=(ints([]).reshape(0, 4), ints([-1, -1, -1])), error_flag=f)
     assert f.item() == 0 and out.equal(x)
+
+
+# ----------------------------------------------------------------------------- forms of a call that large steps and views of buffers take
+
+@pytest.mark.parametrize("vocab,requests,nodes,width", [(210, 310, 31, 12), (40, 3900, 9, 6), (2100, 160, 31, 12)])
+@pytest.mark.parametrize("order", ["in order", "shuffled", "strangers"])
+def test_adjust_of_several_rows_a_block(vocab, requests, nodes, width, order):
+    """So many rows that a block takes two (4,736 chunks and more) or eight (18,944) in turn, with every option: what is marked for a request is kept over its rows, and
+    made anew where the next row is another's, in the middle of a block too.  Strangers: rows between those of one request that ask for one beyond the tensors; they pass with their mask alone."""
+    from lmsf_b200 import kernels
+    rng = random.Random(vocab)
+    lens = [rng.choice([nodes, nodes - 1, nodes // 2, 1, nodes]) for _ in range(requests)]
+    short = {210: 4736, 40: 18944, 2100: 2368}[vocab] - sum(lens)
+    lens += [nodes] * max(0, -(-short // nodes))
+    logits, host, dev = adjust_case(vocab, vocab, lens, width=width)
+    rows, seq = sum(lens), list(host["row_req"])
+    host["allowed"][1][:] = [w if r % 6 == 0 else -1 for r, w in enumerate(host["allowed"][1])]
+    if order == "shuffled":                                       # (bits of a row's mask are places in its request's tree, whichever that is)
+        for at in range(0, rows, 5):
+            part = seq[at:at + 5]
+            rng.shuffle(part)
+            seq[at:at + 5] = part
+    host["row_req"], asked, strange = seq, list(seq), []
+    if order == "strangers":
+        strange = list(range(3, rows, 7))
+        for r in strange:
+            asked[r] = len(lens) + r % 3 if r % 2 else -1 - r % 3
+    dev["row_req"], dev["allowed"] = ints(asked), (dev["allowed"][0], ints(host["allowed"][1]))
+    f, out = flag(), torch.full_like(logits, 7.0)
+    kernels.adjust_logits(out, logits, error_flag=f, **dev)
+    assert f.item() == (5 if strange else 0)
+    plain = [r for r in range(rows) if r not in set(strange)]
+    some = [r for r in plain if vocab != 40 or r % 3 == 0]       # (the plain loops are slow: of the most rows every third)
+    tokens, mask, cu = host["tree"]
+    want_host = dict(host, row_req=[seq[r] for r in some], tree=(tokens, mask[some], cu), allowed=(host["allowed"][0], [host["allowed"][1][r] for r in some]))
+    check_adjusted(out[some], logits[some], want_host)
+    if strange:
+        want, _ = P.adjust(logits[strange], [0] * len(strange), allowed=(host["allowed"][0], [host["allowed"][1][r] for r in strange]))
+        assert out[strange].cpu().double().equal(want)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "bf16 on the CUDA cores"])
+@pytest.mark.parametrize("hd,heads,kvh", [(64, 8, 2), (128, 4, 2), (112, 6, 6), (33, 4, 2)])
+@pytest.mark.parametrize("lens,prefix", [([37, 5, 64], [0, 0, 0]), ([40, 3], [900, 130])])
+@pytest.mark.parametrize("first,more", [(3, 7), (1, 16), (8, 16), (0, 9)])
+def test_attention_into_columns_of_a_buffer(dtype, hd, heads, kvh, lens, prefix, first, more, monkeypatch):
+    """The output as columns of wider rows, at every alignment, of units that one block finishes and of those that are joined; what lies around it is left alone."""
+    c = attention_case(hd + first, lens, prefix, heads, kvh, hd, 16, on_cores(monkeypatch, dtype), spare_rows=2)
+    n, w = c["q"].shape[0], heads * hd
+    wide = torch.full((n, w + more), 7.0, dtype=c["dtype"], device=D)
+    out = wide[:, first:first + w]
+    call_attention(c, out)
+    check_attention(c, out)
+    assert (wide[:, :first] == 7.0).all() and (wide[:, first + w:] == 7.0).all()
+
+
+@pytest.mark.parametrize("what", ["q", "k", "v", "rows of k", "cache", "negative", "zero", "group"])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_that_the_tensor_cores_do_not_take(what, hd):
+    """bfloat16 of their head sizes, but rows off 16 bytes, a scale that is not positive, more than 128 heads a group."""
+    heads, kvh = (129, 1) if what == "group" else (8, 2)
+    c = attention_case(hd, [20, 3], [200, 70], heads, kvh, hd, 16, "bf16")
+    if what in ("q", "k", "v"):
+        wide = torch.zeros((c[what].shape[0], c[what].shape[1] + 8), dtype=torch.bfloat16, device=D)
+        wide[:, 1:-7] = c[what]
+        c[what] = wide[:, 1:-7]
+    elif what == "rows of k":
+        wide = torch.zeros((c["k"].shape[0], c["k"].shape[1] + 3), dtype=torch.bfloat16, device=D)
+        wide[:, :-3] = c["k"]
+        c["k"] = wide[:, :-3]
+    elif what == "cache":
+        line = torch.zeros(c["cache"].numel() + 1, dtype=torch.bfloat16, device=D)
+        line[1:] = c["cache"].flatten()
+        c["cache"] = line[1:].view(c["cache"].shape)
+    elif what != "group":
+        c["scale"] = -0.07 if what == "negative" else 0.0
+    check_attention(c, call_attention(c))
