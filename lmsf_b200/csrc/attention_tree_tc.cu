@@ -5,9 +5,10 @@
 // kv head (nodes x heads of the group) the kernel is bound by their bytes, above by the tensor cores and the exponentials.  What holds it
 // from both is the way of one tile: scores, their maximum, weights, the product with v and the next scores follow one another, some 3,100 cycles for a tile of two
 // items where their products take 2,048, and the first tile of a block has its way from memory before it.
-// Measured (captured in a graph, other inputs in every launch): 64 requests of 33..64 nodes behind 2,048..4,096 keys, 32 heads of 128 over 8: 226 us, 685 TFLOP/s
-// (of 1,628 that a library product reaches); 2 of 48 behind 24,000..32,000: 80 us, 600 TFLOP/s and 3.1 TB/s; 8 of 32 behind 2,047: 27.5 us, 2.6 TB/s (of 6.55); 27 of 1..64 behind
-// 130..2,300, 32 heads of 64 over 8: 40.5 us; one of 8 behind 97: 10.7 us.
+// Measured (captured in a graph, other inputs in every launch): 64 requests of 33..64 nodes behind 2,048..4,096 keys, 32 heads of 128 over 8: 225 us, 688 TFLOP/s
+// (of 1,628 that a library product reaches); 2 of 48 behind 24,000..32,000: 80 us, 600 TFLOP/s and 3.1 TB/s; 8 of 32 behind 2,047: 27.7 us, 2.6 TB/s (of 6.55); 27 of 1..64 behind
+// 130..2,300, 32 heads of 64 over 8: 40.9 us; one of 8 behind 97: 10.2 us.  A window that hides nothing takes 0.2 to 0.6 us more than
+// none (the rows' positions are read for its edge), one that does takes tiles away: 8 of 32 behind 2,047 with a window of 64 13.0 us, of 1,024 23.8.
 //
 // An item is up to 128 rows: 128 / group nodes x the heads of the group, which one copy brings into shared memory node-major.  A
 // block works on pieces of units (a request, a kv head, two items; see attention_tree.cuh) with 128 keys a tile:
